@@ -26,6 +26,10 @@ struct ocr_ctx {
     // scratch of the low-level ops (grown on demand, freed with the context)
     void* op_scratch = nullptr;
     size_t op_scratch_bytes = 0;
+    // partial results and tickets of the attentions over a caller's KV cache: the tickets are zero between calls, so
+    // no other op writes here (grown on demand, freed with the context)
+    void* kv_work = nullptr;
+    size_t kv_work_bytes = 0;
     // pinned staging for uploads
     void* h_stage = nullptr;
     void* d_stage = nullptr;

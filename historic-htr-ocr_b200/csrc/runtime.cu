@@ -1236,6 +1236,7 @@ void ocr::ctx_release(ocr_ctx* c) {
     cudaSetDevice(c->device);
     cudaStreamSynchronize(c->stream);
     if (c->op_scratch) cudaFree(c->op_scratch);
+    if (c->kv_work) cudaFree(c->kv_work);
     if (c->h_stage) cudaFreeHost(c->h_stage);
     if (c->d_stage) cudaFree(c->d_stage);
     if (c->d_err) cudaFree(c->d_err);
@@ -1608,6 +1609,15 @@ ocr_status ocr_session_kv(const ocr_session* s, int layer, int slot, int row0, i
         OCR_CUDA(cudaMemcpy2D(v_out + (size_t)j * 128, row_bytes, s->vcl(layer) + src, 256, 256, n_rows,
                               cudaMemcpyDeviceToHost));
     }
+    return OCR_OK;
+}
+
+ocr_status ocr_session_kv_cache(const ocr_session* s, int layer, ocr_kv_cache* out) {
+    if (!s || !out) return fail(OCR_ERR_ARG, "null argument");
+    const auto& c = s->m->cfg;
+    if (layer < 0 || layer >= c.n_layer) return fail(OCR_ERR_ARG, "layer out of range");
+    *out = ocr_kv_cache{OCR_KV_F16,      s->B, c.n_kv, 128, s->n_ctx, 0, 0, 0, s->kcl(layer), s->vcl(layer),
+                        nullptr, nullptr};
     return OCR_OK;
 }
 

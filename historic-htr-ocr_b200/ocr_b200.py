@@ -66,6 +66,17 @@ class Page(C.Structure):
                 ("n_out", C.c_int32)]
 
 
+class KvCacheC(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("type", "n_slot", "n_kv", "d_head", "n_rows", "window", "sinks", "ring")] + \
+        [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")]
+
+
+class Rows(C.Structure):
+    """ocr_rows: vectors of d_head consecutive elements, slot b, row t, head h at the given strides"""
+    _fields_ = [("data", C.c_void_p), ("half", C.c_int32)] + \
+        [(n, C.c_int64) for n in ("slot_stride", "row_stride", "head_stride")]
+
+
 PAGE_CB = C.CFUNCTYPE(C.c_int, C.c_void_p, C.POINTER(Page))
 
 
@@ -134,6 +145,15 @@ _SIGS = {
                                         _P]),
     "ocr_op_lm_head_sample_noalloc": (C.c_int, [_P, _P, C.c_int, C.c_int, _P, _P, C.c_float, C.c_float, C.c_int, _P,
                                                 _P, _P, _P]),
+    "ocr_kv_cache_bytes": (C.c_int, [C.POINTER(KvCacheC), C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]),
+    "ocr_session_kv_cache": (C.c_int, [_P, C.c_int, C.POINTER(KvCacheC)]),
+    "ocr_op_kv_write": (C.c_int, [_P, C.POINTER(KvCacheC), C.POINTER(Rows), C.POINTER(Rows), C.c_int, _P, _P]),
+    "ocr_op_kv_read": (C.c_int, [_P, C.POINTER(KvCacheC), C.POINTER(Rows), C.POINTER(Rows), C.c_int, _P, _P]),
+    "ocr_op_attention_window": (C.c_int, [_P, C.POINTER(KvCacheC), C.POINTER(Rows), C.c_int, C.c_int, _P, _P, C.c_float,
+                                          C.POINTER(Rows)]),
+    "ocr_op_attention_tree": (C.c_int, [_P, C.POINTER(KvCacheC), C.POINTER(Rows), C.c_int, C.c_int, _P, _P, _P,
+                                        C.c_float, C.POINTER(Rows)]),
+    "ocr_op_kv_keep": (C.c_int, [_P, C.POINTER(KvCacheC), C.c_int, C.c_int, _P, _P, _P]),
     "ocr_op_wait_probe": (C.c_int, [_P, C.c_int, C.POINTER(C.c_int)]),
     "ocr_op_attention_full": (C.c_int, [_P, _P, C.c_int, C.c_int, C.c_int, _P, _P, C.c_int, C.c_int, C.c_float, _P,
                                         C.c_int]),
@@ -472,6 +492,12 @@ class Session:
         _check(lib().ocr_session_kv(self.h, layer, slot, row0, n_rows, _ptr(k), _ptr(v)))
         return k, v
 
+    def kv_cache(self, layer: int) -> "KvCache":
+        """a layer's KV rows, live, as an f16 cache for the op_kv_* and op_attention_* calls"""
+        c = KvCacheC()
+        _check(lib().ocr_session_kv_cache(self.h, layer, C.byref(c)))
+        return KvCache._of(c, (self,))
+
     def prefill(self, slot: int = 0, ids: Optional[Sequence[int]] = None, embd: Optional[np.ndarray] = None,
                 logits: bool = True) -> Optional[np.ndarray]:
         """rows: ids[i] >= 0 → token, else embedding row i of embd ([n][dim] f32: a host array, or a device tensor
@@ -759,6 +785,123 @@ def attention_tiles(k: np.ndarray, v: np.ndarray, n_pad: int) -> tuple[np.ndarra
             dst = ((q ^ (r & 7)) * 8)[:, None] + np.arange(8)[None, :]
             vt[:, t0 // 64, r[:, None], dst] = vtb[:, :, 8 * q:8 * q + 8]
     return kt.view(np.uint16), vt.view(np.uint16)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# a KV cache in fewer bits, attention within a window, trees of drafts (the caller's device memory)
+# ---------------------------------------------------------------------------------------------------------------------
+KV_TYPES = {"f16": 1, "q4_0": 2, "q8_0": 8}
+_KV_ITEM = {1: 2.0, 2: 0.5, 8: 1.0}
+
+
+class KvCache:
+    """A view of one layer's cache (ocr_kv_cache): k, v [n_slot][n_kv][n_rows][row bytes] and, for q8_0 and q4_0, the
+    f16 scales [n_slot][n_kv][n_rows][d_head / 32], contiguous device tensors that this view keeps alive. window 0: every
+    position is seen; ring: the rows from `sinks` on are used round and round."""
+
+    def __init__(self, type: str, k, v, k_scale=None, v_scale=None, d_head: int = 128, window: int = 0, sinks: int = 0,
+                 ring: bool = False):
+        if type not in KV_TYPES:
+            raise OcrError(1, f"KV cache type {type!r}: one of {', '.join(KV_TYPES)}")
+        t = KV_TYPES[type]
+        lead = tuple(k.shape[:3])
+        for x, width in ((k, int(d_head * _KV_ITEM[t])), (v, int(d_head * _KV_ITEM[t])), (k_scale, d_head // 16),
+                         (v_scale, d_head // 16)):
+            if x is None and t == 1:
+                continue
+            if x is None or tuple(x.shape[:3]) != lead or x.dim() != 4 or not x.is_contiguous() or \
+                    x.shape[3] * x.element_size() != width:
+                raise OcrError(1, "KV cache tensors must be contiguous [n_slot][n_kv][n_rows][row], rows of d_head")
+        self.c = KvCacheC(t, *lead[:2], d_head, lead[2], window, sinks, int(ring), _ptr(k), _ptr(v),
+                          None if t == 1 else _ptr(k_scale), None if t == 1 else _ptr(v_scale))
+        self._keep = (k, v, k_scale, v_scale)
+
+    @classmethod
+    def _of(cls, c: KvCacheC, keep: tuple) -> "KvCache":
+        v = cls.__new__(cls)
+        v.c, v._keep = c, keep
+        return v
+
+    def nbytes(self) -> tuple[int, int]:
+        """the bytes of k (or v) and of k_scale (or v_scale)"""
+        return kv_cache_bytes(self.c)
+
+
+def kv_cache_bytes(c: KvCacheC) -> tuple[int, int]:
+    q, s = C.c_size_t(), C.c_size_t()
+    _check(lib().ocr_kv_cache_bytes(C.byref(c), C.byref(q), C.byref(s)))
+    return q.value, s.value
+
+
+def rows_of(t, cache: KvCache, heads: Optional[int] = None) -> Rows:
+    """a device tensor [n_slot][rows][heads][d_head], f32 or f16, of any strides but the last → ocr_rows"""
+    shape, stride, item = t.shape, t.stride(), t.element_size()
+    c = cache.c
+    if len(shape) != 4 or shape[0] != c.n_slot or shape[3] != c.d_head or stride[3] != 1 or \
+            (heads is not None and shape[2] != heads) or not t.is_floating_point() or \
+            str(t.dtype) not in ("torch.float32", "torch.float16"):
+        raise OcrError(1, "rows must be an f32 or f16 tensor [n_slot][rows][heads][d_head], d_head contiguous")
+    return Rows(t.data_ptr(), int(item == 2), *(s if n > 1 else 0 for s, n in zip(stride[:3], shape)))
+
+
+def _ints(t, *shape) -> Optional[int]:
+    if t is None:
+        return None
+    if tuple(t.shape) != shape or str(t.dtype) != "torch.int32" or not t.is_contiguous():
+        raise OcrError(1, f"positions, counts, parents and paths are contiguous int32 device tensors, here {list(shape)}")
+    return t.data_ptr()
+
+
+def op_kv_write(ctx: Context, cache: KvCache, k, v, pos, n=None) -> None:
+    """rows of keys and values [n_slot][rows][n_kv][d_head] → the cache, from position pos[slot] on (below 0: idle),
+    n[slot] of them in use"""
+    c = cache.c
+    if k.shape != v.shape:
+        raise OcrError(1, "k and v must be of one shape")
+    _check(lib().ocr_op_kv_write(ctx.h, C.byref(c), C.byref(rows_of(k, cache, c.n_kv)),
+                                 C.byref(rows_of(v, cache, c.n_kv)), k.shape[1], _ints(pos, c.n_slot),
+                                 _ints(n, c.n_slot)))
+
+
+def op_kv_read(ctx: Context, cache: KvCache, k, v, pos, n=None) -> None:
+    """the cache's rows → values in k and v; rows that are not in use are zeros"""
+    c = cache.c
+    if k.shape != v.shape:
+        raise OcrError(1, "k and v must be of one shape")
+    _check(lib().ocr_op_kv_read(ctx.h, C.byref(c), C.byref(rows_of(k, cache, c.n_kv)),
+                                C.byref(rows_of(v, cache, c.n_kv)), k.shape[1], _ints(pos, c.n_slot),
+                                _ints(n, c.n_slot)))
+
+
+def op_attention_window(ctx: Context, cache: KvCache, q, out, pos, scale: float, n=None) -> None:
+    """rows q [n_slot][rows][n_head][d_head], which the cache already holds from pos[slot] on, attend it: causal, within
+    the cache's window and sinks"""
+    c = cache.c
+    if q.shape != out.shape:
+        raise OcrError(1, "q and out must be of one shape")
+    _check(lib().ocr_op_attention_window(ctx.h, C.byref(c), C.byref(rows_of(q, cache)), q.shape[2], q.shape[1],
+                                         _ints(pos, c.n_slot), _ints(n, c.n_slot), scale,
+                                         C.byref(rows_of(out, cache))))
+
+
+def op_attention_tree(ctx: Context, cache: KvCache, q, out, pos, parent, scale: float, n=None) -> None:
+    """the same for a tree of drafts: parent [n_slot][rows], parent[i] < i, -1 for a child of the last committed
+    position"""
+    c = cache.c
+    if q.shape != out.shape:
+        raise OcrError(1, "q and out must be of one shape")
+    _check(lib().ocr_op_attention_tree(ctx.h, C.byref(c), C.byref(rows_of(q, cache)), q.shape[2], q.shape[1],
+                                       _ints(pos, c.n_slot), _ints(n, c.n_slot), _ints(parent, c.n_slot, q.shape[1]),
+                                       scale, C.byref(rows_of(out, cache))))
+
+
+def op_kv_keep(ctx: Context, caches: Sequence[KvCache], pos, path, n) -> None:
+    """the accepted drafts' rows move together in every layer's cache: position pos + path[i] → pos + i, i < n[slot]"""
+    c = caches[0].c
+    rows = path.shape[1]
+    arr = (KvCacheC * len(caches))(*[x.c for x in caches])
+    _check(lib().ocr_op_kv_keep(ctx.h, arr, len(caches), rows, _ints(pos, c.n_slot), _ints(path, c.n_slot, rows),
+                                _ints(n, c.n_slot)))
 
 
 def op_wait_probe(ctx: Context, tries: int) -> bool:

@@ -297,6 +297,70 @@ ocr_status ocr_op_attention_decode(ocr_ctx* ctx, float* d_qkv, const float* d_q_
                                    const float* d_rope, uint16_t* d_k_cache, uint16_t* d_v_cache, int n_head, int n_kv,
                                    int n_ctx, int pos, float eps, float* d_out);
 
+/* ---- a KV cache in fewer bits, attention within a window, trees of drafts ----------------------------------------- */
+/* Operators over ONE layer's KV cache in the caller's device memory (the reference keeps an f16 cache per layer,
+ * Session, app/crates/ocr-wgpu/src/text.rs:242-328, and has no counterpart of the rest). All run on the context's
+ * stream and return when queued; memory that another stream wrote needs an order against ocr_ctx_stream's stream. The
+ * rows' positions and counts are device memory, so a captured step can be replayed as the sequences grow; what is
+ * wrong with them shows as OCR_ERR_DEVICE at the next ocr_ctx_sync, and the slot concerned is left alone. */
+enum { OCR_KV_F16 = 1, OCR_KV_Q4_0 = 2, OCR_KV_Q8_0 = 8 }; /* ggml's type numbers */
+/* k and v: quants [n_slot][n_kv][n_rows][row bytes], 16-byte aligned; k_scale and v_scale: f16 [n_slot][n_kv][n_rows]
+ * [d_head / 32], 8-byte aligned (null for OCR_KV_F16). A row holds d_head values (64 or 128):
+ *   OCR_KV_F16   d_head f16;
+ *   OCR_KV_Q8_0  d_head int8: value = q * scale of its block of 32;
+ *   OCR_KV_Q4_0  d_head / 2 bytes, byte j of a block's 16 holding value j in its low nibble and value j + 16 in its
+ *                high one: value = (nibble - 8) * scale.
+ * Position p is held by row p. With ring != 0 (needs window > 0) the rows from `sinks` on are used round and round:
+ * position p >= sinks is held by row sinks + (p - sinks) % (n_rows - sinks), and positions have no end.
+ * window > 0: a row at position p sees the last `window` positions up to p, and the first `sinks`; 0: every one. */
+typedef struct {
+    int32_t type, n_slot, n_kv, d_head, n_rows, window, sinks, ring;
+    void *k, *v;
+    uint16_t *k_scale, *v_scale;
+} ocr_kv_cache;
+/* vectors of d_head consecutive elements (f32, or f16 if half != 0): slot b, row t, head h at element
+ * b * slot_stride + t * row_stride + h * head_stride of data. data and the strides in bytes are multiples of 16. */
+typedef struct {
+    void* data;
+    int32_t half;
+    int64_t slot_stride, row_stride, head_stride;
+} ocr_rows;
+/* the bytes that k and v (each) and k_scale and v_scale (each) take, for the cache's shape */
+ocr_status ocr_kv_cache_bytes(const ocr_kv_cache* c, size_t* quants, size_t* scales);
+/* a layer of a live session as such a cache (f16, the session's memory): valid as long as the session. Positions up to
+ * the slot's n_past hold its rows; the session does not see what is written there. */
+ocr_status ocr_session_kv_cache(const ocr_session* s, int layer, ocr_kv_cache* out);
+/* Every call below takes `rows` rows of each slot, from position d_pos[slot] on (device int32 [n_slot]; below 0: the
+ * slot is idle), d_n[slot] of them in use (device int32 [n_slot]; null: all). Rows that are not in use are not written
+ * to the cache, and are zeros in an output. A slot whose rows do not fit the cache is flagged and treated as idle. In
+ * a ring cache rows is at most n_rows - sinks - window + 1: more would overwrite what the first of them sees. */
+/* rows of keys and values → the cache, quantised per block of 32 as ggml's reference quantisers do: q8_0 with
+ * scale = f16(max|x| / 127) and q = x / scale before its rounding to f16, to the nearest, halves away from zero; q4_0
+ * with scale = f16(m / -8), m the first value of the largest magnitude. A block with an infinity or a NaN, or whose
+ * scale passes f16's range, reads back as NaN. */
+ocr_status ocr_op_kv_write(ocr_ctx* ctx, const ocr_kv_cache* c, const ocr_rows* k, const ocr_rows* v, int rows,
+                           const int32_t* d_pos, const int32_t* d_n);
+/* the cache's rows → values */
+ocr_status ocr_op_kv_read(ocr_ctx* ctx, const ocr_kv_cache* c, const ocr_rows* k, const ocr_rows* v, int rows,
+                          const int32_t* d_pos, const int32_t* d_n);
+/* softmax(q k^T * scale) v of the rows, which the cache already holds, over the positions each sees: up to its own,
+ * within the window, the sinks. n_head query heads, head h reading kv head h / (n_head / n_kv). A row that
+ * sees nothing gives zeros; what a row does not see has no part in it, not even a NaN. A NaN that a row sees, in a key
+ * or a value, or an infinite value, leaves its output without a finite value there. */
+ocr_status ocr_op_attention_window(ocr_ctx* ctx, const ocr_kv_cache* c, const ocr_rows* q, int n_head, int rows,
+                                   const int32_t* d_pos, const int32_t* d_n, float scale, const ocr_rows* out);
+/* the same for a tree of at most 64 drafted tokens per slot: row i, held at position d_pos + i, stands at position
+ * d_pos + its depth. d_parent (device int32 [n_slot][rows]): d_parent[i] < i, or -1 for a child of the last committed
+ * position (depth 0). A row sees the committed positions, its ancestors and itself, within the window. */
+ocr_status ocr_op_attention_tree(ocr_ctx* ctx, const ocr_kv_cache* c, const ocr_rows* q, int n_head, int rows,
+                                 const int32_t* d_pos, const int32_t* d_n, const int32_t* d_parent, float scale,
+                                 const ocr_rows* out);
+/* After the drafts are judged: the accepted path's rows move together. In each of n_layer caches of one shape (at most
+ * 64), the row of position d_pos + d_path[i] becomes that of d_pos + i for i < d_n[slot]; d_path (device int32
+ * [n_slot][rows]) rises strictly. The committed length is then d_pos + d_n. */
+ocr_status ocr_op_kv_keep(ocr_ctx* ctx, const ocr_kv_cache* caches, int n_layer, int rows, const int32_t* d_pos,
+                          const int32_t* d_path, const int32_t* d_n);
+
 /* Test hook for the device's bounded waits (the reference's Health rule, app/crates/ocr-wgpu/src/gpu.rs:901-970: a
  * device failure becomes an error, not a hang). Every kernel waits on mbarriers for at most a fixed number of polls,
  * then flags an error and skips the work. This runs one such wait that cannot complete, limited to `tries` polls of
