@@ -1,109 +1,778 @@
-// k_kv_attn.cu — attention of rows over a KV cache (kv.cuh): causal or a tree of drafts, within a sliding window, the
-// first `sinks` positions always visible.
+// k_kv_attn.cu — attention of a few rows per kv head (a decode step, a small tree of drafts) over a KV cache (kv.cuh).
 //
 // out[t] = sum_p softmax_p(scale q_t . k_p) v_p over the visible positions p: p <= pos + t, and with a window also
 // p > pos + t - window or p < sinks. Drafts (a parent for each row): row t stands at position pos + depth(t) and sees
 // the committed positions and, of the drafts, its ancestors and itself. A row that sees nothing gives zeros.
 //
-// The simple form: one warp per (slot, row, head), a key at a time, lane i holding dims i, i + 32, …
+// Bound: memory — each visible row of the cache is read once for all rows of the call. The work is cut evenly: the key
+// tiles of all (slot, kv head) pairs form one line, CTA c of C takes the c-th part of it, its warps take the tiles in
+// turn, whatever the lengths. A pair that lies in several CTAs is joined by the last of them to arrive (a ticket; the
+// parts are added in the order of the CTAs, so the result does not depend on who is last). Each warp streams its tiles
+// through a ring of its own with asynchronous copies and needs no barrier with the others; the ring runs on into the
+// next pair while one is joined.
+//
+// Products: warp-level tensor-core products m16n8k16 (f16 in, f32 out) with the keys as the 16 rows and up to eight
+// (row, query head) pairs as the columns: S = K Q^T, then O = V^T P with the dims as the rows. A decode step has no use
+// for the 128-row tcgen05 shapes, and the operands here come out of registers, where the quants become f16 — no pass
+// through shared memory. Exactness: q8_0 and q4_0 quants are integers and exact in f16; a key's block scale multiplies
+// the block's f32 partial score, a value's block scale goes into P (one P per block of 32 dims). f32 queries, and P,
+// are split into f16 hi + lo (22 bits); f16 queries are exact, and P is rounded to f16 like the output. A row's query
+// is scaled by a power of two so that its lo part does not fall below f16's range, P likewise by the tile's largest
+// scale.
 #include "kv.cuh"
 
 namespace ocr {
 
-template <int TYPE>
-__device__ __forceinline__ float kv_value(const uint8_t* q, const __half* s, size_t row, int d, int i) {
-    if (TYPE == KV_F16) return __half2float(reinterpret_cast<const __half*>(q)[row * d + i]);
-    const float scale = __half2float(s[row * (d / KV_BLOCK) + i / KV_BLOCK]);
-    if (TYPE == KV_Q8_0) return (float)reinterpret_cast<const int8_t*>(q)[row * d + i] * scale;
-    const int j = i % KV_BLOCK;
-    const uint8_t w = q[row * (d / 2) + i / KV_BLOCK * 16 + j % 16];
-    return ((float)(j < 16 ? w & 15 : w >> 4) - 8.0f) * scale;
+constexpr int KA_WARPS = 8;
+constexpr int KA_THREADS = KA_WARPS * 32;
+constexpr int KA_SLOTS = 512;        // slots of one launch (the line's prefix sums are in shared memory)
+constexpr int KA_TICKETS = 4096;     // bytes before the partial results: a ticket per CTA
+constexpr int KA_RING = 26112;       // a warp's share of the rings: three q8_0 tiles of 32 keys
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <int TYPE, int D>
+struct KaTile {
+    static constexpr int ROW = kv_row_bytes(TYPE, D);
+    static constexpr int NB = TYPE == KV_F16 ? 0 : D / KV_BLOCK;
+    static constexpr int KEYS = TYPE == KV_F16 ? 2048 / D : TYPE == KV_Q8_0 ? 4096 / D : D == 128 ? 32 : 64;
+    static constexpr int K_BYTES = KEYS * ROW, S_BYTES = KEYS * NB * 2;
+    static constexpr int STAGE = 2 * (K_BYTES + S_BYTES);  // K, V, K scales, V scales
+    static constexpr int STAGES = KA_RING / STAGE;         // per warp
+    // the byte offset of 16-byte piece c of key i: permuted so that the eight (K) or four (V) keys that a warp reads at
+    // once lie in different banks
+    __device__ static __forceinline__ int off(int i, int c, bool v) {
+        if (TYPE == KV_F16) return i * ROW + ((c ^ (i & 7)) << 4);
+        if (TYPE == KV_Q8_0 && D == 128)
+            return i * ROW + ((c ^ ((v ? (i >> 2) & 3 : (i & 1) | ((i >> 1) & 2)) << 1)) << 4);
+        if (TYPE == KV_Q8_0) return (i ^ ((i >> 3) & 1)) * ROW + ((c ^ (((i >> 2) & 1) << 1)) << 4);
+        if (D == 128) return i * ROW + ((c ^ ((i >> 2) & 3)) << 4);
+        return (i ^ (((i >> 3) & 1) << 1)) * ROW + ((c ^ ((i >> 2) & 1)) << 4);
+    }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// the remainders of a and b past their f16 rounding `hi`
+__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t hi) {
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    return pack2(a - h.x, b - h.y);
+}
+__device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix4(uint32_t* r, uint32_t addr) {
+    if (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(addr));
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(addr));
+}
+template <int N>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool live) {
+    const int n = live ? N : 0;  // the rest is filled with zeros
+    if (N == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// an unsigned byte pair placed as halves of 1024 + u, less `bias`
+__device__ __forceinline__ uint32_t bytes_h2(uint32_t w, uint32_t sel, uint32_t bias) {
+    const uint32_t m = __byte_perm(w, 0x64646464u, sel);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&m), *reinterpret_cast<const __half2*>(&bias));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+constexpr uint32_t H2_1152 = 0x64806480u;  // 1024 + 128: an int8 with its sign bit flipped
+// the low (SHIFT = 0) or high nibbles of bytes 0 and 2 of w, less 8
+template <bool HIGH>
+__device__ __forceinline__ uint32_t nibbles_h2(uint32_t w) {
+    const uint32_t m = (w & (HIGH ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;  // 1024 + n, or 1024 + 16 n
+    const __half2 x = *reinterpret_cast<const __half2*>(&m);
+    __half2 r;
+    if (HIGH)
+        r = __hfma2(x, __float2half2_rn(0.0625f), __float2half2_rn(-72.0f));
+    else
+        r = __hsub2(x, __float2half2_rn(1032.0f));
+    return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-template <int TYPE, int D, class T>
-__global__ void __launch_bounds__(128) k_kv_attn_simple(KvAttnArgs a) {
+// one (slot, kv head) pair's visible keys, in order: the sinks that lie before the window, then positions lo … end - 1
+struct KaSpan {
+    int pos, m, lo, ns, nv;  // rows in use, first position of the window, sinks before it, keys
+    __device__ __forceinline__ void set(const KvAttnArgs& a, int b) {
+        pos = a.r.pos[b];
+        m = a.r.rows(a.c, b, a.err);
+        lo = a.c.window ? max(0, pos - a.c.window + 1) : 0;
+        ns = min(a.c.sinks, lo);
+        nv = m ? ns + pos + m - lo : 0;
+    }
+    __device__ __forceinline__ int position(int v) const { return v < ns ? v : lo + v - ns; }
+};
+
+// where a CTA stands in the line of tiles
+struct KaCursor {
+    int b, h, first, tiles;  // the pair, its first tile in the line, its tiles
+    __device__ __forceinline__ void at(int g, const int* prefix, int n_slot, int n_kv) {  // the pair of tile g
+        int lo = 0, hi = n_slot;  // prefix[lo] <= g < prefix[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (prefix[mid] <= g)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        b = lo;
+        tiles = (prefix[b + 1] - prefix[b]) / n_kv;
+        h = (g - prefix[b]) / tiles;
+        first = prefix[b] + h * tiles;
+    }
+};
+
+template <int TYPE, int D, int WR, class T>
+__global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant__ KvAttnArgs a) {
+    using KT = KaTile<TYPE, D>;
+    constexpr bool LO = sizeof(T) == 4;          // the lo halves of q and P
+    constexpr int TEAMS = KA_WARPS / WR;         // WR warps share a ring, eight rows each
+    constexpr int STAGES = KT::STAGES * WR;
+    constexpr int KEYS = KT::KEYS, MT = KEYS / 16, NB = KT::NB;
+    constexpr int KSTEPS = D / 16, DT = D / 16;  // 16-dim steps of S, 16-dim tiles of O
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int prefix[KA_SLOTS + 1];
+    __shared__ int wsum[KA_WARPS];
+    __shared__ int s_at[8 * WR], s_depth[KV_TREE_MAX];
+    __shared__ uint64_t s_anc[8 * WR];
+    __shared__ float s_ml[KA_WARPS][16];
+    __shared__ int s_last;
     pdl_trigger();
     pdl_wait();
     const KvView& c = a.c;
-    const int lane = threadIdx.x & 31;
-    const long w = ((long)blockIdx.x * 128 + threadIdx.x) >> 5;
-    const long per_slot = (long)a.r.T * a.n_head;
-    const int b = (int)(w / per_slot);
-    if (b >= c.n_slot) return;
-    const int t = (int)(w % per_slot) / a.n_head, h = (int)(w % a.n_head);
-    const T* q = static_cast<const T*>(a.q) + b * a.q_slot + t * a.q_row + h * a.q_head;
-    T* out = static_cast<T*>(a.out) + b * a.o_slot + t * a.o_row + h * a.o_head;
-    const int n = a.r.rows(c, b, a.err);
-    if (t >= n) {
-        for (int i = lane; i < D; i += 32) out[i] = (T)0.0f;
-        return;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int team = warp / WR, wr = warp % WR, tl = tid - team * WR * 32;
+    const int G = a.n_head / c.n_kv;
+
+    // ---- the line: exclusive sums of the slots' tiles ----
+    bool idle_rows = false;
+    int total = 0;
+    for (int b0 = 0; b0 < c.n_slot; b0 += KA_THREADS) {
+        const int b = b0 + tid;
+        KaSpan s;
+        s.nv = 0;
+        if (b < c.n_slot) {
+            s.set(a, b);
+            idle_rows |= s.m < a.r.T;
+        }
+        int x = (s.nv + KEYS - 1) / KEYS * c.n_kv;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(FULL, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) wsum[warp] = x;
+        __syncthreads();
+        for (int w = 0; w < warp; w++) x += wsum[w];
+        if (b < c.n_slot) prefix[b + 1] = total + x;
+        for (int w = 0; w < KA_WARPS; w++) total += wsum[w];
+        __syncthreads();
     }
-    const int pos = a.r.pos[b];
-    const int32_t* parent = a.parent ? a.parent + (size_t)b * a.r.T : nullptr;
-    uint64_t anc = 0;
-    int at = pos + t;
-    if (parent) {
-        int depth = -1;
-        for (int i = t; i >= 0; depth++) {
-            anc |= 1ull << i;
-            const int p = parent[i];
-            if (p >= i || p < -1) {
-                dev_error(a.err, DEV_BAD_INDEX);
-                depth++;
-                break;
+    if (tid == 0) prefix[0] = 0;
+    if (__syncthreads_or(idle_rows)) {  // rows that are not in use are zeros
+        const long n = (long)c.n_slot * a.r.T * a.n_head;
+        for (long i = (long)blockIdx.x * KA_WARPS + warp; i < n; i += (long)gridDim.x * KA_WARPS) {
+            const int h = (int)(i % a.n_head), r = (int)(i / a.n_head % a.r.T), b = (int)(i / a.n_head / a.r.T);
+            if (r < a.r.rows(c, b, nullptr)) continue;
+            T* o = static_cast<T*>(a.out) + b * a.o_slot + r * a.o_row + h * a.o_head;
+            for (int d = lane; d < D; d += 32) o[d] = (T)0.0f;
+        }
+    }
+    // parts of at least a tile per team: a short line takes fewer CTAs, and fewer parts to join
+    const int n_cta = min((int)gridDim.x, (total + TEAMS - 1) / TEAMS);
+    const int cta = blockIdx.x;
+    if (cta >= n_cta) return;
+    auto part = [&](int i) { return (int)((long)total * i / n_cta); };
+    auto owner = [&](int tile) {  // the CTA whose part holds it
+        int i = (int)(((long)tile * n_cta) / total);
+        while (part(i + 1) <= tile) i++;
+        return i;
+    };
+    const int begin = part(cta), end = part(cta + 1);
+
+    uint8_t* ring = smem + team * WR * KA_RING;
+    float* joined = reinterpret_cast<float*>(smem + KA_WARPS * KA_RING);  // [4 warps][D / 4 registers][32 lanes]
+
+    // ---- the copies of a tile, by the team's threads ----
+    KaCursor lc;
+    KaSpan ls;
+    lc.at(begin, prefix, c.n_slot, c.n_kv);
+    ls.set(a, lc.b);
+    int lt = begin + team, ln = 0;  // the next tile to copy, the copies so far
+    auto load = [&]() {
+        if (lt < end) {
+            if (lt >= lc.first + lc.tiles) {
+                lc.at(lt, prefix, c.n_slot, c.n_kv);
+                ls.set(a, lc.b);
             }
-            i = p;
+            const uint32_t dst = smem_u32(ring + ln % STAGES * KT::STAGE);
+            const int v0 = (lt - lc.first) * KEYS;
+            const size_t base = kv_index(c, lc.b, lc.h, 0);
+            constexpr int PIECES = KT::ROW / 16;
+#pragma unroll
+            for (int e = 0; e < KEYS * PIECES / 32; e += WR) {
+                const int x = e * 32 + tl, i = x / PIECES, p = x % PIECES;
+                if (KEYS * PIECES % (32 * WR) && x >= KEYS * PIECES) break;
+                const bool live = v0 + i < ls.nv;
+                const size_t row = base + (live ? kv_row(c, ls.position(v0 + i)) : 0);
+                cp_async<16>(dst + KT::off(i, p, false), c.k + row * KT::ROW + p * 16, live);
+                cp_async<16>(dst + KT::K_BYTES + KT::off(i, p, true), c.v + row * KT::ROW + p * 16, live);
+            }
+            if constexpr (NB > 0) {
+                for (int i = tl; i < KEYS; i += 32 * WR) {
+                    const bool live = v0 + i < ls.nv;
+                    const size_t row = base + (live ? kv_row(c, ls.position(v0 + i)) : 0);
+                    cp_async<NB * 2>(dst + 2 * KT::K_BYTES + i * NB * 2, c.ks + row * NB, live);
+                    cp_async<NB * 2>(dst + 2 * KT::K_BYTES + KT::S_BYTES + i * NB * 2, c.vs + row * NB, live);
+                }
+            }
+            lt += TEAMS;
+            ln++;
         }
-        at = pos + depth;
-    }
-    float qv[D / 32], o[D / 32] = {}, m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < D / 32; i++) qv[i] = (float)q[lane + 32 * i] * a.scale;
-    const int lo = c.window ? max(0, at - c.window + 1) : 0;
-    const int end = pos + t + 1;
-    for (int p = 0; p < end; p++) {
-        if (p == min(c.sinks, lo) && p < lo) p = min(lo, pos);
-        int where = p;
-        if (parent && p >= pos) {
-            if (!((anc >> (p - pos)) & 1)) continue;
-            where = pos - 1;
-            for (int i = p - pos; i >= 0; where++) i = parent[i] < i ? parent[i] : -1;
+        cp_commit();
+    };
+#pragma unroll 1
+    for (int i = 0; i < STAGES - 1; i++) load();
+
+    int done = 0;  // tiles computed by the team
+    int ct = begin + team;
+    for (int seg = begin; seg < end;) {
+        KaCursor cc;
+        KaSpan sp;
+        cc.at(seg, prefix, c.n_slot, c.n_kv);
+        sp.set(a, cc.b);
+        const int seg_end = min(end, cc.first + cc.tiles);
+        const int rows = sp.m * G;
+        const bool many = a.r.T > 1;
+        // ---- what each row sees ----
+        if (many) {
+            const int32_t* parent = a.parent ? a.parent + (size_t)cc.b * a.r.T : nullptr;
+            for (int r = tid; r < max(8 * WR, parent ? sp.m : 0); r += KA_THREADS) {
+                const int row = min(r / G, sp.m - 1);
+                int at = sp.pos + row;
+                if (parent) {
+                    uint64_t anc = 0;
+                    auto climb = [&](int i, bool set) {
+                        int depth = -1;
+                        while (i >= 0) {
+                            depth++;
+                            if (set) anc |= 1ull << i;
+                            const int p = parent[i];
+                            if (p >= i || p < -1) {
+                                dev_error(a.err, DEV_BAD_INDEX);
+                                break;
+                            }
+                            i = p;
+                        }
+                        return depth;
+                    };
+                    at = sp.pos + climb(row, true);
+                    if (r < 8 * WR) s_anc[r] = anc;
+                    if (r < sp.m) s_depth[r] = climb(r, false);
+                }
+                if (r < 8 * WR) s_at[r] = at;
+            }
+            __syncthreads();
         }
-        if (c.window && where <= at - c.window && where >= c.sinks) continue;
-        const size_t row = kv_index(c, b, h / (a.n_head / c.n_kv), kv_row(c, p));
-        float s = 0.0f;
+        // ---- this warp's queries, as the products' B operand: column g is row 8 wr + g ----
+        uint32_t qh[KSTEPS][2], ql[LO ? KSTEPS : 1][2];
+        float sfac[2];
+        {
+            const int r = 8 * wr + g;
+            const bool live = r < rows;
+            const T* qp = static_cast<const T*>(a.q) + cc.b * a.q_slot + (r / G) * a.q_row + (cc.h * G + r % G) * a.q_head;
+            float x[D / 4];  // the lane's dims: of step s, k = 2t, 2t + 1, 2t + 8, 2t + 9 at x[4 s …]
 #pragma unroll
-        for (int i = 0; i < D / 32; i++) s += qv[i] * kv_value<TYPE>(c.k, c.ks, row, D, lane + 32 * i);
-        s = warp_sum(s);
-        const float mn = fmaxf(m, s), f = expf(m - mn), e = mn == -INFINITY ? 0.0f : expf(s - mn);
-        l = (m == -INFINITY ? 0.0f : l * f) + e;
+            for (int s = 0; s < KSTEPS; s++)
 #pragma unroll
-        for (int i = 0; i < D / 32; i++)
-            o[i] = (m == -INFINITY ? 0.0f : o[i] * f) + e * kv_value<TYPE>(c.v, c.vs, row, D, lane + 32 * i);
-        m = mn;
+                for (int i = 0; i < 4; i++) {
+                    int d;
+                    if (TYPE == KV_F16)
+                        d = 16 * s + 2 * t + (i & 1) + 8 * (i >> 1);
+                    else if (TYPE == KV_Q8_0)
+                        d = 32 * (s >> 1) + 8 * t + 4 * (s & 1) + i;
+                    else  // bytes 4t … 4t + 3 of the block: pairs (0, 2), (1, 3)
+                        d = 32 * (s >> 1) + 16 * (s & 1) + 4 * t + ((i & 1) << 1) + (i >> 1);
+                    x[4 * s + i] = live ? (float)qp[d] : 0.0f;
+                }
+            float f = a.scale * LOG2E;
+            if constexpr (LO) {
+                // the row times a power of two that brings its largest to 2^10 … 2^11 (an infinity or a NaN: 1)
+                float big = 0.0f;
+#pragma unroll
+                for (int i = 0; i < D / 4; i++) big = fmaxf(big, fabsf(x[i]));
+                big = fmaxf(big, __shfl_xor_sync(FULL, big, 1));
+                big = fmaxf(big, __shfl_xor_sync(FULL, big, 2));
+                const int e = big > 0.0f && big <= 3.4028234e38f ? min(120, 137 - (int)(__float_as_uint(big) >> 23)) : 0;
+                const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+                f *= __uint_as_float((uint32_t)(127 - e) << 23);
+#pragma unroll
+                for (int i = 0; i < D / 4; i++) x[i] *= up;
+            }
+#pragma unroll
+            for (int s = 0; s < KSTEPS; s++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    qh[s][i] = pack2(x[4 * s + 2 * i], x[4 * s + 2 * i + 1]);
+                    if constexpr (LO) ql[s][i] = rest2(x[4 * s + 2 * i], x[4 * s + 2 * i + 1], qh[s][i]);
+                }
+            // column 2t and 2t + 1's factor (held by the lanes of g = 2t, 2t + 1)
+            sfac[0] = __shfl_sync(FULL, f, 8 * t);
+            sfac[1] = __shfl_sync(FULL, f, 8 * t + 4);
+        }
+        float o[DT][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+        // ---- a tile ----
+        auto compute = [&](int tile, const uint8_t* st, auto edge_) {
+            constexpr bool EDGE = decltype(edge_)::value;
+            const uint8_t *kt = st, *vt = st + KT::K_BYTES;
+            [[maybe_unused]] const uint8_t *kst = st + 2 * KT::K_BYTES, *vst = kst + KT::S_BYTES;
+            const int v0 = (tile - cc.first) * KEYS;
+            float p[MT][4];
+            // S: rows g and g + 8 of 16 keys are keys kA and kB, columns 2t and 2t + 1. f16: keys g and g + 8; quants:
+            // the order in which one lane's four keys of V's transposition are 4t … 4t + 3
+            auto key = [&](int i, int up) {
+                return 16 * i + (TYPE == KV_F16 ? g + 8 * up : 4 * (g >> 1) + (g & 1) + 2 * up);
+            };
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                if constexpr (TYPE == KV_F16) {
+                    float acc[4] = {};
+#pragma unroll
+                    for (int s = 0; s < KSTEPS; s++) {
+                        uint32_t ka[4];
+                        ldmatrix4<false>(ka, smem_u32(kt + KT::off(16 * i + (lane & 15), 2 * s + (lane >> 4), false)));
+                        mma16816(acc, ka, qh[s][0], qh[s][1]);
+                        if constexpr (LO) mma16816(acc, ka, ql[s][0], ql[s][1]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; j++) p[i][j] = acc[j];
+                } else {
+                    const int kA = key(i, 0), kB = key(i, 1);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) p[i][j] = 0.0f;
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        uint32_t ka[2][4];
+                        if constexpr (TYPE == KV_Q8_0) {
+                            const uint2 wA = *reinterpret_cast<const uint2*>(kt + KT::off(kA, 2 * b + (t >> 1), false) + (t & 1) * 8);
+                            const uint2 wB = *reinterpret_cast<const uint2*>(kt + KT::off(kB, 2 * b + (t >> 1), false) + (t & 1) * 8);
+#pragma unroll
+                            for (int s = 0; s < 2; s++) {
+                                const uint32_t A = (s ? wA.y : wA.x) ^ 0x80808080u, B = (s ? wB.y : wB.x) ^ 0x80808080u;
+                                ka[s][0] = bytes_h2(A, 0x4140, H2_1152), ka[s][2] = bytes_h2(A, 0x4342, H2_1152);
+                                ka[s][1] = bytes_h2(B, 0x4140, H2_1152), ka[s][3] = bytes_h2(B, 0x4342, H2_1152);
+                            }
+                        } else {
+                            const uint32_t A = *reinterpret_cast<const uint32_t*>(kt + KT::off(kA, b, false) + t * 4);
+                            const uint32_t B = *reinterpret_cast<const uint32_t*>(kt + KT::off(kB, b, false) + t * 4);
+                            ka[0][0] = nibbles_h2<false>(A), ka[0][2] = nibbles_h2<false>(A >> 8);
+                            ka[1][0] = nibbles_h2<true>(A), ka[1][2] = nibbles_h2<true>(A >> 8);
+                            ka[0][1] = nibbles_h2<false>(B), ka[0][3] = nibbles_h2<false>(B >> 8);
+                            ka[1][1] = nibbles_h2<true>(B), ka[1][3] = nibbles_h2<true>(B >> 8);
+                        }
+                        float acc[4] = {};
+#pragma unroll
+                        for (int s = 0; s < 2; s++) {
+                            mma16816(acc, ka[s], qh[2 * b + s][0], qh[2 * b + s][1]);
+                            if constexpr (LO) mma16816(acc, ka[s], ql[2 * b + s][0], ql[2 * b + s][1]);
+                        }
+                        const float dA = __half2float(reinterpret_cast<const __half*>(kst)[kA * NB + b]);
+                        const float dB = __half2float(reinterpret_cast<const __half*>(kst)[kB * NB + b]);
+                        p[i][0] = fmaf(acc[0], dA, p[i][0]), p[i][1] = fmaf(acc[1], dA, p[i][1]);
+                        p[i][2] = fmaf(acc[2], dB, p[i][2]), p[i][3] = fmaf(acc[3], dB, p[i][3]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) p[i][j] *= sfac[j & 1];
+            }
+            // ---- the mask ----
+            uint32_t bad = 0;       // (f16) keys of the tile whose values are not all finite
+            uint32_t seen = ~0u;    // this lane's scores that their rows see, bit 4 i + j
+            if constexpr (EDGE) {
+                if (TYPE == KV_F16 && many) {
+                    // a value that some rows see and some do not must not reach the latter as 0 * inf: such rows of V
+                    // are taken out of the product and given to those who see them as a NaN weight
+                    for (int i = 0; i < KEYS; i++) {
+                        bool b = false;
+                        if (lane < KT::ROW / 16) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(vt + KT::off(i, lane, true));
+                            auto inf = [](uint32_t w) { return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u; };
+                            b = inf(x.x) || inf(x.y) || inf(x.z) || inf(x.w);
+                        }
+                        if (__any_sync(FULL, b)) bad |= 1u << i;
+                    }
+                }
+                seen = 0;
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int kk = key(i, j >> 1), v = v0 + kk;
+                        bool s = v < sp.nv;
+                        if (s && many) {
+                            const int r = 8 * wr + 2 * t + (j & 1), at = s_at[r];
+                            int where = sp.position(v);
+                            if (a.parent) {
+                                if (where >= sp.pos) {
+                                    s = (s_anc[r] >> (where - sp.pos)) & 1;
+                                    where = sp.pos + s_depth[where - sp.pos];
+                                }
+                            } else {
+                                s = where <= at;
+                            }
+                            if (c.window) s = s && (where > at - c.window || where < c.sinks);
+                        }
+                        if (s) seen |= 1u << (4 * i + j);
+                        if (TYPE == KV_F16 && s && ((bad >> kk) & 1)) p[i][j] = NAN;
+                        if (!s) p[i][j] = -INFINITY;
+                    }
+            }
+            // ---- the running maximum, the weights ----
+            float alpha[2], ref[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float x = fmaxf(p[0][j], p[0][j + 2]);
+#pragma unroll
+                for (int i = 1; i < MT; i++) x = fmaxf(x, fmaxf(p[i][j], p[i][j + 2]));
+                x = fmaxf(x, __shfl_xor_sync(FULL, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(FULL, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(FULL, x, 16));
+                const float mn = fmaxf(m[j], x), safe = mn == -INFINITY ? 0.0f : mn;
+                alpha[j] = ex2(m[j] - safe);
+                ref[j] = safe - 8.0f;  // weights up to 2^8: the small ones stay further from f16's smallest
+                m[j] = mn;
+                l[j] *= alpha[j];
+            }
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    p[i][j] = ex2(p[i][j] - ref[j & 1]);
+                    l[j & 1] += p[i][j];
+                }
+            // ---- O = O alpha + V^T P ----
+            if constexpr (TYPE == KV_F16) {
+                uint32_t ph[MT][2];
+                [[maybe_unused]] uint32_t pl[LO ? MT : 1][2];
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const uint32_t h = pack2(p[i][2 * j], p[i][2 * j + 1]);
+                        ph[i][j] = transpose8(h);
+                        if constexpr (LO) pl[i][j] = transpose8(rest2(p[i][2 * j], p[i][2 * j + 1], h));
+                    }
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    float acc[4] = {};
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        uint32_t va[4];
+                        ldmatrix4<true>(va, smem_u32(vt + KT::off(16 * i + (lane & 7) + ((lane >> 4) << 3),
+                                                                 2 * d + ((lane >> 3) & 1), true)));
+                        if (EDGE && bad) {  // keys 2t, 2t + 1 (registers 0, 1) and 2t + 8, 2t + 9 (2, 3)
+                            const uint32_t z = bad >> (16 * i + 2 * t);
+                            const uint32_t k0 = (z & 1 ? 0u : 0xffffu) | (z & 2 ? 0u : 0xffff0000u);
+                            const uint32_t k1 = (z & 0x100 ? 0u : 0xffffu) | (z & 0x200 ? 0u : 0xffff0000u);
+                            va[0] &= k0, va[1] &= k0, va[2] &= k1, va[3] &= k1;
+                        }
+                        mma16816(acc, va, ph[i][0], ph[i][1]);
+                        if constexpr (LO) mma16816(acc, va, pl[i][0], pl[i][1]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; j++) o[d][j] = fmaf(o[d][j], alpha[j & 1], acc[j]);
+                }
+            } else {
+                // the scales of this lane's two keys of each 16, and the tile's largest of each block
+                __half2 dv[MT][2][NB / 2], top[NB / 2];
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++)
+#pragma unroll
+                        for (int b = 0; b < NB / 2; b++) {
+                            dv[i][u][b] = reinterpret_cast<const __half2*>(vst)[key(i, u) * (NB / 2) + b];
+                            const __half2 x = __habs2(dv[i][u][b]);
+                            top[b] = i + u == 0 ? x : __hmax2(top[b], x);
+                        }
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    if ((b & 1) == 0) {
+#pragma unroll
+                        for (int s = 4; s <= 16; s <<= 1) {
+                            const uint32_t y = __shfl_xor_sync(FULL, *reinterpret_cast<uint32_t*>(&top[b / 2]), s);
+                            top[b / 2] = __hmax2(top[b / 2], *reinterpret_cast<const __half2*>(&y));
+                        }
+                    }
+                    const float big = b & 1 ? __high2float(top[b / 2]) : __low2float(top[b / 2]);
+                    // 2^e <= big < 2^(e + 1); zero, or no finite scale: e = 0 or 16
+                    const int e = big > 0.0f ? min(16, (int)(__float_as_uint(big) >> 23) - 127) : 0;
+                    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+                    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+                    float acc[2][4] = {};
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        uint32_t ph[2];
+                        [[maybe_unused]] uint32_t pl[2];
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const float dd = (b & 1 ? __high2float(dv[i][u][b / 2]) : __low2float(dv[i][u][b / 2])) * down;
+                            float x = p[i][2 * u] * dd, y = p[i][2 * u + 1] * dd;
+                            if (EDGE) {  // (0 times a scale that is no number)
+                                if (!((seen >> (4 * i + 2 * u)) & 1)) x = 0.0f;
+                                if (!((seen >> (4 * i + 2 * u + 1)) & 1)) y = 0.0f;
+                            }
+                            const uint32_t h = pack2(x, y);
+                            ph[u] = transpose8(h);
+                            if constexpr (LO) pl[u] = transpose8(rest2(x, y, h));
+                        }
+                        uint32_t va[2][4];
+                        if constexpr (TYPE == KV_Q8_0) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                w[j] = *reinterpret_cast<const uint32_t*>(
+                                           vt + KT::off(16 * i + 4 * t + j, 2 * b + (g >> 2), true) + (g & 3) * 4) ^
+                                       0x80808080u;
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {  // keys 4t + 2u, 4t + 2u + 1; dims 4g … 4g + 3 of the block
+                                const uint32_t x = __byte_perm(w[2 * u], w[2 * u + 1], 0x5140);
+                                const uint32_t y = __byte_perm(w[2 * u], w[2 * u + 1], 0x7362);
+                                va[0][2 * u] = bytes_h2(x, 0x4140, H2_1152), va[0][2 * u + 1] = bytes_h2(x, 0x4342, H2_1152);
+                                va[1][2 * u] = bytes_h2(y, 0x4140, H2_1152), va[1][2 * u + 1] = bytes_h2(y, 0x4342, H2_1152);
+                            }
+                        } else {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                w[j] = *reinterpret_cast<const uint16_t*>(vt + KT::off(16 * i + 4 * t + j, b, true) + g * 2);
+#pragma unroll
+                            for (int u = 0; u < 2; u++) {  // dims 2g, 2g + 1 (low nibbles) and 16 + 2g, 17 + 2g (high)
+                                const uint32_t x = __byte_perm(w[2 * u], w[2 * u + 1], 0x5410);
+                                va[0][2 * u] = nibbles_h2<false>(x), va[0][2 * u + 1] = nibbles_h2<false>(x >> 8);
+                                va[1][2 * u] = nibbles_h2<true>(x), va[1][2 * u + 1] = nibbles_h2<true>(x >> 8);
+                            }
+                        }
+#pragma unroll
+                        for (int s = 0; s < 2; s++) {
+                            mma16816(acc[s], va[s], ph[0], ph[1]);
+                            if constexpr (LO) mma16816(acc[s], va[s], pl[0], pl[1]);
+                        }
+                    }
+#pragma unroll
+                    for (int s = 0; s < 2; s++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) o[2 * b + s][j] = fmaf(o[2 * b + s][j], alpha[j & 1], acc[s][j] * up);
+                }
+            }
+        };
+
+        for (; ct < seg_end; ct += TEAMS, done++) {
+            cp_wait<STAGES - 2>();
+            if constexpr (WR == 1)
+                __syncwarp();
+            else
+                bar_sync(1 + team, WR * 32);
+            load();  // into the stage that was computed last
+            const uint8_t* st = ring + done % STAGES * KT::STAGE;
+            // whether every row sees every key of the tile
+            const int v0 = (ct - cc.first) * KEYS, v1 = v0 + KEYS;
+            bool edge = v1 > sp.nv;
+            if (many && !edge && v1 > sp.ns) {
+                const int p0 = sp.position(v0), p1 = sp.position(v1 - 1);
+                edge = v0 < sp.ns || p1 >= sp.pos + (a.parent ? 0 : 1) ||
+                       (c.window && p0 <= sp.pos + sp.m - 1 - c.window && p1 >= c.sinks);
+            }
+            if (edge)
+                compute(ct, st, std::true_type{});
+            else
+                compute(ct, st, std::false_type{});
+        }
+
+        // ---- the teams' parts joined: halves of them at a time, the upper into the lower ----
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            l[j] += __shfl_xor_sync(FULL, l[j], 4);
+            l[j] += __shfl_xor_sync(FULL, l[j], 8);
+            l[j] += __shfl_xor_sync(FULL, l[j], 16);
+        }
+        auto fold = [&](float* mo, float* lo, float f0[2], float f1[2]) {  // weights of the own and the other part
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float mn = fmaxf(m[j], mo[j]), safe = mn == -INFINITY ? 0.0f : mn;
+                f0[j] = ex2(m[j] - safe), f1[j] = ex2(mo[j] - safe);
+                l[j] = l[j] * f0[j] + lo[j] * f1[j];
+                m[j] = mn;
+            }
+        };
+#pragma unroll
+        for (int half = TEAMS / 2; half >= 1; half /= 2) {
+            if (team >= half && team < 2 * half) {
+                const int w = warp - half * WR;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) joined[(w * (D / 4) + 4 * d + j) * 32 + lane] = o[d][j];
+                if (g == 0) {
+                    s_ml[w][2 * t] = m[0], s_ml[w][2 * t + 1] = m[1];
+                    s_ml[w][8 + 2 * t] = l[0], s_ml[w][8 + 2 * t + 1] = l[1];
+                }
+            }
+            __syncthreads();
+            if (team < half) {
+                float mo[2] = {s_ml[warp][2 * t], s_ml[warp][2 * t + 1]};
+                float lo[2] = {s_ml[warp][8 + 2 * t], s_ml[warp][8 + 2 * t + 1]}, f0[2], f1[2];
+                fold(mo, lo, f0, f1);
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        o[d][j] = o[d][j] * f0[j & 1] + joined[(warp * (D / 4) + 4 * d + j) * 32 + lane] * f1[j & 1];
+            }
+            __syncthreads();
+        }
+        // ---- the output, or this CTA's part of it ----
+        auto dim = [&](int d, int up) {  // the dim of tile d's row g (up = 0) or g + 8
+            if (TYPE == KV_F16) return 16 * d + 8 * up + g;
+            if (TYPE == KV_Q8_0) return 32 * (d >> 1) + 4 * g + 2 * (d & 1) + up;
+            return 32 * (d >> 1) + 16 * (d & 1) + 2 * g + up;
+        };
+        auto put = [&](int w, int d, const float* x, const float* ll) {  // rows 8 w + 2t, 8 w + 2t + 1
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int r = 8 * w + 2 * t + j;
+                if (r >= rows) continue;
+                T* op = static_cast<T*>(a.out) + cc.b * a.o_slot + (r / G) * a.o_row + (cc.h * G + r % G) * a.o_head;
+                const float inv = ll[j] == 0.0f ? 0.0f : 1.0f / ll[j];
+                op[dim(d, 0)] = (T)(ll[j] == 0.0f ? 0.0f : x[j] * inv);
+                op[dim(d, 1)] = (T)(ll[j] == 0.0f ? 0.0f : x[j + 2] * inv);
+            }
+        };
+        if (seg_end - seg == cc.tiles) {
+            if (team == 0)
+#pragma unroll
+                for (int d = 0; d < DT; d++) put(wr, d, o[d], l);
+        } else {
+            // parts: [2 CTAs][WR][D / 4 registers][32 lanes], then [WR][m 8, l 8]; the pair's first CTA holds it as its
+            // last pair (part 1), the others as their first (part 0)
+            constexpr int PART = WR * (D * 8 + 16);
+            uint32_t* tickets = static_cast<uint32_t*>(a.work);
+            float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + KA_TICKETS);
+            const int c0 = owner(cc.first), c1 = owner(cc.first + cc.tiles - 1);
+            float* mine = parts + (size_t)(2 * cta + (cta == c0)) * PART;
+            if (team == 0) {
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) __stcg(&mine[(wr * (D / 4) + 4 * d + j) * 32 + lane], o[d][j]);
+                if (g == 0) {
+                    float* ml = mine + WR * D * 8 + wr * 16;
+                    __stcg(&ml[2 * t], m[0]), __stcg(&ml[2 * t + 1], m[1]);
+                    __stcg(&ml[8 + 2 * t], l[0]), __stcg(&ml[8 + 2 * t + 1], l[1]);
+                }
+            }
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                const bool last = atomicAdd(&tickets[c0], 1u) == (uint32_t)(c1 - c0);
+                if (last) tickets[c0] = 0;
+                __threadfence();
+                s_last = last;
+            }
+            __syncthreads();
+            if (s_last) {
+                for (int w = warp; w < WR * DT; w += KA_WARPS) {  // (rows 8 r …, tile d) in the CTAs' order
+                    const int r = w / DT, d = w % DT;
+                    float mx[2] = {-INFINITY, -INFINITY}, ll[2] = {0.0f, 0.0f}, x[4] = {};
+                    auto ml_of = [&](int i) { return parts + (size_t)(2 * i + (i == c0)) * PART + WR * D * 8 + r * 16; };
+                    for (int i = c0; i <= c1; i++)
+#pragma unroll
+                        for (int j = 0; j < 2; j++) mx[j] = fmaxf(mx[j], __ldcg(&ml_of(i)[2 * t + j]));
+#pragma unroll
+                    for (int j = 0; j < 2; j++) mx[j] = mx[j] == -INFINITY ? 0.0f : mx[j];
+                    for (int i = c0; i <= c1; i++) {
+                        const float* q = parts + (size_t)(2 * i + (i == c0)) * PART + (r * (D / 4) + 4 * d) * 32 + lane;
+                        float f[2];
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            f[j] = ex2(__ldcg(&ml_of(i)[2 * t + j]) - mx[j]);
+                            ll[j] += __ldcg(&ml_of(i)[8 + 2 * t + j]) * f[j];
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; j++) x[j] += __ldcg(&q[32 * j]) * f[j & 1];
+                    }
+                    put(r, d, x, ll);
+                }
+            }
+        }
+        seg = seg_end;
+        if (many && seg < end) __syncthreads();  // (the rows' table is the next pair's)
     }
-#pragma unroll
-    for (int i = 0; i < D / 32; i++) out[lane + 32 * i] = (T)(l == 0.0f ? 0.0f : o[i] / l);
+    cp_wait<0>();
 }
 
-template <int TYPE, int D>
-static cudaError_t launch_d(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
-    const long warps = (long)a.c.n_slot * a.r.T * a.n_head;
-    const dim3 grid((unsigned)((warps + 3) / 4));
-    return a.half ? kv_launch(k_kv_attn_simple<TYPE, D, __half>, grid, 128, 0, st, pdl, a)
-                  : kv_launch(k_kv_attn_simple<TYPE, D, float>, grid, 128, 0, st, pdl, a);
+template <int TYPE, int D, int WR, class T>
+static cudaError_t launch_few(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
+    constexpr int SMEM = KA_WARPS * KA_RING + 4 * D * 8 * 4;
+    static PerDeviceOnce once;
+    once([] {
+        cudaFuncSetAttribute(k_kv_attn<TYPE, D, WR, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    });
+    return kv_launch(k_kv_attn<TYPE, D, WR, T>, dim3(a.num_sms), KA_THREADS, SMEM, st, pdl, a);
+}
+template <int TYPE, int D, class T>
+static cudaError_t launch_rows(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
+    const int rows = a.r.T * (a.n_head / a.c.n_kv);
+    if (rows <= 8) return launch_few<TYPE, D, 1, T>(st, a, pdl);
+    if (rows <= 16) return launch_few<TYPE, D, 2, T>(st, a, pdl);
+    return launch_few<TYPE, D, 4, T>(st, a, pdl);
 }
 template <int TYPE>
 static cudaError_t launch_type(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
-    return a.c.d == 128 ? launch_d<TYPE, 128>(st, a, pdl) : launch_d<TYPE, 64>(st, a, pdl);
+    if (a.c.d == 128)
+        return a.half ? launch_rows<TYPE, 128, __half>(st, a, pdl) : launch_rows<TYPE, 128, float>(st, a, pdl);
+    return a.half ? launch_rows<TYPE, 64, __half>(st, a, pdl) : launch_rows<TYPE, 64, float>(st, a, pdl);
 }
-cudaError_t launch_kv_attention(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
-    switch (a.c.type) {
-        case KV_F16: return launch_type<KV_F16>(st, a, pdl);
-        case KV_Q8_0: return launch_type<KV_Q8_0>(st, a, pdl);
-        default: return launch_type<KV_Q4_0>(st, a, pdl);
+
+cudaError_t launch_kv_attention_few(cudaStream_t st, const KvAttnArgs& all, bool pdl) {
+    for (int b = 0; b < all.c.n_slot; b += KA_SLOTS) {
+        const KvAttnArgs a = kv_slots(all, b, min(KA_SLOTS, all.c.n_slot - b));
+        const cudaError_t e = a.c.type == KV_F16    ? launch_type<KV_F16>(st, a, pdl)
+                              : a.c.type == KV_Q8_0 ? launch_type<KV_Q8_0>(st, a, pdl)
+                                                    : launch_type<KV_Q4_0>(st, a, pdl);
+        if (e != cudaSuccess) return e;
     }
+    return cudaSuccess;
 }
-size_t kv_attention_work_bytes(const KvAttnArgs&) { return 0; }
 
 }  // namespace ocr

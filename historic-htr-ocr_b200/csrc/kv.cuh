@@ -96,6 +96,22 @@ struct KvAttnArgs {
     int num_sms;
     int* err;
 };
+// the call for slots b … b + n - 1 alone
+inline KvAttnArgs kv_slots(const KvAttnArgs& all, int b, int n) {
+    KvAttnArgs a = all;
+    const size_t rows = (size_t)b * a.c.n_kv * a.c.n_rows, bytes = rows * kv_row_bytes(a.c.type, a.c.d);
+    a.c.n_slot = n;
+    a.c.k += bytes, a.c.v += bytes;
+    if (a.c.ks) a.c.ks += rows * (a.c.d / KV_BLOCK), a.c.vs += rows * (a.c.d / KV_BLOCK);
+    a.r.pos += b;
+    if (a.r.n) a.r.n += b;
+    if (a.parent) a.parent += (size_t)b * a.r.T;
+    const long item = a.half ? 2 : 4;
+    a.q = static_cast<const char*>(a.q) + b * a.q_slot * item;
+    a.out = static_cast<char*>(a.out) + b * a.o_slot * item;
+    return a;
+}
+cudaError_t launch_kv_attention_few(cudaStream_t st, const KvAttnArgs& a, bool pdl);
 cudaError_t launch_kv_attention(cudaStream_t st, const KvAttnArgs& a, bool pdl);
 size_t kv_attention_work_bytes(const KvAttnArgs& a);
 
