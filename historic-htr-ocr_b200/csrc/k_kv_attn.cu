@@ -19,16 +19,14 @@
 // are split into f16 hi + lo (22 bits); f16 queries are exact, and P is rounded to f16 like the output. A row's query
 // is scaled by a power of two so that its lo part does not fall below f16's range, P likewise by the tile's largest
 // scale.
-#include "kv.cuh"
+#include "kv_attn.cuh"
 
 namespace ocr {
 
+constexpr int KA_ROWS = 32;          // (row, query head) pairs of a kv head up to which this kernel runs
 constexpr int KA_WARPS = 8;
 constexpr int KA_THREADS = KA_WARPS * 32;
-constexpr int KA_SLOTS = 512;        // slots of one launch (the line's prefix sums are in shared memory)
-constexpr int KA_TICKETS = 4096;     // bytes before the partial results: a ticket per CTA
 constexpr int KA_RING = 26112;       // a warp's share of the rings: three q8_0 tiles of 32 keys
-constexpr float LOG2E = 1.4426950408889634f;
 
 template <int TYPE, int D>
 struct KaTile {
@@ -50,20 +48,6 @@ struct KaTile {
     }
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-}
-// the remainders of a and b past their f16 rounding `hi`
-__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t hi) {
-    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-    return pack2(a - h.x, b - h.y);
-}
 __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -99,58 +83,6 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// an unsigned byte pair placed as halves of 1024 + u, less `bias`
-__device__ __forceinline__ uint32_t bytes_h2(uint32_t w, uint32_t sel, uint32_t bias) {
-    const uint32_t m = __byte_perm(w, 0x64646464u, sel);
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&m), *reinterpret_cast<const __half2*>(&bias));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-constexpr uint32_t H2_1152 = 0x64806480u;  // 1024 + 128: an int8 with its sign bit flipped
-// the low (SHIFT = 0) or high nibbles of bytes 0 and 2 of w, less 8
-template <bool HIGH>
-__device__ __forceinline__ uint32_t nibbles_h2(uint32_t w) {
-    const uint32_t m = (w & (HIGH ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;  // 1024 + n, or 1024 + 16 n
-    const __half2 x = *reinterpret_cast<const __half2*>(&m);
-    __half2 r;
-    if (HIGH)
-        r = __hfma2(x, __float2half2_rn(0.0625f), __float2half2_rn(-72.0f));
-    else
-        r = __hsub2(x, __float2half2_rn(1032.0f));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-// one (slot, kv head) pair's visible keys, in order: the sinks that lie before the window, then positions lo … end - 1
-struct KaSpan {
-    int pos, m, lo, ns, nv;  // rows in use, first position of the window, sinks before it, keys
-    __device__ __forceinline__ void set(const KvAttnArgs& a, int b) {
-        pos = a.r.pos[b];
-        m = a.r.rows(a.c, b, a.err);
-        lo = a.c.window ? max(0, pos - a.c.window + 1) : 0;
-        ns = min(a.c.sinks, lo);
-        nv = m ? ns + pos + m - lo : 0;
-    }
-    __device__ __forceinline__ int position(int v) const { return v < ns ? v : lo + v - ns; }
-};
-
-// where a CTA stands in the line of tiles
-struct KaCursor {
-    int b, h, first, tiles;  // the pair, its first tile in the line, its tiles
-    __device__ __forceinline__ void at(int g, const int* prefix, int n_slot, int n_kv) {  // the pair of tile g
-        int lo = 0, hi = n_slot;  // prefix[lo] <= g < prefix[hi]
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (prefix[mid] <= g)
-                lo = mid;
-            else
-                hi = mid;
-        }
-        b = lo;
-        tiles = (prefix[b + 1] - prefix[b]) / n_kv;
-        h = (g - prefix[b]) / tiles;
-        first = prefix[b] + h * tiles;
-    }
-};
-
 template <int TYPE, int D, int WR, class T>
 __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant__ KvAttnArgs a) {
     using KT = KaTile<TYPE, D>;
@@ -160,7 +92,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
     constexpr int KEYS = KT::KEYS, MT = KEYS / 16, NB = KT::NB;
     constexpr int KSTEPS = D / 16, DT = D / 16;  // 16-dim steps of S, 16-dim tiles of O
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int prefix[KA_SLOTS + 1];
+    __shared__ int prefix[KV_LINE + 1];
     __shared__ int wsum[KA_WARPS];
     __shared__ int s_at[8 * WR], s_depth[KV_TREE_MAX];
     __shared__ uint64_t s_anc[8 * WR];
@@ -178,10 +110,10 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
     int total = 0;
     for (int b0 = 0; b0 < c.n_slot; b0 += KA_THREADS) {
         const int b = b0 + tid;
-        KaSpan s;
+        KvSpan s;
         s.nv = 0;
         if (b < c.n_slot) {
-            s.set(a, b);
+            s.set(a, b, 0, a.r.T);
             idle_rows |= s.m < a.r.T;
         }
         int x = (s.nv + KEYS - 1) / KEYS * c.n_kv;
@@ -223,16 +155,16 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
     float* joined = reinterpret_cast<float*>(smem + KA_WARPS * KA_RING);  // [4 warps][D / 4 registers][32 lanes]
 
     // ---- the copies of a tile, by the team's threads ----
-    KaCursor lc;
-    KaSpan ls;
+    KvCursor lc;
+    KvSpan ls;
     lc.at(begin, prefix, c.n_slot, c.n_kv);
-    ls.set(a, lc.b);
+    ls.set(a, lc.b, 0, a.r.T);
     int lt = begin + team, ln = 0;  // the next tile to copy, the copies so far
     auto load = [&]() {
         if (lt < end) {
             if (lt >= lc.first + lc.tiles) {
                 lc.at(lt, prefix, c.n_slot, c.n_kv);
-                ls.set(a, lc.b);
+                ls.set(a, lc.b, 0, a.r.T);
             }
             const uint32_t dst = smem_u32(ring + ln % STAGES * KT::STAGE);
             const int v0 = (lt - lc.first) * KEYS;
@@ -266,10 +198,10 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
     int done = 0;  // tiles computed by the team
     int ct = begin + team;
     for (int seg = begin; seg < end;) {
-        KaCursor cc;
-        KaSpan sp;
+        KvCursor cc;
+        KvSpan sp;
         cc.at(seg, prefix, c.n_slot, c.n_kv);
-        sp.set(a, cc.b);
+        sp.set(a, cc.b, 0, a.r.T);
         const int seg_end = min(end, cc.first + cc.tiles);
         const int rows = sp.m * G;
         const bool many = a.r.T > 1;
@@ -332,7 +264,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
                 for (int i = 0; i < D / 4; i++) big = fmaxf(big, fabsf(x[i]));
                 big = fmaxf(big, __shfl_xor_sync(FULL, big, 1));
                 big = fmaxf(big, __shfl_xor_sync(FULL, big, 2));
-                const int e = big > 0.0f && big <= 3.4028234e38f ? min(120, 137 - (int)(__float_as_uint(big) >> 23)) : 0;
+                const int e = big > 0.0f && big <= 3.4028234e38f ? min(100, 137 - (int)(__float_as_uint(big) >> 23)) : 0;
                 const float up = __uint_as_float((uint32_t)(127 + e) << 23);
                 f *= __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
@@ -687,7 +619,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
             // last pair (part 1), the others as their first (part 0)
             constexpr int PART = WR * (D * 8 + 16);
             uint32_t* tickets = static_cast<uint32_t*>(a.work);
-            float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + KA_TICKETS);
+            float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + KV_TICKETS);
             const int c0 = owner(cc.first), c1 = owner(cc.first + cc.tiles - 1);
             float* mine = parts + (size_t)(2 * cta + (cta == c0)) * PART;
             if (team == 0) {
@@ -742,7 +674,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
 }
 
 template <int TYPE, int D, int WR, class T>
-static cudaError_t launch_few(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
+static cudaError_t launch_team(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
     constexpr int SMEM = KA_WARPS * KA_RING + 4 * D * 8 * 4;
     static PerDeviceOnce once;
     once([] {
@@ -753,9 +685,9 @@ static cudaError_t launch_few(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
 template <int TYPE, int D, class T>
 static cudaError_t launch_rows(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
     const int rows = a.r.T * (a.n_head / a.c.n_kv);
-    if (rows <= 8) return launch_few<TYPE, D, 1, T>(st, a, pdl);
-    if (rows <= 16) return launch_few<TYPE, D, 2, T>(st, a, pdl);
-    return launch_few<TYPE, D, 4, T>(st, a, pdl);
+    if (rows <= 8) return launch_team<TYPE, D, 1, T>(st, a, pdl);
+    if (rows <= 16) return launch_team<TYPE, D, 2, T>(st, a, pdl);
+    return launch_team<TYPE, D, 4, T>(st, a, pdl);
 }
 template <int TYPE>
 static cudaError_t launch_type(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
@@ -764,9 +696,10 @@ static cudaError_t launch_type(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
     return a.half ? launch_rows<TYPE, 64, __half>(st, a, pdl) : launch_rows<TYPE, 64, float>(st, a, pdl);
 }
 
-cudaError_t launch_kv_attention_few(cudaStream_t st, const KvAttnArgs& all, bool pdl) {
-    for (int b = 0; b < all.c.n_slot; b += KA_SLOTS) {
-        const KvAttnArgs a = kv_slots(all, b, min(KA_SLOTS, all.c.n_slot - b));
+static size_t few_work(const KvAttnArgs& a) { return KV_TICKETS + (size_t)a.num_sms * 2 * 4 * (a.c.d * 8 + 16) * 4; }
+static cudaError_t launch_few(cudaStream_t st, const KvAttnArgs& all, bool pdl) {
+    for (int b = 0; b < all.c.n_slot; b += KV_LINE) {
+        const KvAttnArgs a = kv_slots(all, b, min(KV_LINE, all.c.n_slot - b));
         const cudaError_t e = a.c.type == KV_F16    ? launch_type<KV_F16>(st, a, pdl)
                               : a.c.type == KV_Q8_0 ? launch_type<KV_Q8_0>(st, a, pdl)
                                                     : launch_type<KV_Q4_0>(st, a, pdl);
@@ -774,5 +707,11 @@ cudaError_t launch_kv_attention_few(cudaStream_t st, const KvAttnArgs& all, bool
     }
     return cudaSuccess;
 }
+
+static bool is_few(const KvAttnArgs& a) { return (long)a.r.T * (a.n_head / a.c.n_kv) <= KA_ROWS; }
+cudaError_t launch_kv_attention(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
+    return is_few(a) ? launch_few(st, a, pdl) : launch_kv_attention_many(st, a, pdl);
+}
+size_t kv_attention_work_bytes(const KvAttnArgs& a) { return is_few(a) ? few_work(a) : kv_attention_many_work(a); }
 
 }  // namespace ocr

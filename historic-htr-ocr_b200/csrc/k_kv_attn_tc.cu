@@ -1,0 +1,827 @@
+// k_kv_attn_tc.cu — attention of many rows per kv head (a prompt's rows, a wide tree of drafts) over a KV cache
+// (kv.cuh), on the 5th-generation tensor cores. The formula is k_kv_attn.cu's.
+//
+// A CTA takes 128 (row, query head) pairs of a kv head (the pairs of a row side by side, so K and V are read once for
+// the whole group) against the keys that any of them sees, in tiles of 128 keys. Bound: the tensor cores (f32 rows),
+// the exponentials (f16 rows: 16 a clock and SM against 128 x 128 of a tile).
+//
+// Products: S = Q K^T (M = N = 128, both operands in shared memory), O += P V (A = P in TMEM, written over S in place;
+// B = V^T in shared memory), f16 operands, f32 sums in TMEM. Exactness: f32 queries and P are f16 hi + lo (22 bits);
+// f16 queries are exact, and P is rounded to f16 as the output is. f16 keys and values are exact; a quantised value
+// q d (at most 19 bits) splits exactly into f16 hi + lo, so S = Q_hi K_hi + Q_lo K_hi + Q_hi K_lo, and P V alike, carry
+// the f32 product to 2^-22. A row's query is scaled by a power of two (its lo part stays in f16's range), a tile's
+// scales by a power of two 2^-e, e from the tile's largest: S takes 2^e back with the row's factor; for V the score
+// itself takes e as an addend, so that P carries 2^e and the row's reference bounds both.
+//
+// Softmax: online. Two warpgroups take the tiles in turn, each with sums, reference and O of its own (joined at the
+// end), so one's exponentials run beside the other's products. The reference moves when a tile's maximum passes it by
+// 2^6 (then O is rescaled in TMEM); weights stay below 2^14.
+//
+// Roles (544 threads): warps 0-3 and 4-7 the two softmax groups, a row per thread; warps 8-15 stage K and V: raw loads
+// one tile ahead in registers, quants to f16, V transposed (every operand K-major, 128-byte swizzle); warp 16 issues
+// the products. Every wait is bounded: a role that gives up sets a flag, the others follow, and no copy is in flight
+// (the staging is plain loads and stores).
+//
+// The work: as in k_kv_attn.cu, the tiles of all (slot, row block, kv head) triples form a line cut evenly over the
+// SMs, triples in several CTAs joined by the last to arrive; past KV_LINE (slot, row block) pairs a CTA takes one
+// triple, longest first.
+#include "kv_attn.cuh"
+#include "tc.cuh"
+
+namespace ocr {
+
+constexpr int KC_M = 128, KC_KEYS = 128;
+constexpr int KC_LOADERS = 8;
+constexpr int KC_THREADS = (8 + KC_LOADERS + 1) * 32;
+constexpr int KC_RING = 4;  // tiles whose exponents and marks are kept
+constexpr float KC_LAG = 6.0f, KC_BIAS = 8.0f;
+
+template <int TYPE, int D, class T>
+struct KcPlan {
+    static constexpr bool LO = sizeof(T) == 4, QN = TYPE != KV_F16;
+    static constexpr int NB = D / KV_BLOCK, ROW = kv_row_bytes(TYPE, D);
+    static constexpr uint32_t Q_BYTES = KC_M * D * 2, T_BYTES = KC_KEYS * D * 2;  // one f16 operand of Q; of K or V
+    static constexpr int PARTS = QN ? 2 : 1;                                      // hi (and lo) of K and V
+    static constexpr int NS = QN && D == 128 ? 1 : 2;                             // stages
+    static constexpr uint32_t SMEM = (LO ? 2 : 1) * Q_BYTES + 2 * NS * PARTS * T_BYTES + 1024;
+    // the joined parts: [D][128] sums, [128] references, [128] weights' sums
+    static constexpr int PART = (D + 2) * KC_M;
+};
+
+struct KcShared {
+    uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], odone[2], xfull[KC_RING], mdone;
+    uint32_t tmem;
+    int abort_flag, last;
+    int prefix[KV_LINE + 1], wsum[KC_THREADS / 32];
+    float fac[KC_M];             // the rows' factors on S
+    float ml[2][2][KC_M];        // the groups' references and sums
+    int ex[KC_RING][2];          // the tiles' exponents of K and V
+    uint32_t bad[KC_RING][4];    // keys of an edge tile whose values are not all finite
+    uint32_t red[2][KC_LOADERS];
+    int parent[KV_TREE_MAX], depth[KV_TREE_MAX];
+};
+
+__device__ __forceinline__ uint32_t kc_sw(int r, int p) { return (uint32_t)r * 128u + (uint32_t)((p ^ (r & 7)) << 4); }
+
+__device__ __forceinline__ bool kc_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+    for (uint32_t i = 0; i < MBAR_TRIES; i++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+    }
+    *abort_flag = 1;
+    dev_error(err, DEV_TIMEOUT);
+    return false;
+}
+// the same for a whole warp, with one answer: TMEM accesses are the warp's together, none of its lanes may leave alone
+__device__ __forceinline__ bool kc_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+    return __all_sync(FULL, kc_wait(bar, parity, abort_flag, err));
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
+    tmem_ld16(taddr, r);
+    tmem_ld16(taddr + 16, r + 16);
+}
+__device__ __forceinline__ uint32_t h2mul(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// a b - c, rounded once: the rest of a product past its rounding c
+__device__ __forceinline__ uint32_t h2rest(uint32_t a, uint32_t b, uint32_t c) {
+    const uint32_t n = c ^ 0x80008000u;
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
+                              *reinterpret_cast<const __half2*>(&n));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t h2max(uint32_t a, uint32_t b) {
+    const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ bool h2_not_finite(uint32_t w) {
+    return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
+}
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+// ---- the staging of a tile, by 256 threads: raw rows to registers, later to operands ------------------------------------
+template <int TYPE, int D>
+struct KcRaw {
+    static constexpr int ROW = kv_row_bytes(TYPE, D), UPK = ROW / 16, KU = KC_KEYS * UPK / (KC_LOADERS * 32);
+    static constexpr int VW = TYPE == KV_F16 ? 4 : TYPE == KV_Q8_0 ? 2 : 1;  // words of a key in a thread's block of V
+    static constexpr bool QN = TYPE != KV_F16;
+    static constexpr int NB = D / KV_BLOCK;
+    uint4 k[KU];
+    __half kd[KU];
+    uint32_t v[8][VW];
+    __half vd[8];
+    uint32_t ex[NB / 2];
+
+    // the key and the 16-byte unit of the i-th piece of K: eight keys to a store's eight lanes
+    __device__ static __forceinline__ void unit(int i, int lw, int lane, int& key, int& u) {
+        const int w = i * KC_LOADERS + lw;
+        if (UPK >= 4) {
+            key = 8 * (w / (UPK >= 4 ? UPK / 4 : 1)) + (lane & 7);
+            u = w % (UPK >= 4 ? UPK / 4 : 1) * 4 + (lane >> 3);
+        } else {
+            key = 16 * w + (lane & 15);
+            u = lane >> 4;
+        }
+    }
+    // the thread's 8 x 8 block of V: keys 64 half + 8 ka …, group b of eight dims
+    __device__ static __forceinline__ bool block(int lt, int& ka, int& b, int& half) {
+        ka = lt & 7;
+        b = (lt >> 3) % (D / 8);
+        half = (lt >> 3) / (D / 8);
+        return half < 2;
+    }
+
+    __device__ __forceinline__ void load_k(const KvView& c, const KvSpan& s, size_t base, int v0, int lw, int lane) {
+#pragma unroll
+        for (int i = 0; i < KU; i++) {
+            int key, u;
+            unit(i, lw, lane, key, u);
+            k[i] = make_uint4(0u, 0u, 0u, 0u);
+            kd[i] = __ushort_as_half(0);
+            if (v0 + key < s.nv) {
+                const size_t row = base + kv_row(c, s.position(v0 + key));
+                k[i] = *reinterpret_cast<const uint4*>(c.k + row * ROW + u * 16);
+                if constexpr (QN) kd[i] = c.ks[row * NB + (TYPE == KV_Q8_0 ? u >> 1 : u)];
+            }
+        }
+        if constexpr (QN) {  // the scales of one key: K's for threads 0 … 127, V's for the others
+            const int key = (lw * 32 + lane) & (KC_KEYS - 1);
+#pragma unroll
+            for (int j = 0; j < NB / 2; j++) ex[j] = 0u;
+            if (v0 + key < s.nv) {
+                const size_t row = base + kv_row(c, s.position(v0 + key));
+                const uint32_t* p = reinterpret_cast<const uint32_t*>((lw < KC_LOADERS / 2 ? c.ks : c.vs) + row * NB);
+#pragma unroll
+                for (int j = 0; j < NB / 2; j++) ex[j] = p[j];
+            }
+        }
+    }
+    __device__ __forceinline__ void load_v(const KvView& c, const KvSpan& s, size_t base, int v0, int lt) {
+        int ka, b, half;
+        const bool on = block(lt, ka, b, half);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int key = 64 * half + 8 * ka + i;
+#pragma unroll
+            for (int j = 0; j < VW; j++) v[i][j] = 0u;
+            vd[i] = __ushort_as_half(0);
+            if (on && v0 + key < s.nv) {
+                const size_t row = base + kv_row(c, s.position(v0 + key));
+                const uint8_t* p = c.v + row * ROW + b * (VW * 4);
+                if constexpr (VW == 4) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(p);
+                    v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+                } else if constexpr (VW == 2) {
+                    const uint2 x = *reinterpret_cast<const uint2*>(p);
+                    v[i][0] = x.x, v[i][1] = x.y;
+                } else {
+                    v[i][0] = *reinterpret_cast<const uint32_t*>(p);
+                }
+                if constexpr (QN) vd[i] = c.vs[row * NB + b / 4];
+            }
+        }
+    }
+    // K as the product's operand: rows of 64 dims (128 bytes) in D / 64 halves of 128 keys
+    __device__ __forceinline__ void store_k(uint8_t* hi, uint8_t* lo, int e, int lw, int lane) const {
+        const float down = exp2i(-e);
+#pragma unroll
+        for (int i = 0; i < KU; i++) {
+            int key, u;
+            unit(i, lw, lane, key, u);
+            const uint32_t w[4] = {k[i].x, k[i].y, k[i].z, k[i].w};
+            if constexpr (TYPE == KV_F16) {
+                *reinterpret_cast<uint4*>(hi + (u >> 3) * (KC_KEYS * 128) + kc_sw(key, u & 7)) = k[i];
+            } else {
+                const __half2 dh = __float2half2_rn(__half2float(kd[i]) * down);
+                const uint32_t d = *reinterpret_cast<const uint32_t*>(&dh);
+                uint32_t q[TYPE == KV_Q8_0 ? 8 : 16];  // pairs of dims in order
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if constexpr (TYPE == KV_Q8_0) {
+                        q[2 * j] = bytes_h2(w[j] ^ 0x80808080u, 0x4140, H2_1152);
+                        q[2 * j + 1] = bytes_h2(w[j] ^ 0x80808080u, 0x4342, H2_1152);
+                    } else {
+                        const uint32_t x = __byte_perm(w[j], 0u, 0x4140), y = __byte_perm(w[j], 0u, 0x4342);
+                        q[2 * j] = nibbles_h2<false>(x), q[2 * j + 1] = nibbles_h2<false>(y);
+                        q[8 + 2 * j] = nibbles_h2<true>(x), q[8 + 2 * j + 1] = nibbles_h2<true>(y);
+                    }
+                }
+                constexpr int PC = TYPE == KV_Q8_0 ? 2 : 4;  // 16-byte pieces of the unit
+#pragma unroll
+                for (int j = 0; j < PC; j++) {
+                    const int pc = PC * u + j;
+                    const uint32_t at = (pc >> 3) * (KC_KEYS * 128) + kc_sw(key, pc & 7);
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        h[x] = h2mul(q[4 * j + x], d);
+                        l[x] = h2rest(q[4 * j + x], d, h[x]);
+                    }
+                    *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+                }
+            }
+        }
+    }
+    // V transposed: rows of 64 keys (128 bytes) in two halves of D dims. In an edge tile, what is not finite becomes
+    // zero and its key is marked.
+    __device__ __forceinline__ void store_v(uint8_t* hi, uint8_t* lo, int e, bool edge, uint32_t* bad, int lt) {
+        int ka, b, half;
+        if (!block(lt, ka, b, half)) return;
+        if (edge) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                bool x = false;
+                if constexpr (QN)
+                    x = h2_not_finite((uint32_t)__half_as_ushort(vd[i]));
+                else
+#pragma unroll
+                    for (int j = 0; j < VW; j++) x |= h2_not_finite(v[i][j]);
+                if (x) {
+                    atomicOr(&bad[2 * half + (ka >> 2)], 1u << (8 * (ka & 3) + i));
+                    vd[i] = __ushort_as_half(0);
+                    if constexpr (!QN)
+#pragma unroll
+                        for (int j = 0; j < VW; j++) v[i][j] = 0u;
+                }
+            }
+        }
+        uint8_t *h0 = hi + half * (D * 128), *l0 = lo + half * (D * 128);
+        if constexpr (TYPE == KV_F16) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+                const int w = j >> 1;
+                *reinterpret_cast<uint4*>(h0 + kc_sw(8 * b + j, ka)) =
+                    make_uint4(__byte_perm(v[0][w], v[1][w], sel), __byte_perm(v[2][w], v[3][w], sel),
+                               __byte_perm(v[4][w], v[5][w], sel), __byte_perm(v[6][w], v[7][w], sel));
+            }
+        } else {
+            const float down = exp2i(-e);
+            uint32_t d[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) d[i] = pack2(__half2float(vd[2 * i]) * down, __half2float(vd[2 * i + 1]) * down);
+#pragma unroll
+            for (int x = 0; x < 4; x++) {  // two dims at a time
+                uint32_t q[2][4];
+                int dim[2];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if constexpr (TYPE == KV_Q8_0) {  // dims 8 b + 2 x, + 1: bytes 2 (x % 2) … of word x / 2
+                        const uint32_t m = __byte_perm(v[2 * i][x >> 1], v[2 * i + 1][x >> 1], x & 1 ? 0x7362 : 0x5140) ^
+                                           0x80808080u;
+                        q[0][i] = bytes_h2(m, 0x4140, H2_1152), q[1][i] = bytes_h2(m, 0x4342, H2_1152);
+                    } else {  // byte x of the word: dim 4 w + x (low) and 16 + 4 w + x (high) of the block
+                        const uint32_t m = __byte_perm(v[2 * i][0], v[2 * i + 1][0], x & 2 ? 0x7632 : 0x5410) >> (8 * (x & 1));
+                        q[0][i] = nibbles_h2<false>(m), q[1][i] = nibbles_h2<true>(m);
+                    }
+                }
+                if constexpr (TYPE == KV_Q8_0)
+                    dim[0] = 8 * b + 2 * x, dim[1] = dim[0] + 1;
+                else
+                    dim[0] = 32 * (b >> 2) + 4 * (b & 3) + x, dim[1] = dim[0] + 16;
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        h[i] = h2mul(q[y][i], d[i]);
+                        l[i] = h2rest(q[y][i], d[i], h[i]);
+                    }
+                    *reinterpret_cast<uint4*>(h0 + kc_sw(dim[y], ka)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4*>(l0 + kc_sw(dim[y], ka)) = make_uint4(l[0], l[1], l[2], l[3]);
+                }
+            }
+        }
+    }
+};
+
+template <int TYPE, int D, class T>
+__global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_constant__ KvAttnArgs a, int blocks, int line) {
+    using P = KcPlan<TYPE, D, T>;
+    using Raw = KcRaw<TYPE, D>;
+    constexpr int NS = P::NS;
+    extern __shared__ uint8_t sm_raw[];
+    __shared__ __align__(8) KcShared sh;
+    volatile int* abort_flag = &sh.abort_flag;
+    const KvView& c = a.c;
+    int* err = a.err;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int G = a.n_head / c.n_kv;
+    uint8_t* Qh = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
+    uint8_t* Ql = Qh + P::Q_BYTES;
+    uint8_t* Kr = Qh + (P::LO ? 2 : 1) * P::Q_BYTES;
+    uint8_t* Vr = Kr + NS * P::PARTS * P::T_BYTES;
+    pdl_trigger();
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sh.kfull[i], KC_LOADERS);
+            mbar_init(&sh.kempty[i], 1);
+            mbar_init(&sh.vfull[i], KC_LOADERS);
+            mbar_init(&sh.vempty[i], 1);
+            mbar_init(&sh.sfull[i], 1);
+            mbar_init(&sh.pfull[i], 4);
+            mbar_init(&sh.odone[i], 1);
+        }
+        for (int i = 0; i < KC_RING; i++) mbar_init(&sh.xfull[i], 1);
+        mbar_init(&sh.mdone, 1);
+        sh.abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 16) {
+        tmem_alloc(&sh.tmem, 512);
+        tmem_relinquish();
+    }
+    pdl_wait();
+
+    // ---- the line: exclusive sums of the tiles of every (slot, row block) ----
+    const int entries = c.n_slot * blocks;
+    auto rows_of_block = [&](int blk, int& t0, int& t1) { t0 = blk * KC_M / G, t1 = (blk * KC_M + KC_M - 1) / G + 1; };
+    bool idle_rows = false;
+    for (int b = tid; b < c.n_slot; b += KC_THREADS) idle_rows |= a.r.rows(c, b, err) < a.r.T;
+    int total = 0;
+    if (line) {
+        int x = 0;
+        if (tid < entries) {  // (at most KV_LINE of them)
+            int t0, t1;
+            rows_of_block(tid % blocks, t0, t1);
+            KvSpan s;
+            s.set(a, tid / blocks, t0, t1);
+            x = (s.nv + KC_KEYS - 1) / KC_KEYS * c.n_kv;
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(FULL, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) sh.wsum[warp] = x;
+        __syncthreads();
+        for (int w = 0; w < warp; w++) x += sh.wsum[w];
+        if (tid < entries) sh.prefix[tid + 1] = x;
+        if (tid == 0) sh.prefix[0] = 0;
+        for (int w = 0; w < KC_THREADS / 32; w++) total += sh.wsum[w];
+    }
+    tc_fence_before();
+    const bool some_idle = __syncthreads_or(idle_rows);
+    tc_fence_after();
+    if (some_idle) {  // rows that are not in use are zeros
+        const long n = (long)c.n_slot * a.r.T * a.n_head;
+        for (long i = (long)blockIdx.x * (KC_THREADS / 32) + warp; i < n; i += (long)gridDim.x * (KC_THREADS / 32)) {
+            const int h = (int)(i % a.n_head), r = (int)(i / a.n_head % a.r.T), b = (int)(i / a.n_head / a.r.T);
+            if (r < a.r.rows(c, b, nullptr)) continue;
+            T* o = static_cast<T*>(a.out) + b * a.o_slot + r * a.o_row + h * a.o_head;
+            for (int d = lane; d < D; d += 32) o[d] = (T)0.0f;
+        }
+    }
+    const uint32_t tmem = sh.tmem;
+    const int n_cta = line ? min((int)gridDim.x, total) : (int)gridDim.x;
+    const int cta = blockIdx.x;
+    auto part = [&](int i) { return (int)((long)total * i / n_cta); };
+    auto owner = [&](int tile) {
+        int i = (int)(((long)tile * n_cta) / total);
+        while (part(i + 1) <= tile) i++;
+        return i;
+    };
+    int begin = 0, end = 0;
+    KvCursor cc;
+    if (line) {
+        if (cta < n_cta) begin = part(cta), end = part(cta + 1);
+    } else {  // one triple, the last row blocks (the longest) first
+        const int per = c.n_slot * c.n_kv;
+        const int blk = blocks - 1 - cta / per, b = cta % per / c.n_kv;
+        int t0, t1;
+        rows_of_block(blk, t0, t1);
+        KvSpan s;
+        s.set(a, b, t0, t1);
+        cc.b = b * blocks + blk;
+        cc.h = cta % c.n_kv;
+        cc.first = 0;
+        cc.tiles = (s.nv + KC_KEYS - 1) / KC_KEYS;
+        end = cc.tiles;
+    }
+
+    int n0 = 0;          // tiles of this CTA before the triple
+    bool any_mma = false;  // (the issuing lane)
+    for (int seg = begin; seg < end;) {
+        if (line) cc.at(seg, sh.prefix, entries, c.n_kv);
+        const int slot = cc.b / blocks, blk = cc.b % blocks;
+        int t0, t1;
+        rows_of_block(blk, t0, t1);
+        KvSpan sp;
+        sp.set(a, slot, t0, t1);
+        const int seg_end = min(end, cc.first + cc.tiles), N = seg_end - seg;
+        const int r0 = blk * KC_M, rows = min(KC_M, sp.m * G - r0);
+        const size_t base = kv_index(c, slot, cc.h, 0);
+        // whether some row of the block does not see some key of the tile
+        auto edge_of = [&](int v0) {
+            if (v0 + KC_KEYS > sp.nv) return true;
+            if (v0 + KC_KEYS <= sp.ns) return false;
+            const int p0 = sp.position(v0), p1 = sp.position(v0 + KC_KEYS - 1);
+            const int lowest = sp.pos + (a.parent ? -1 : t0), highest = sp.pos + (a.parent ? sp.m : min(t1, sp.m)) - 1;
+            return v0 < sp.ns || p1 > lowest || (c.window && p0 <= highest - c.window && p1 >= c.sinks);
+        };
+        if (a.parent && tid < sp.m) sh.parent[tid] = a.parent[(size_t)slot * a.r.T + tid];
+        // ---- the queries: hi and lo, a row per warp at a time ----
+        if (warp < 16) {
+            for (int r = warp; r < KC_M; r += 16) {
+                const int row = r0 + r;
+                const bool live = r < rows;
+                const T* qp = static_cast<const T*>(a.q) + slot * a.q_slot + (row / G) * a.q_row +
+                              (cc.h * G + row % G) * a.q_head + lane * (D / 32);
+                float x[D / 32];
+                float f = a.scale * LOG2E;
+#pragma unroll
+                for (int i = 0; i < D / 32; i++) x[i] = live ? (float)qp[i] : 0.0f;
+                if constexpr (P::LO) {  // the row's largest to 2^10 … 2^11
+                    float big = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < D / 32; i++) big = fmaxf(big, fabsf(x[i]));
+                    big = warp_max(big);
+                    const int e = big > 0.0f && big <= 3.4028234e38f ? min(100, 137 - (int)(__float_as_uint(big) >> 23)) : 0;
+                    f *= exp2i(-e);
+#pragma unroll
+                    for (int i = 0; i < D / 32; i++) x[i] *= exp2i(e);
+                }
+                if (lane == 0) sh.fac[r] = f;
+                const int byte = lane * (D / 16);  // of the row's D f16
+                const uint32_t at = (byte >> 7) * (KC_M * 128) + kc_sw(r, (byte >> 4) & 7) + (byte & 15);
+#pragma unroll
+                for (int i = 0; i < D / 64; i++) {
+                    const uint32_t h = pack2(x[2 * i], x[2 * i + 1]);
+                    *reinterpret_cast<uint32_t*>(Qh + at + 4 * i) = h;
+                    if constexpr (P::LO) *reinterpret_cast<uint32_t*>(Ql + at + 4 * i) = rest2(x[2 * i], x[2 * i + 1], h);
+                }
+            }
+            fence_proxy_async();
+        }
+        __syncthreads();
+        if (a.parent) {
+            if (tid < sp.m) {
+                int d = -1;
+                for (int i = tid; i >= 0; d++) {
+                    const int p = sh.parent[i];
+                    if (p >= i || p < -1) dev_error(err, DEV_BAD_INDEX);
+                    i = p < i ? p : -1;
+                }
+                sh.depth[tid] = d;
+            }
+            __syncthreads();
+        }
+
+        if (warp >= 8 && warp < 16) {
+            // ---- the staging ----
+            const int lw = warp - 8, lt = tid - 256;
+            Raw raw;
+            const int vb = (seg - cc.first) * KC_KEYS;
+            raw.load_k(c, sp, base, vb, lw, lane);
+            raw.load_v(c, sp, base, vb, lt);
+            bool ok = true;  // (a thread that gave up still meets the others at every tile's barrier)
+            for (int i = 0; i < N; i++) {
+                const int n = n0 + i, st = n % NS, x = n % KC_RING, v0 = vb + i * KC_KEYS;
+                int eK = 0, eV = 0;
+                if (lt < 4) sh.bad[x][lt] = 0u;
+                if constexpr (P::QN) {
+                    uint32_t big = raw.ex[0] & 0x7fff7fffu;
+#pragma unroll
+                    for (int j = 1; j < P::NB / 2; j++) big = h2max(big, raw.ex[j] & 0x7fff7fffu);
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) big = h2max(big, __shfl_xor_sync(FULL, big, o));
+                    if (lane == 0) sh.red[n & 1][lw] = big;
+                }
+                bar_sync(2, KC_LOADERS * 32);
+                if constexpr (P::QN) {
+                    auto exponent = [&](int w) {
+                        uint32_t b = sh.red[n & 1][w];
+                        for (int j = 1; j < KC_LOADERS / 2; j++) b = h2max(b, sh.red[n & 1][w + j]);
+                        const __half2 h = *reinterpret_cast<const __half2*>(&b);
+                        const float f = fmaxf(__low2float(h), __high2float(h));
+                        return f > 0.0f ? min(16, (int)(__float_as_uint(f) >> 23) - 127) : 0;
+                    };
+                    eK = exponent(0), eV = exponent(KC_LOADERS / 2);
+                    if (lt == 0) {
+                        sh.ex[x][0] = eK, sh.ex[x][1] = eV;
+                        mbar_arrive(&sh.xfull[x]);
+                    }
+                }
+                ok = ok && (n < NS || kc_wait(&sh.kempty[st], (n / NS - 1) & 1, abort_flag, err));
+                uint8_t* kh = Kr + st * P::PARTS * P::T_BYTES;
+                if (ok) raw.store_k(kh, kh + P::T_BYTES, eK, lw, lane);
+                fence_proxy_async();
+                __syncwarp();
+                if (ok && lane == 0) mbar_arrive(&sh.kfull[st]);
+                if (i + 1 < N) raw.load_k(c, sp, base, v0 + KC_KEYS, lw, lane);
+                ok = ok && (n < NS || kc_wait(&sh.vempty[st], (n / NS - 1) & 1, abort_flag, err));
+                uint8_t* vh = Vr + st * P::PARTS * P::T_BYTES;
+                if (ok) raw.store_v(vh, vh + P::T_BYTES, eV, edge_of(v0), sh.bad[x], lt);
+                fence_proxy_async();
+                __syncwarp();
+                if (ok && lane == 0) mbar_arrive(&sh.vfull[st]);
+                if (i + 1 < N) raw.load_v(c, sp, base, v0 + KC_KEYS, lt);
+            }
+        } else if (warp == 16) {
+            // ---- the products ----
+            if (lane == 0) {
+                constexpr uint32_t idS = bg_idesc(KC_KEYS), idO = bg_idesc(D);
+                auto qk = [&](int n) -> bool {
+                    const int w = n & 1, st = n % NS;
+                    // P of this group's last tile lies over S: its product is done first
+                    if (n >= 2 && !kc_wait(&sh.odone[w], ((n >> 1) - 1) & 1, abort_flag, err)) return false;
+                    if (!kc_wait(&sh.kfull[st], (n / NS) & 1, abort_flag, err)) return false;
+                    tc_fence_after();
+                    const uint32_t qh = smem_u32(Qh), ql = smem_u32(Ql);
+                    const uint32_t kh = smem_u32(Kr + st * P::PARTS * P::T_BYTES), kl = kh + P::T_BYTES;
+                    const uint32_t tS = tmem + w * KC_KEYS;
+#pragma unroll
+                    for (int k = 0; k < D / 16; k++) {
+                        const uint32_t o = (k >> 2) * (128 * 128) + (k & 3) * 32;
+                        mma_f16(tS, bg_desc(qh + o), bg_desc(kh + o), idS, k > 0 ? 1u : 0u);
+                        if constexpr (P::LO) mma_f16(tS, bg_desc(ql + o), bg_desc(kh + o), idS, 1u);
+                        if constexpr (P::QN) mma_f16(tS, bg_desc(qh + o), bg_desc(kl + o), idS, 1u);
+                    }
+                    mma_commit(&sh.sfull[w]);
+                    mma_commit(&sh.kempty[st]);
+                    any_mma = true;
+                    return true;
+                };
+                bool ok = qk(n0);
+                for (int i = 0; i < N && ok; i++) {
+                    const int n = n0 + i, w = n & 1, st = n % NS;
+                    if (i + 1 < N && !(ok = qk(n + 1))) break;
+                    if (!kc_wait(&sh.pfull[w], (n >> 1) & 1, abort_flag, err) ||
+                        !kc_wait(&sh.vfull[st], (n / NS) & 1, abort_flag, err))
+                        break;
+                    tc_fence_after();
+                    const uint32_t vh = smem_u32(Vr + st * P::PARTS * P::T_BYTES), vl = vh + P::T_BYTES;
+                    const uint32_t tP = tmem + w * KC_KEYS, tO = tmem + 256 + w * 128;
+#pragma unroll
+                    for (int k = 0; k < KC_KEYS / 16; k++) {  // 32 keys' P: hi in 16 columns, lo in the next 16
+                        const uint32_t p = tP + (k >> 1) * 32 + (k & 1) * 8;
+                        const uint32_t o = (k >> 2) * (D * 128) + (k & 3) * 32;
+                        mma_f16_ts(tO, p, bg_desc(vh + o), idO, (i >= 2 || k > 0) ? 1u : 0u);
+                        if constexpr (P::LO) mma_f16_ts(tO, p + 16, bg_desc(vh + o), idO, 1u);
+                        if constexpr (P::QN) mma_f16_ts(tO, p, bg_desc(vl + o), idO, 1u);
+                    }
+                    mma_commit(&sh.odone[w]);
+                    mma_commit(&sh.vempty[st]);
+                }
+            }
+            __syncwarp();
+        } else {
+            // ---- the rows: thread r of group wg owns pair r0 + r (TMEM lane r) ----
+            const int wg = warp >> 2, r = tid & 127;
+            const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+            const uint32_t tS = tmem + lanes + wg * KC_KEYS, tO = tmem + lanes + 256 + wg * 128;
+            const int row = min((r0 + r) / G, sp.m - 1);
+            int at = sp.pos + row;
+            uint64_t anc = 0;
+            if (a.parent) {
+                for (int i = row; i >= 0;) {
+                    anc |= 1ull << i;
+                    const int p = sh.parent[i];
+                    i = p < i ? p : -1;
+                }
+                at = sp.pos + sh.depth[row];
+            }
+            const float fac0 = sh.fac[r];
+            float m = -INFINITY, l = 0.0f;
+            for (int i = (n0 & 1) ^ wg; i < N; i += 2) {
+                const int n = n0 + i, x = n % KC_RING, v0 = (seg - cc.first + i) * KC_KEYS;
+                const bool edge = edge_of(v0);
+                float fac = fac0, ev = 0.0f;
+                if constexpr (P::QN) {
+                    if (!kc_wait_warp(&sh.xfull[x], (n / KC_RING) & 1, abort_flag, err)) break;
+                    fac *= exp2i(sh.ex[x][0]);
+                    ev = (float)sh.ex[x][1];
+                }
+                if (!kc_wait_warp(&sh.sfull[wg], (n >> 1) & 1, abort_flag, err)) break;
+                if (edge && !kc_wait_warp(&sh.vfull[n % NS], (n / NS) & 1, abort_flag, err)) break;  // (the marks)
+                tc_fence_after();
+                // a chunk of 32 scores, what the row does not see taken out
+                auto chunk = [&](int ch, uint32_t* s) {
+                    tmem_ld32(tS + 32 * ch, s);
+                    tmem_wait_ld();
+                    if (!edge) return;
+                    const uint32_t bad = sh.bad[x][ch];
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        const int v = v0 + 32 * ch + j;
+                        bool see = v < sp.nv;
+                        int where = sp.position(v);
+                        if (a.parent) {
+                            if (see && where >= sp.pos) {
+                                see = (anc >> (where - sp.pos)) & 1;
+                                where = sp.pos + sh.depth[where - sp.pos];
+                            }
+                        } else {
+                            see = see && where <= at;
+                        }
+                        if (c.window) see = see && (where > at - c.window || where < c.sinks);
+                        if (!see)
+                            s[j] = 0xff800000u;
+                        else if ((bad >> j) & 1)
+                            s[j] = 0x7fffffffu;
+                    }
+                };
+                float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+                for (int ch = 0; ch < 4; ch++) {
+                    uint32_t s[32];
+                    chunk(ch, s);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) mq[j & 3] = fmaxf(mq[j & 3], __uint_as_float(s[j]));
+                }
+                const float mt = fmaf(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])), fac, ev);
+                if (i < 2) {
+                    m = mt;
+                } else if (__any_sync(FULL, mt > m + KC_LAG)) {
+                    // (warp-uniform: TMEM loads and stores are the whole warp's; a row that stays scales by 1)
+                    if (!kc_wait_warp(&sh.odone[wg], ((n >> 1) - 1) & 1, abort_flag, err)) break;
+                    tc_fence_after();
+                    const bool up = mt > m + KC_LAG;
+                    const float f = up ? ex2(m - mt) : 1.0f;
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(tO + d, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                        tmem_st16(tO + d, o);
+                    }
+                    l *= f;
+                    if (up) m = mt;
+                }
+                const float ref = ev + KC_BIAS - (m == -INFINITY ? 0.0f : m);
+                float sum[2] = {0.0f, 0.0f};
+#pragma unroll 1
+                for (int ch = 0; ch < 4; ch++) {
+                    uint32_t s[32], h[16];
+                    chunk(ch, s);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        const float p = ex2(fmaf(__uint_as_float(s[j]), fac, ref));
+                        s[j] = __float_as_uint(p);
+                        sum[j & 1] += p;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const float p0 = __uint_as_float(s[2 * j]), p1 = __uint_as_float(s[2 * j + 1]);
+                        h[j] = pack2(p0, p1);
+                        if constexpr (P::LO) s[j] = rest2(p0, p1, h[j]);
+                    }
+                    tmem_st16(tS + 32 * ch, h);
+                    if constexpr (P::LO) tmem_st16(tS + 32 * ch + 16, s);
+                }
+                l = fmaf(sum[0] + sum[1], exp2i(P::QN ? -(int)ev : 0), l);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.pfull[wg]);
+            }
+            sh.ml[wg][0][r] = m;
+            sh.ml[wg][1][r] = l;
+            // both groups' products are done: this group's last tile, and the other's
+            bool ok = __all_sync(FULL, *abort_flag == 0);
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                const int last = n0 + N - 1 - ((n0 + N - 1 - w) & 1);  // the last tile of group w
+                if (last >= n0 && ok) ok = kc_wait_warp(&sh.odone[w], (last >> 1) & 1, abort_flag, err);
+            }
+            tc_fence_after();
+            bar_sync(3, 256);
+            // the row's sums: each group writes half of the dims
+            const int w0 = n0 & 1;
+            const bool two = N > 1;
+            const float ma = sh.ml[w0][0][r], mb = two ? sh.ml[w0 ^ 1][0][r] : -INFINITY;
+            const float mx = fmaxf(ma, mb), safe = mx == -INFINITY ? 0.0f : mx;
+            const float fa = ex2(ma - safe), fb = ex2(mb - safe);
+            const float lt = sh.ml[w0][1][r] * fa + (two ? sh.ml[w0 ^ 1][1][r] * fb : 0.0f);
+            const bool whole = N == cc.tiles;
+            const int c0 = whole ? 0 : owner(cc.first);
+            float* mine = reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + KV_TICKETS) +
+                          (size_t)(2 * cta + (cta == c0)) * P::PART;
+            const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+            T* op = static_cast<T*>(a.out) + slot * a.o_slot + ((r0 + r) / G) * a.o_row + (cc.h * G + (r0 + r) % G) * a.o_head;
+            if (ok) {
+#pragma unroll 1
+                for (int d = wg * (D / 2); d < (wg + 1) * (D / 2); d += 16) {
+                    uint32_t o[16], o2[16];
+                    tmem_ld16(tmem + lanes + 256 + w0 * 128 + d, o);
+                    if (two) tmem_ld16(tmem + lanes + 256 + (w0 ^ 1) * 128 + d, o2);
+                    tmem_wait_ld();
+                    float y[16];
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        y[j] = __uint_as_float(o[j]) * fa;
+                        if (two) y[j] = fmaf(__uint_as_float(o2[j]), fb, y[j]);
+                    }
+                    if (!whole) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++) __stcg(&mine[(d + j) * KC_M + r], y[j]);
+                    } else if (r < rows) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++) y[j] = lt == 0.0f ? 0.0f : y[j] * inv;
+                        if constexpr (P::LO) {
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                *reinterpret_cast<float4*>(op + d + 4 * j) = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 2; j++)
+                                *reinterpret_cast<uint4*>(op + d + 8 * j) =
+                                    make_uint4(pack2(y[8 * j], y[8 * j + 1]), pack2(y[8 * j + 2], y[8 * j + 3]),
+                                               pack2(y[8 * j + 4], y[8 * j + 5]), pack2(y[8 * j + 6], y[8 * j + 7]));
+                        }
+                    }
+                }
+                if (!whole && wg == 0) {
+                    __stcg(&mine[D * KC_M + r], mx);
+                    __stcg(&mine[(D + 1) * KC_M + r], lt);
+                }
+                __threadfence();
+            }
+            tc_fence_before();
+        }
+        __syncthreads();
+        tc_fence_after();
+        if (*abort_flag) break;
+        // ---- a triple that lies in several CTAs: the last of them joins the parts in the CTAs' order ----
+        if (N != cc.tiles) {
+            const int c0 = owner(cc.first), c1 = owner(cc.first + cc.tiles - 1);
+            uint32_t* tickets = static_cast<uint32_t*>(a.work);
+            if (tid == 0) {
+                const bool last = atomicAdd(&tickets[c0], 1u) == (uint32_t)(c1 - c0);
+                if (last) tickets[c0] = 0;
+                __threadfence();
+                sh.last = last;
+            }
+            __syncthreads();
+            if (sh.last && tid < 512) {
+                const int r = tid & 127, d0 = (tid >> 7) * (D / 4);
+                const float* parts = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.work) + KV_TICKETS);
+                auto of = [&](int i) { return parts + (size_t)(2 * i + (i == c0)) * P::PART; };
+                float mx = -INFINITY, l = 0.0f, y[D / 4] = {};
+                for (int i = c0; i <= c1; i++) mx = fmaxf(mx, __ldcg(&of(i)[D * KC_M + r]));
+                if (mx == -INFINITY) mx = 0.0f;
+                for (int i = c0; i <= c1; i++) {
+                    const float* q = of(i);
+                    const float f = ex2(__ldcg(&q[D * KC_M + r]) - mx);
+                    l = fmaf(__ldcg(&q[(D + 1) * KC_M + r]), f, l);
+#pragma unroll
+                    for (int d = 0; d < D / 4; d++) y[d] = fmaf(__ldcg(&q[(d0 + d) * KC_M + r]), f, y[d]);
+                }
+                if (r < rows) {
+                    T* op = static_cast<T*>(a.out) + slot * a.o_slot + ((r0 + r) / G) * a.o_row +
+                            (cc.h * G + (r0 + r) % G) * a.o_head + d0;
+                    const float inv = 1.0f / l;
+#pragma unroll
+                    for (int d = 0; d < D / 4; d++) op[d] = (T)(l == 0.0f ? 0.0f : y[d] * inv);
+                }
+            }
+        }
+        n0 += N;
+        seg = seg_end;
+    }
+    // ---- every product complete before the TMEM is given back ----
+    if (warp == 16) {
+        if (lane == 0 && any_mma) {
+            mma_commit(&sh.mdone);
+            mbar_wait(&sh.mdone, 0, err);
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 16) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <int TYPE, int D, class T>
+static cudaError_t launch_tc(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
+    using P = KcPlan<TYPE, D, T>;
+    static PerDeviceOnce once;
+    once([] { cudaFuncSetAttribute(k_kv_attn_tc<TYPE, D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::SMEM); });
+    const int blocks = (int)(((long)a.r.T * (a.n_head / a.c.n_kv) + KC_M - 1) / KC_M);
+    const bool line = (long)a.c.n_slot * blocks <= KV_LINE;
+    const long grid = line ? a.num_sms : (long)a.c.n_slot * blocks * a.c.n_kv;
+    return kv_launch(k_kv_attn_tc<TYPE, D, T>, dim3((unsigned)grid), KC_THREADS, P::SMEM, st, pdl, a, blocks, line ? 1 : 0);
+}
+template <int TYPE>
+static cudaError_t launch_type(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
+    if (a.c.d == 128) return a.half ? launch_tc<TYPE, 128, __half>(st, a, pdl) : launch_tc<TYPE, 128, float>(st, a, pdl);
+    return a.half ? launch_tc<TYPE, 64, __half>(st, a, pdl) : launch_tc<TYPE, 64, float>(st, a, pdl);
+}
+// tickets, and two parts for each CTA
+size_t kv_attention_many_work(const KvAttnArgs& a) { return KV_TICKETS + (size_t)a.num_sms * 2 * (a.c.d + 2) * KC_M * 4; }
+cudaError_t launch_kv_attention_many(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
+    switch (a.c.type) {
+        case KV_F16: return launch_type<KV_F16>(st, a, pdl);
+        case KV_Q8_0: return launch_type<KV_Q8_0>(st, a, pdl);
+        default: return launch_type<KV_Q4_0>(st, a, pdl);
+    }
+}
+
+}  // namespace ocr

@@ -111,8 +111,9 @@ inline KvAttnArgs kv_slots(const KvAttnArgs& all, int b, int n) {
     a.out = static_cast<char*>(a.out) + b * a.o_slot * item;
     return a;
 }
-cudaError_t launch_kv_attention_few(cudaStream_t st, const KvAttnArgs& a, bool pdl);
 cudaError_t launch_kv_attention(cudaStream_t st, const KvAttnArgs& a, bool pdl);
+cudaError_t launch_kv_attention_many(cudaStream_t st, const KvAttnArgs& a, bool pdl);
+size_t kv_attention_many_work(const KvAttnArgs& a);
 size_t kv_attention_work_bytes(const KvAttnArgs& a);
 
 // a launch that may start while its predecessor on the stream still runs: the kernel calls pdl_wait() before it

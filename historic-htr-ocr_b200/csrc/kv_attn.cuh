@@ -1,0 +1,82 @@
+// kv_attn.cuh — what the two attentions over a KV cache share (k_kv_attn.cu: a few rows per kv head; k_kv_attn_tc.cu:
+// many): the line of key tiles that is cut evenly over the CTAs, the positions that a range of rows sees, the quants'
+// way to f16.
+#pragma once
+
+#include "kv.cuh"
+
+namespace ocr {
+
+constexpr int KV_LINE = 512;      // entries (slots, or slots x row blocks) whose prefix sums a CTA holds
+constexpr int KV_TICKETS = 4096;  // bytes of the workspace before the partial results: a ticket per CTA
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// the remainders of a and b past their f16 rounding `hi`
+__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t hi) {
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    return pack2(a - h.x, b - h.y);
+}
+// an unsigned byte pair placed as halves of 1024 + u, less `bias`
+__device__ __forceinline__ uint32_t bytes_h2(uint32_t w, uint32_t sel, uint32_t bias) {
+    const uint32_t m = __byte_perm(w, 0x64646464u, sel);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&m), *reinterpret_cast<const __half2*>(&bias));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+constexpr uint32_t H2_1152 = 0x64806480u;  // 1024 + 128: an int8 with its sign bit flipped
+// the low (SHIFT = 0) or high nibbles of bytes 0 and 2 of w, less 8
+template <bool HIGH>
+__device__ __forceinline__ uint32_t nibbles_h2(uint32_t w) {
+    const uint32_t m = (w & (HIGH ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;  // 1024 + n, or 1024 + 16 n
+    const __half2 x = *reinterpret_cast<const __half2*>(&m);
+    __half2 r;
+    if (HIGH)
+        r = __hfma2(x, __float2half2_rn(0.0625f), __float2half2_rn(-72.0f));
+    else
+        r = __hsub2(x, __float2half2_rn(1032.0f));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// the keys that rows t0 … t1 - 1 of a slot's call see together, in order: the sinks that lie before the first row's
+// window, then positions lo … end - 1 (drafts: every row may stand at the first position)
+struct KvSpan {
+    int pos, m, lo, ns, nv;  // m: the slot's rows in use
+    __device__ __forceinline__ void set(const KvAttnArgs& a, int b, int t0, int t1) {
+        pos = a.r.pos[b];
+        m = a.r.rows(a.c, b, a.err);
+        const int first = pos + (a.parent ? 0 : t0);
+        lo = a.c.window ? max(0, first - a.c.window + 1) : 0;
+        ns = min(a.c.sinks, lo);
+        nv = t0 < m ? ns + pos + (a.parent ? m : min(t1, m)) - lo : 0;
+    }
+    __device__ __forceinline__ int position(int v) const { return v < ns ? v : lo + v - ns; }
+};
+
+// where a CTA stands in the line of tiles
+struct KvCursor {
+    int b, h, first, tiles;  // the entry and the kv head, the first of its tiles in the line, their number
+    __device__ __forceinline__ void at(int g, const int* prefix, int n, int n_kv) {  // the pair of tile g
+        int lo = 0, hi = n;  // prefix[lo] <= g < prefix[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (prefix[mid] <= g)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        b = lo;
+        tiles = (prefix[b + 1] - prefix[b]) / n_kv;
+        h = (g - prefix[b]) / tiles;
+        first = prefix[b] + h * tiles;
+    }
+};
+
+}  // namespace ocr

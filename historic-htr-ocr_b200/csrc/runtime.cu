@@ -76,6 +76,8 @@ ocr_status check_device_error(ocr_ctx* ctx) {
     OCR_CUDA(cudaMemcpy(&err, ctx->d_err, sizeof(int), cudaMemcpyDeviceToHost));
     if (err != DEV_OK) {
         OCR_CUDA(cudaMemsetAsync(ctx->d_err, 0, sizeof(int), ctx->stream));  // (ordered before later kernels)
+        // a kernel that gave up may have left the KV attentions' tickets short
+        if (err == DEV_TIMEOUT && ctx->kv_work) OCR_CUDA(cudaMemsetAsync(ctx->kv_work, 0, 4096, ctx->stream));
         return fail(OCR_ERR_DEVICE, err == DEV_BAD_POS     ? "a kernel saw a position outside the KV cache"
                                     : err == DEV_TIMEOUT ? "a kernel's bounded wait ran out (its work was skipped)"
                                                          : "a kernel saw an index outside its buffer");
