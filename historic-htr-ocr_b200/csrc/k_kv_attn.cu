@@ -94,8 +94,8 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int prefix[KV_LINE + 1];
     __shared__ int wsum[KA_WARPS];
-    __shared__ int s_at[8 * WR], s_depth[KV_TREE_MAX];
-    __shared__ uint64_t s_anc[8 * WR];
+    __shared__ int s_parent[KV_TREE_MAX], s_depth[KV_TREE_MAX];
+    __shared__ KvSight s_sight[8 * WR];
     __shared__ float s_ml[KA_WARPS][16];
     __shared__ int s_last;
     pdl_trigger();
@@ -143,13 +143,9 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
     const int n_cta = min((int)gridDim.x, (total + TEAMS - 1) / TEAMS);
     const int cta = blockIdx.x;
     if (cta >= n_cta) return;
-    auto part = [&](int i) { return (int)((long)total * i / n_cta); };
-    auto owner = [&](int tile) {  // the CTA whose part holds it
-        int i = (int)(((long)tile * n_cta) / total);
-        while (part(i + 1) <= tile) i++;
-        return i;
-    };
-    const int begin = part(cta), end = part(cta + 1);
+    KvLine cut;
+    cut.cut(total, n_cta);
+    const int begin = cut.part(cta), end = cut.part(cta + 1);
 
     uint8_t* ring = smem + team * WR * KA_RING;
     float* joined = reinterpret_cast<float*>(smem + KA_WARPS * KA_RING);  // [4 warps][D / 4 registers][32 lanes]
@@ -207,31 +203,18 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
         const bool many = a.r.T > 1;
         // ---- what each row sees ----
         if (many) {
-            const int32_t* parent = a.parent ? a.parent + (size_t)cc.b * a.r.T : nullptr;
-            for (int r = tid; r < max(8 * WR, parent ? sp.m : 0); r += KA_THREADS) {
-                const int row = min(r / G, sp.m - 1);
-                int at = sp.pos + row;
-                if (parent) {
-                    uint64_t anc = 0;
-                    auto climb = [&](int i, bool set) {
-                        int depth = -1;
-                        while (i >= 0) {
-                            depth++;
-                            if (set) anc |= 1ull << i;
-                            const int p = parent[i];
-                            if (p >= i || p < -1) {
-                                dev_error(a.err, DEV_BAD_INDEX);
-                                break;
-                            }
-                            i = p;
-                        }
-                        return depth;
-                    };
-                    at = sp.pos + climb(row, true);
-                    if (r < 8 * WR) s_anc[r] = anc;
-                    if (r < sp.m) s_depth[r] = climb(r, false);
-                }
-                if (r < 8 * WR) s_at[r] = at;
+            if (a.parent) {
+                if (tid < sp.m) s_parent[tid] = a.parent[(size_t)cc.b * a.r.T + tid];
+                __syncthreads();
+                if (tid < sp.m) s_depth[tid] = kv_depth(tid, s_parent, a.err);
+                __syncthreads();
+            }
+            if (tid < 8 * WR) {
+                const int row = min(tid / G, sp.m - 1);
+                if (a.parent)
+                    kv_draft(c, sp, row, s_parent, s_depth, s_sight[tid]);
+                else
+                    s_sight[tid].rows(c, sp, sp.pos + row, sp.pos + row);
             }
             __syncthreads();
         }
@@ -365,25 +348,21 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
                     }
                 }
                 seen = 0;
+                uint32_t mask[2][(KEYS + 31) / 32];  // the tile's keys that the lane's two rows see
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+#pragma unroll
+                    for (int w = 0; w < (KEYS + 31) / 32; w++) {
+                        const int v = v0 + 32 * w, left = sp.nv - v;
+                        mask[j][w] = many ? s_sight[8 * wr + 2 * t + j].mask(v)
+                                          : left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;
+                    }
 #pragma unroll
                 for (int i = 0; i < MT; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const int kk = key(i, j >> 1), v = v0 + kk;
-                        bool s = v < sp.nv;
-                        if (s && many) {
-                            const int r = 8 * wr + 2 * t + (j & 1), at = s_at[r];
-                            int where = sp.position(v);
-                            if (a.parent) {
-                                if (where >= sp.pos) {
-                                    s = (s_anc[r] >> (where - sp.pos)) & 1;
-                                    where = sp.pos + s_depth[where - sp.pos];
-                                }
-                            } else {
-                                s = where <= at;
-                            }
-                            if (c.window) s = s && (where > at - c.window || where < c.sinks);
-                        }
+                        const int kk = key(i, j >> 1);
+                        const bool s = (mask[j & 1][i / 2] >> (kk & 31)) & 1;
                         if (s) seen |= 1u << (4 * i + j);
                         if (TYPE == KV_F16 && s && ((bad >> kk) & 1)) p[i][j] = NAN;
                         if (!s) p[i][j] = -INFINITY;
@@ -620,7 +599,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
             constexpr int PART = WR * (D * 8 + 16);
             uint32_t* tickets = static_cast<uint32_t*>(a.work);
             float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + KV_TICKETS);
-            const int c0 = owner(cc.first), c1 = owner(cc.first + cc.tiles - 1);
+            const int c0 = cut.owner(cc.first), c1 = cut.owner(cc.first + cc.tiles - 1);
             float* mine = parts + (size_t)(2 * cta + (cta == c0)) * PART;
             if (team == 0) {
 #pragma unroll

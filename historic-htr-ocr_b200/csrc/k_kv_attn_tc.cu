@@ -36,6 +36,20 @@ constexpr int KC_THREADS = (8 + KC_LOADERS + 1) * 32;
 constexpr int KC_RING = 4;  // tiles whose exponents and marks are kept
 constexpr float KC_LAG = 6.0f, KC_BIAS = 8.0f;
 
+template <int BYTES>
+struct KcWord;
+template <>
+struct KcWord<16> {
+    using type = uint4;
+};
+template <>
+struct KcWord<8> {
+    using type = uint2;
+};
+template <>
+struct KcWord<4> {
+    using type = uint32_t;
+};
 template <int TYPE, int D, class T>
 struct KcPlan {
     static constexpr bool LO = sizeof(T) == 4, QN = TYPE != KV_F16;
@@ -132,53 +146,92 @@ struct KcRaw {
         return half < 2;
     }
 
-    __device__ __forceinline__ void load_k(const KvView& c, const KvSpan& s, size_t base, int v0, int lw, int lane) {
+    // Loads of the tile at key v0. Where its 128 rows lie one after another (all but the tiles at an end of the span, of
+    // the sinks or of a ring), the addresses are one base and constants.
+    struct Tile {
+        size_t row;  // of the first key
+        int v0;
+        bool run;
+        __device__ __forceinline__ Tile(const KvView& c, const KvSpan& s, size_t base, int v) : v0(v) {
+            const int r = kv_row(c, s.position(v)), last = v + KC_KEYS - 1;
+            run = last < s.nv && (v >= s.ns || last < s.ns) && kv_row(c, s.position(last)) - r == KC_KEYS - 1;
+            row = base + r;
+        }
+    };
+    __device__ __forceinline__ void load_k(const KvView& c, const KvSpan& s, size_t base, const Tile& t, int lw, int lane) {
+        const int ekey = (lw * 32 + lane) & (KC_KEYS - 1);  // threads 0 … 127: K's scales of a key, the others V's
+        const __half* es = lw < KC_LOADERS / 2 ? c.ks : c.vs;
+        if (t.run) {
+            int key, u;
+            unit(0, lw, lane, key, u);
+            constexpr int STEP = KC_KEYS / KU;  // keys from one piece of a thread to its next
+            const uint8_t* p = c.k + (t.row + key) * ROW + u * 16;
+            const __half* d = c.ks + (t.row + key) * NB + (TYPE == KV_Q8_0 ? u >> 1 : u);
+#pragma unroll
+            for (int i = 0; i < KU; i++) {
+                k[i] = *reinterpret_cast<const uint4*>(p + i * STEP * ROW);
+                if constexpr (QN) kd[i] = d[i * STEP * NB];
+            }
+            if constexpr (QN) {
+                const uint32_t* e = reinterpret_cast<const uint32_t*>(es + (t.row + ekey) * NB);
+#pragma unroll
+                for (int j = 0; j < NB / 2; j++) ex[j] = e[j];
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < KU; i++) {
             int key, u;
             unit(i, lw, lane, key, u);
             k[i] = make_uint4(0u, 0u, 0u, 0u);
             kd[i] = __ushort_as_half(0);
-            if (v0 + key < s.nv) {
-                const size_t row = base + kv_row(c, s.position(v0 + key));
+            if (t.v0 + key < s.nv) {
+                const size_t row = base + kv_row(c, s.position(t.v0 + key));
                 k[i] = *reinterpret_cast<const uint4*>(c.k + row * ROW + u * 16);
                 if constexpr (QN) kd[i] = c.ks[row * NB + (TYPE == KV_Q8_0 ? u >> 1 : u)];
             }
         }
-        if constexpr (QN) {  // the scales of one key: K's for threads 0 … 127, V's for the others
-            const int key = (lw * 32 + lane) & (KC_KEYS - 1);
+        if constexpr (QN) {
 #pragma unroll
             for (int j = 0; j < NB / 2; j++) ex[j] = 0u;
-            if (v0 + key < s.nv) {
-                const size_t row = base + kv_row(c, s.position(v0 + key));
-                const uint32_t* p = reinterpret_cast<const uint32_t*>((lw < KC_LOADERS / 2 ? c.ks : c.vs) + row * NB);
+            if (t.v0 + ekey < s.nv) {
+                const size_t row = base + kv_row(c, s.position(t.v0 + ekey));
 #pragma unroll
-                for (int j = 0; j < NB / 2; j++) ex[j] = p[j];
+                for (int j = 0; j < NB / 2; j++) ex[j] = reinterpret_cast<const uint32_t*>(es + row * NB)[j];
             }
         }
     }
-    __device__ __forceinline__ void load_v(const KvView& c, const KvSpan& s, size_t base, int v0, int lt) {
+    __device__ __forceinline__ void load_v(const KvView& c, const KvSpan& s, size_t base, const Tile& t, int lt) {
         int ka, b, half;
-        const bool on = block(lt, ka, b, half);
+        if (!block(lt, ka, b, half)) return;
+        const int key0 = 64 * half + 8 * ka;
+        auto one = [&](int i, const uint8_t* p, const __half* d) {
+            if constexpr (VW == 4) {
+                const uint4 x = *reinterpret_cast<const uint4*>(p);
+                v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+            } else if constexpr (VW == 2) {
+                const uint2 x = *reinterpret_cast<const uint2*>(p);
+                v[i][0] = x.x, v[i][1] = x.y;
+            } else {
+                v[i][0] = *reinterpret_cast<const uint32_t*>(p);
+            }
+            if constexpr (QN) vd[i] = *d;
+        };
+        if (t.run) {
+            const uint8_t* p = c.v + (t.row + key0) * ROW + b * (VW * 4);
+            const __half* d = c.vs + (t.row + key0) * NB + b / 4;
+#pragma unroll
+            for (int i = 0; i < 8; i++) one(i, p + i * ROW, d + i * NB);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const int key = 64 * half + 8 * ka + i;
 #pragma unroll
             for (int j = 0; j < VW; j++) v[i][j] = 0u;
             vd[i] = __ushort_as_half(0);
-            if (on && v0 + key < s.nv) {
-                const size_t row = base + kv_row(c, s.position(v0 + key));
-                const uint8_t* p = c.v + row * ROW + b * (VW * 4);
-                if constexpr (VW == 4) {
-                    const uint4 x = *reinterpret_cast<const uint4*>(p);
-                    v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
-                } else if constexpr (VW == 2) {
-                    const uint2 x = *reinterpret_cast<const uint2*>(p);
-                    v[i][0] = x.x, v[i][1] = x.y;
-                } else {
-                    v[i][0] = *reinterpret_cast<const uint32_t*>(p);
-                }
-                if constexpr (QN) vd[i] = c.vs[row * NB + b / 4];
+            if (t.v0 + key0 + i < s.nv) {
+                const size_t row = base + kv_row(c, s.position(t.v0 + key0 + i));
+                one(i, c.v + row * ROW + b * (VW * 4), c.vs + row * NB + b / 4);
             }
         }
     }
@@ -377,16 +430,12 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
     const uint32_t tmem = sh.tmem;
     const int n_cta = line ? min((int)gridDim.x, total) : (int)gridDim.x;
     const int cta = blockIdx.x;
-    auto part = [&](int i) { return (int)((long)total * i / n_cta); };
-    auto owner = [&](int tile) {
-        int i = (int)(((long)tile * n_cta) / total);
-        while (part(i + 1) <= tile) i++;
-        return i;
-    };
+    KvLine cut;
+    cut.cut(total, n_cta);
     int begin = 0, end = 0;
     KvCursor cc;
     if (line) {
-        if (cta < n_cta) begin = part(cta), end = part(cta + 1);
+        if (cta < n_cta) begin = cut.part(cta), end = cut.part(cta + 1);
     } else {  // one triple, the last row blocks (the longest) first
         const int per = c.n_slot * c.n_kv;
         const int blk = blocks - 1 - cta / per, b = cta % per / c.n_kv;
@@ -424,33 +473,43 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
         if (a.parent && tid < sp.m) sh.parent[tid] = a.parent[(size_t)slot * a.r.T + tid];
         // ---- the queries: hi and lo, a row per warp at a time ----
         if (warp < 16) {
-            for (int r = warp; r < KC_M; r += 16) {
-                const int row = r0 + r;
-                const bool live = r < rows;
+            constexpr int R = KC_M / 16, V = D / 32;  // a lane's dims
+            alignas(16) T q[R][V];
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                const int r = warp + 16 * i, row = r0 + r;
                 const T* qp = static_cast<const T*>(a.q) + slot * a.q_slot + (row / G) * a.q_row +
-                              (cc.h * G + row % G) * a.q_head + lane * (D / 32);
-                float x[D / 32];
+                              (cc.h * G + row % G) * a.q_head + lane * V;
+                using Word = typename KcWord<V * sizeof(T)>::type;
+                Word w = {};
+                if (r < rows) w = *reinterpret_cast<const Word*>(qp);
+                *reinterpret_cast<Word*>(q[i]) = w;
+            }
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                const int r = warp + 16 * i;
+                float x[V];
                 float f = a.scale * LOG2E;
 #pragma unroll
-                for (int i = 0; i < D / 32; i++) x[i] = live ? (float)qp[i] : 0.0f;
+                for (int j = 0; j < V; j++) x[j] = (float)q[i][j];
                 if constexpr (P::LO) {  // the row's largest to 2^10 … 2^11
                     float big = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < D / 32; i++) big = fmaxf(big, fabsf(x[i]));
+                    for (int j = 0; j < V; j++) big = fmaxf(big, fabsf(x[j]));
                     big = warp_max(big);
                     const int e = big > 0.0f && big <= 3.4028234e38f ? min(100, 137 - (int)(__float_as_uint(big) >> 23)) : 0;
                     f *= exp2i(-e);
 #pragma unroll
-                    for (int i = 0; i < D / 32; i++) x[i] *= exp2i(e);
+                    for (int j = 0; j < V; j++) x[j] *= exp2i(e);
                 }
                 if (lane == 0) sh.fac[r] = f;
                 const int byte = lane * (D / 16);  // of the row's D f16
                 const uint32_t at = (byte >> 7) * (KC_M * 128) + kc_sw(r, (byte >> 4) & 7) + (byte & 15);
 #pragma unroll
-                for (int i = 0; i < D / 64; i++) {
-                    const uint32_t h = pack2(x[2 * i], x[2 * i + 1]);
-                    *reinterpret_cast<uint32_t*>(Qh + at + 4 * i) = h;
-                    if constexpr (P::LO) *reinterpret_cast<uint32_t*>(Ql + at + 4 * i) = rest2(x[2 * i], x[2 * i + 1], h);
+                for (int j = 0; j < V / 2; j++) {
+                    const uint32_t h = pack2(x[2 * j], x[2 * j + 1]);
+                    *reinterpret_cast<uint32_t*>(Qh + at + 4 * j) = h;
+                    if constexpr (P::LO) *reinterpret_cast<uint32_t*>(Ql + at + 4 * j) = rest2(x[2 * j], x[2 * j + 1], h);
                 }
             }
             fence_proxy_async();
@@ -458,13 +517,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
         __syncthreads();
         if (a.parent) {
             if (tid < sp.m) {
-                int d = -1;
-                for (int i = tid; i >= 0; d++) {
-                    const int p = sh.parent[i];
-                    if (p >= i || p < -1) dev_error(err, DEV_BAD_INDEX);
-                    i = p < i ? p : -1;
-                }
-                sh.depth[tid] = d;
+                sh.depth[tid] = kv_depth(tid, sh.parent, err);
             }
             __syncthreads();
         }
@@ -474,8 +527,9 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             const int lw = warp - 8, lt = tid - 256;
             Raw raw;
             const int vb = (seg - cc.first) * KC_KEYS;
-            raw.load_k(c, sp, base, vb, lw, lane);
-            raw.load_v(c, sp, base, vb, lt);
+            typename Raw::Tile next(c, sp, base, vb);
+            raw.load_k(c, sp, base, next, lw, lane);
+            raw.load_v(c, sp, base, next, lt);
             bool ok = true;  // (a thread that gave up still meets the others at every tile's barrier)
             for (int i = 0; i < N; i++) {
                 const int n = n0 + i, st = n % NS, x = n % KC_RING, v0 = vb + i * KC_KEYS;
@@ -510,14 +564,17 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 fence_proxy_async();
                 __syncwarp();
                 if (ok && lane == 0) mbar_arrive(&sh.kfull[st]);
-                if (i + 1 < N) raw.load_k(c, sp, base, v0 + KC_KEYS, lw, lane);
+                if (i + 1 < N) {
+                    next = typename Raw::Tile(c, sp, base, v0 + KC_KEYS);
+                    raw.load_k(c, sp, base, next, lw, lane);
+                }
                 ok = ok && (n < NS || kc_wait(&sh.vempty[st], (n / NS - 1) & 1, abort_flag, err));
                 uint8_t* vh = Vr + st * P::PARTS * P::T_BYTES;
                 if (ok) raw.store_v(vh, vh + P::T_BYTES, eV, edge_of(v0), sh.bad[x], lt);
                 fence_proxy_async();
                 __syncwarp();
                 if (ok && lane == 0) mbar_arrive(&sh.vfull[st]);
-                if (i + 1 < N) raw.load_v(c, sp, base, v0 + KC_KEYS, lt);
+                if (i + 1 < N) raw.load_v(c, sp, base, next, lt);
             }
         } else if (warp == 16) {
             // ---- the products ----
@@ -532,13 +589,16 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                     const uint32_t qh = smem_u32(Qh), ql = smem_u32(Ql);
                     const uint32_t kh = smem_u32(Kr + st * P::PARTS * P::T_BYTES), kl = kh + P::T_BYTES;
                     const uint32_t tS = tmem + w * KC_KEYS;
+                    // the small products first: a sum loses what falls below its last bit at every product added
+                    constexpr int SMALL = (P::LO ? 1 : 0) + (P::QN ? 1 : 0);
 #pragma unroll
-                    for (int k = 0; k < D / 16; k++) {
-                        const uint32_t o = (k >> 2) * (128 * 128) + (k & 3) * 32;
-                        mma_f16(tS, bg_desc(qh + o), bg_desc(kh + o), idS, k > 0 ? 1u : 0u);
-                        if constexpr (P::LO) mma_f16(tS, bg_desc(ql + o), bg_desc(kh + o), idS, 1u);
-                        if constexpr (P::QN) mma_f16(tS, bg_desc(qh + o), bg_desc(kl + o), idS, 1u);
-                    }
+                    for (int x = 0; x <= SMALL; x++)
+#pragma unroll
+                        for (int k = 0; k < D / 16; k++) {
+                            const uint32_t o = (k >> 2) * (128 * 128) + (k & 3) * 32;
+                            const bool lq = P::LO && x == 0, lk = P::QN && x == (P::LO ? 1 : 0);
+                            mma_f16(tS, bg_desc((lq ? ql : qh) + o), bg_desc((lk ? kl : kh) + o), idS, x + k > 0 ? 1u : 0u);
+                        }
                     mma_commit(&sh.sfull[w]);
                     mma_commit(&sh.kempty[st]);
                     any_mma = true;
@@ -573,16 +633,11 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
             const uint32_t tS = tmem + lanes + wg * KC_KEYS, tO = tmem + lanes + 256 + wg * 128;
             const int row = min((r0 + r) / G, sp.m - 1);
-            int at = sp.pos + row;
-            uint64_t anc = 0;
-            if (a.parent) {
-                for (int i = row; i >= 0;) {
-                    anc |= 1ull << i;
-                    const int p = sh.parent[i];
-                    i = p < i ? p : -1;
-                }
-                at = sp.pos + sh.depth[row];
-            }
+            KvSight sight;
+            if (a.parent)
+                kv_draft(c, sp, row, sh.parent, sh.depth, sight);
+            else
+                sight.rows(c, sp, sp.pos + row, sp.pos + row);
             const float fac0 = sh.fac[r];
             float m = -INFINITY, l = 0.0f;
             for (int i = (n0 & 1) ^ wg; i < N; i += 2) {
@@ -602,25 +657,14 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                     tmem_ld32(tS + 32 * ch, s);
                     tmem_wait_ld();
                     if (!edge) return;
-                    const uint32_t bad = sh.bad[x][ch];
+                    const uint32_t see = sight.mask(v0 + 32 * ch), bad = sh.bad[x][ch] & see;
 #pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const int v = v0 + 32 * ch + j;
-                        bool see = v < sp.nv;
-                        int where = sp.position(v);
-                        if (a.parent) {
-                            if (see && where >= sp.pos) {
-                                see = (anc >> (where - sp.pos)) & 1;
-                                where = sp.pos + sh.depth[where - sp.pos];
-                            }
-                        } else {
-                            see = see && where <= at;
-                        }
-                        if (c.window) see = see && (where > at - c.window || where < c.sinks);
-                        if (!see)
-                            s[j] = 0xff800000u;
-                        else if ((bad >> j) & 1)
-                            s[j] = 0x7fffffffu;
+                    for (int j = 0; j < 32; j++)
+                        if (!((see >> j) & 1)) s[j] = 0xff800000u;
+                    if (bad) {
+#pragma unroll
+                        for (int j = 0; j < 32; j++)
+                            if ((bad >> j) & 1) s[j] = 0x7fffffffu;
                     }
                 };
                 float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -698,11 +742,12 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             const float fa = ex2(ma - safe), fb = ex2(mb - safe);
             const float lt = sh.ml[w0][1][r] * fa + (two ? sh.ml[w0 ^ 1][1][r] * fb : 0.0f);
             const bool whole = N == cc.tiles;
-            const int c0 = whole ? 0 : owner(cc.first);
+            const int c0 = whole ? 0 : cut.owner(cc.first);
             float* mine = reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + KV_TICKETS) +
                           (size_t)(2 * cta + (cta == c0)) * P::PART;
             const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
-            T* op = static_cast<T*>(a.out) + slot * a.o_slot + ((r0 + r) / G) * a.o_row + (cc.h * G + (r0 + r) % G) * a.o_head;
+            // (Q's memory is free: every product is done) the rows of the output, 16-byte pieces moved among eight
+            constexpr int ROW = D * sizeof(T);
             if (ok) {
 #pragma unroll 1
                 for (int d = wg * (D / 2); d < (wg + 1) * (D / 2); d += 16) {
@@ -719,27 +764,38 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                     if (!whole) {
 #pragma unroll
                         for (int j = 0; j < 16; j++) __stcg(&mine[(d + j) * KC_M + r], y[j]);
-                    } else if (r < rows) {
+                        continue;
+                    }
 #pragma unroll
-                        for (int j = 0; j < 16; j++) y[j] = lt == 0.0f ? 0.0f : y[j] * inv;
-                        if constexpr (P::LO) {
+                    for (int j = 0; j < 16; j++) y[j] = lt == 0.0f ? 0.0f : y[j] * inv;
+                    constexpr int E = 16 / sizeof(T);  // elements of a piece
 #pragma unroll
-                            for (int j = 0; j < 4; j++)
-                                *reinterpret_cast<float4*>(op + d + 4 * j) = make_float4(y[4 * j], y[4 * j + 1], y[4 * j + 2], y[4 * j + 3]);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 2; j++)
-                                *reinterpret_cast<uint4*>(op + d + 8 * j) =
-                                    make_uint4(pack2(y[8 * j], y[8 * j + 1]), pack2(y[8 * j + 2], y[8 * j + 3]),
-                                               pack2(y[8 * j + 4], y[8 * j + 5]), pack2(y[8 * j + 6], y[8 * j + 7]));
-                        }
+                    for (int j = 0; j < 16 / E; j++) {
+                        uint4 w;
+                        if constexpr (P::LO)
+                            w = make_uint4(__float_as_uint(y[4 * j]), __float_as_uint(y[4 * j + 1]),
+                                           __float_as_uint(y[4 * j + 2]), __float_as_uint(y[4 * j + 3]));
+                        else
+                            w = make_uint4(pack2(y[8 * j], y[8 * j + 1]), pack2(y[8 * j + 2], y[8 * j + 3]),
+                                           pack2(y[8 * j + 4], y[8 * j + 5]), pack2(y[8 * j + 6], y[8 * j + 7]));
+                        *reinterpret_cast<uint4*>(Qh + r * ROW + (((d / E + j) ^ (r & 7)) << 4)) = w;
+                    }
+                }
+                if (whole) {
+                    bar_sync(3, 256);
+                    constexpr int PC = ROW / 16;
+                    for (int e = tid; e < rows * PC; e += 256) {
+                        const int rr = e / PC, pc = e % PC;
+                        T* op = static_cast<T*>(a.out) + slot * a.o_slot + ((r0 + rr) / G) * a.o_row +
+                                (cc.h * G + (r0 + rr) % G) * a.o_head;
+                        reinterpret_cast<uint4*>(op)[pc] = *reinterpret_cast<const uint4*>(Qh + rr * ROW + ((pc ^ (rr & 7)) << 4));
                     }
                 }
                 if (!whole && wg == 0) {
                     __stcg(&mine[D * KC_M + r], mx);
                     __stcg(&mine[(D + 1) * KC_M + r], lt);
                 }
-                __threadfence();
+                if (!whole) __threadfence();
             }
             tc_fence_before();
         }
@@ -748,7 +804,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
         if (*abort_flag) break;
         // ---- a triple that lies in several CTAs: the last of them joins the parts in the CTAs' order ----
         if (N != cc.tiles) {
-            const int c0 = owner(cc.first), c1 = owner(cc.first + cc.tiles - 1);
+            const int c0 = cut.owner(cc.first), c1 = cut.owner(cc.first + cc.tiles - 1);
             uint32_t* tickets = static_cast<uint32_t*>(a.work);
             if (tid == 0) {
                 const bool last = atomicAdd(&tickets[c0], 1u) == (uint32_t)(c1 - c0);

@@ -60,6 +60,61 @@ struct KvSpan {
     __device__ __forceinline__ int position(int v) const { return v < ns ? v : lo + v - ns; }
 };
 
+// which keys of a span a row sees, as up to two ranges and, for drafts, a set
+struct KvSight {
+    int a, lo, hi;  // keys 0 … a - 1 and lo … hi - 1 of the span
+    int draft;      // the key of the first draft
+    uint64_t set;   // the drafts that the row sees
+    // a row at position `at`, which sees positions up to `last`
+    __device__ __forceinline__ void rows(const KvView& c, const KvSpan& s, int at, int last) {
+        const int shift = s.ns - s.lo;  // key = position + shift, from the window on
+        hi = min(s.nv, last + 1 + shift);
+        lo = c.window ? max(0, at - c.window + 1 + shift) : 0;
+        a = min(hi, max(s.ns, c.sinks + shift));
+        draft = s.pos + shift;
+        set = 0;
+    }
+    // of keys v … v + 31, those that the row sees
+    __device__ __forceinline__ uint32_t mask(int v) const {
+        auto below = [](int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; };
+        uint32_t m = below(a - v) | (below(hi - v) & ~below(lo - v));
+        const int sh = v - draft;
+        if (set && sh > -32 && sh < 64) m |= sh >= 0 ? (uint32_t)(set >> sh) : (uint32_t)(set << -sh);
+        return m;
+    }
+};
+// a draft's place: its depth (position pos + depth) and what it sees; parent and depth of the slot's drafts may be read
+__device__ __forceinline__ void kv_draft(const KvView& c, const KvSpan& s, int row, const int* parent, const int* depth,
+                                         KvSight& sight) {
+    const int at = s.pos + depth[row];
+    sight.rows(c, s, at, s.pos - 1);
+    for (int i = row; i >= 0;) {
+        const int where = s.pos + depth[i];
+        if (!c.window || where > at - c.window || where < c.sinks) sight.set |= 1ull << i;
+        i = parent[i] < i ? parent[i] : -1;
+    }
+}
+__device__ __forceinline__ int kv_depth(int row, const int* parent, int* err) {
+    int d = -1;
+    for (int i = row; i >= 0; d++) {
+        const int p = parent[i];
+        if (p >= i || p < -1) dev_error(err, DEV_BAD_INDEX);  // (then taken for a child of the committed rows)
+        i = p < i ? p : -1;
+    }
+    return d;
+}
+
+// the line of tiles cut into parts of one size, or one more: CTA i takes tiles part(i) … part(i + 1) - 1
+struct KvLine {
+    int n, size, more;  // parts, tiles of each, the first `more` of them have another
+    __device__ __forceinline__ void cut(int total, int parts) { n = parts, size = total / max(parts, 1), more = total - size * parts; }
+    __device__ __forceinline__ int part(int i) const { return i * size + min(i, more); }
+    __device__ __forceinline__ int owner(int tile) const {
+        const int t = tile - more * (size + 1);
+        return t < 0 ? tile / (size + 1) : more + t / size;
+    }
+};
+
 // where a CTA stands in the line of tiles
 struct KvCursor {
     int b, h, first, tiles;  // the entry and the kv head, the first of its tiles in the line, their number
