@@ -17,10 +17,12 @@
 // end), so one's exponentials run beside the other's products. The reference moves when a tile's maximum passes it by
 // 2^6 (then O is rescaled in TMEM); weights stay below 2^14.
 //
-// Roles (544 threads): warps 0-3 and 4-7 the two softmax groups, a row per thread; warps 8-15 stage K and V: raw loads
-// one tile ahead in registers, quants to f16, V transposed (every operand K-major, 128-byte swizzle); warp 16 issues
-// the products. Every wait is bounded: a role that gives up sets a flag, the others follow, and no copy is in flight
-// (the staging is plain loads and stores).
+// Roles (512 threads, so that each has 128 registers): warps 0-3 and 4-7 the two softmax groups, a row per thread, one
+// thread of each issuing the group's products (P V of its tile, then Q K^T of its next); warps 8-15 stage K and V: raw
+// loads one tile ahead in registers, quants to f16, V transposed (every operand K-major, 128-byte swizzle). K runs a
+// tile ahead of V: the next K is staged during P V, V during Q K^T, so one stage of each keeps the tensor cores fed.
+// Every wait is bounded: a role that gives up sets a flag, the others follow, and no copy is in flight (the staging is
+// plain loads and stores).
 //
 // The work: as in k_kv_attn.cu, the tiles of all (slot, row block, kv head) triples form a line cut evenly over the
 // SMs, triples in several CTAs joined by the last to arrive; past KV_LINE (slot, row block) pairs a CTA takes one
@@ -32,7 +34,7 @@ namespace ocr {
 
 constexpr int KC_M = 128, KC_KEYS = 128;
 constexpr int KC_LOADERS = 8;
-constexpr int KC_THREADS = (8 + KC_LOADERS + 1) * 32;
+constexpr int KC_THREADS = (8 + KC_LOADERS) * 32;
 constexpr int KC_RING = 4;  // tiles whose exponents and marks are kept
 constexpr float KC_LAG = 6.0f, KC_BIAS = 8.0f;
 
@@ -62,8 +64,11 @@ struct KcPlan {
     static constexpr int PART = (D + 2) * KC_M;
 };
 
+// Barriers: a waiter must meet every completion of its barrier in turn (a parity tells only one from the next), so what
+// a softmax group waits for is kept per group (tile n is group n % 2's): kfull, vfull, sfull, odone. The staging meets
+// every tile: kempty and vempty are kept per stage.
 struct KcShared {
-    uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], odone[2], xfull[KC_RING], mdone;
+    uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], odone[2], xfull[KC_RING], mdone[2];
     uint32_t tmem;
     int abort_flag, last;
     int prefix[KV_LINE + 1], wsum[KC_THREADS / 32];
@@ -374,15 +379,14 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             mbar_init(&sh.vfull[i], KC_LOADERS);
             mbar_init(&sh.vempty[i], 1);
             mbar_init(&sh.sfull[i], 1);
-            mbar_init(&sh.pfull[i], 4);
+            mbar_init(&sh.mdone[i], 1);
             mbar_init(&sh.odone[i], 1);
         }
         for (int i = 0; i < KC_RING; i++) mbar_init(&sh.xfull[i], 1);
-        mbar_init(&sh.mdone, 1);
         sh.abort_flag = 0;
         mbar_fence_init();
     }
-    if (warp == 16) {
+    if (warp == 0) {
         tmem_alloc(&sh.tmem, 512);
         tmem_relinquish();
     }
@@ -451,7 +455,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
     }
 
     int n0 = 0;          // tiles of this CTA before the triple
-    bool any_mma = false;  // (the issuing lane)
+    bool any_mma = false;  // (the issuing threads)
     for (int seg = begin; seg < end;) {
         if (line) cc.at(seg, sh.prefix, entries, c.n_kv);
         const int slot = cc.b / blocks, blk = cc.b % blocks;
@@ -472,7 +476,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
         };
         if (a.parent && tid < sp.m) sh.parent[tid] = a.parent[(size_t)slot * a.r.T + tid];
         // ---- the queries: hi and lo, a row per warp at a time ----
-        if (warp < 16) {
+        {
             constexpr int R = KC_M / 16, V = D / 32;  // a lane's dims
             alignas(16) T q[R][V];
 #pragma unroll
@@ -523,16 +527,13 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
         }
 
         if (warp >= 8 && warp < 16) {
-            // ---- the staging ----
+            // ---- the staging: K of tile i + 1, then V of tile i ----
             const int lw = warp - 8, lt = tid - 256;
-            Raw raw;
+            Raw raw{};
             const int vb = (seg - cc.first) * KC_KEYS;
-            typename Raw::Tile next(c, sp, base, vb);
-            raw.load_k(c, sp, base, next, lw, lane);
-            raw.load_v(c, sp, base, next, lt);
             bool ok = true;  // (a thread that gave up still meets the others at every tile's barrier)
-            for (int i = 0; i < N; i++) {
-                const int n = n0 + i, st = n % NS, x = n % KC_RING, v0 = vb + i * KC_KEYS;
+            auto put_k = [&](int i) {  // → the exponent of V's tile
+                const int n = n0 + i, st = n % NS, x = n % KC_RING;
                 int eK = 0, eV = 0;
                 if (lt < 4) sh.bad[x][lt] = 0u;
                 if constexpr (P::QN) {
@@ -547,12 +548,14 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 if constexpr (P::QN) {
                     auto exponent = [&](int w) {
                         uint32_t b = sh.red[n & 1][w];
+#pragma unroll
                         for (int j = 1; j < KC_LOADERS / 2; j++) b = h2max(b, sh.red[n & 1][w + j]);
                         const __half2 h = *reinterpret_cast<const __half2*>(&b);
                         const float f = fmaxf(__low2float(h), __high2float(h));
                         return f > 0.0f ? min(16, (int)(__float_as_uint(f) >> 23) - 127) : 0;
                     };
-                    eK = exponent(0), eV = exponent(KC_LOADERS / 2);
+                    eK = exponent(0);
+                    eV = exponent(KC_LOADERS / 2);
                     if (lt == 0) {
                         sh.ex[x][0] = eK, sh.ex[x][1] = eV;
                         mbar_arrive(&sh.xfull[x]);
@@ -563,70 +566,29 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 if (ok) raw.store_k(kh, kh + P::T_BYTES, eK, lw, lane);
                 fence_proxy_async();
                 __syncwarp();
-                if (ok && lane == 0) mbar_arrive(&sh.kfull[st]);
-                if (i + 1 < N) {
-                    next = typename Raw::Tile(c, sp, base, v0 + KC_KEYS);
-                    raw.load_k(c, sp, base, next, lw, lane);
-                }
+                if (ok && lane == 0) mbar_arrive(&sh.kfull[n & 1]);
+                if (i + 1 < N)
+                    raw.load_k(c, sp, base, typename Raw::Tile(c, sp, base, vb + (i + 1) * KC_KEYS), lw, lane);
+                return eV;
+            };
+            {
+                const typename Raw::Tile first(c, sp, base, vb);
+                raw.load_k(c, sp, base, first, lw, lane);
+                raw.load_v(c, sp, base, first, lt);
+            }
+            int eV = put_k(0);
+            for (int i = 0; i < N; i++) {
+                const int n = n0 + i, st = n % NS, v0 = vb + i * KC_KEYS;
+                const int e = eV;
+                if (i + 1 < N) eV = put_k(i + 1);
                 ok = ok && (n < NS || kc_wait(&sh.vempty[st], (n / NS - 1) & 1, abort_flag, err));
                 uint8_t* vh = Vr + st * P::PARTS * P::T_BYTES;
-                if (ok) raw.store_v(vh, vh + P::T_BYTES, eV, edge_of(v0), sh.bad[x], lt);
+                if (ok) raw.store_v(vh, vh + P::T_BYTES, e, edge_of(v0), sh.bad[n % KC_RING], lt);
                 fence_proxy_async();
                 __syncwarp();
-                if (ok && lane == 0) mbar_arrive(&sh.vfull[st]);
-                if (i + 1 < N) raw.load_v(c, sp, base, next, lt);
+                if (ok && lane == 0) mbar_arrive(&sh.vfull[n & 1]);
+                if (i + 1 < N) raw.load_v(c, sp, base, typename Raw::Tile(c, sp, base, v0 + KC_KEYS), lt);
             }
-        } else if (warp == 16) {
-            // ---- the products ----
-            if (lane == 0) {
-                constexpr uint32_t idS = bg_idesc(KC_KEYS), idO = bg_idesc(D);
-                auto qk = [&](int n) -> bool {
-                    const int w = n & 1, st = n % NS;
-                    // P of this group's last tile lies over S: its product is done first
-                    if (n >= 2 && !kc_wait(&sh.odone[w], ((n >> 1) - 1) & 1, abort_flag, err)) return false;
-                    if (!kc_wait(&sh.kfull[st], (n / NS) & 1, abort_flag, err)) return false;
-                    tc_fence_after();
-                    const uint32_t qh = smem_u32(Qh), ql = smem_u32(Ql);
-                    const uint32_t kh = smem_u32(Kr + st * P::PARTS * P::T_BYTES), kl = kh + P::T_BYTES;
-                    const uint32_t tS = tmem + w * KC_KEYS;
-                    // the small products first: a sum loses what falls below its last bit at every product added
-                    constexpr int SMALL = (P::LO ? 1 : 0) + (P::QN ? 1 : 0);
-#pragma unroll
-                    for (int x = 0; x <= SMALL; x++)
-#pragma unroll
-                        for (int k = 0; k < D / 16; k++) {
-                            const uint32_t o = (k >> 2) * (128 * 128) + (k & 3) * 32;
-                            const bool lq = P::LO && x == 0, lk = P::QN && x == (P::LO ? 1 : 0);
-                            mma_f16(tS, bg_desc((lq ? ql : qh) + o), bg_desc((lk ? kl : kh) + o), idS, x + k > 0 ? 1u : 0u);
-                        }
-                    mma_commit(&sh.sfull[w]);
-                    mma_commit(&sh.kempty[st]);
-                    any_mma = true;
-                    return true;
-                };
-                bool ok = qk(n0);
-                for (int i = 0; i < N && ok; i++) {
-                    const int n = n0 + i, w = n & 1, st = n % NS;
-                    if (i + 1 < N && !(ok = qk(n + 1))) break;
-                    if (!kc_wait(&sh.pfull[w], (n >> 1) & 1, abort_flag, err) ||
-                        !kc_wait(&sh.vfull[st], (n / NS) & 1, abort_flag, err))
-                        break;
-                    tc_fence_after();
-                    const uint32_t vh = smem_u32(Vr + st * P::PARTS * P::T_BYTES), vl = vh + P::T_BYTES;
-                    const uint32_t tP = tmem + w * KC_KEYS, tO = tmem + 256 + w * 128;
-#pragma unroll
-                    for (int k = 0; k < KC_KEYS / 16; k++) {  // 32 keys' P: hi in 16 columns, lo in the next 16
-                        const uint32_t p = tP + (k >> 1) * 32 + (k & 1) * 8;
-                        const uint32_t o = (k >> 2) * (D * 128) + (k & 3) * 32;
-                        mma_f16_ts(tO, p, bg_desc(vh + o), idO, (i >= 2 || k > 0) ? 1u : 0u);
-                        if constexpr (P::LO) mma_f16_ts(tO, p + 16, bg_desc(vh + o), idO, 1u);
-                        if constexpr (P::QN) mma_f16_ts(tO, p, bg_desc(vl + o), idO, 1u);
-                    }
-                    mma_commit(&sh.odone[w]);
-                    mma_commit(&sh.vempty[st]);
-                }
-            }
-            __syncwarp();
         } else {
             // ---- the rows: thread r of group wg owns pair r0 + r (TMEM lane r) ----
             const int wg = warp >> 2, r = tid & 127;
@@ -640,17 +602,60 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 sight.rows(c, sp, sp.pos + row, sp.pos + row);
             const float fac0 = sh.fac[r];
             float m = -INFINITY, l = 0.0f;
-            for (int i = (n0 & 1) ^ wg; i < N; i += 2) {
+            // the group's products, by one thread
+            const bool issues = (tid & 127) == 0;
+            constexpr uint32_t idS = bg_idesc(KC_KEYS), idO = bg_idesc(D);
+            auto qk = [&](int n) {
+                const int st = n % NS;
+                if (!kc_wait(&sh.kfull[wg], (n >> 1) & 1, abort_flag, err)) return;
+                tc_fence_after();
+                const uint32_t qh = smem_u32(Qh), ql = smem_u32(Ql);
+                const uint32_t kh = smem_u32(Kr + st * P::PARTS * P::T_BYTES), kl = kh + P::T_BYTES;
+                // the small products first: a sum loses what falls below its last bit at every product added
+                constexpr int SMALL = (P::LO ? 1 : 0) + (P::QN ? 1 : 0);
+#pragma unroll
+                for (int x = 0; x <= SMALL; x++)
+#pragma unroll
+                    for (int k = 0; k < D / 16; k++) {
+                        const uint32_t o = (k >> 2) * (128 * 128) + (k & 3) * 32;
+                        const bool lq = P::LO && x == 0, lk = P::QN && x == (P::LO ? 1 : 0);
+                        mma_f16(tmem + wg * KC_KEYS, bg_desc((lq ? ql : qh) + o), bg_desc((lk ? kl : kh) + o), idS,
+                                x + k > 0 ? 1u : 0u);
+                    }
+                mma_commit(&sh.sfull[wg]);
+                mma_commit(&sh.kempty[st]);
+                any_mma = true;
+            };
+            auto pv = [&](int n, bool fresh) {
+                const int st = n % NS;
+                if (!kc_wait(&sh.vfull[wg], (n >> 1) & 1, abort_flag, err)) return;
+                tc_fence_after();
+                const uint32_t vh = smem_u32(Vr + st * P::PARTS * P::T_BYTES), vl = vh + P::T_BYTES;
+                const uint32_t tP = tmem + wg * KC_KEYS, tD = tmem + 256 + wg * 128;
+#pragma unroll
+                for (int k = 0; k < KC_KEYS / 16; k++) {  // 32 keys' P: hi in 16 columns, lo in the next 16
+                    const uint32_t p = tP + (k >> 1) * 32 + (k & 1) * 8;
+                    const uint32_t o = (k >> 2) * (D * 128) + (k & 3) * 32;
+                    mma_f16_ts(tD, p, bg_desc(vh + o), idO, (!fresh || k > 0) ? 1u : 0u);
+                    if constexpr (P::LO) mma_f16_ts(tD, p + 16, bg_desc(vh + o), idO, 1u);
+                    if constexpr (P::QN) mma_f16_ts(tD, p, bg_desc(vl + o), idO, 1u);
+                }
+                mma_commit(&sh.odone[wg]);
+                mma_commit(&sh.vempty[st]);
+            };
+            if (issues && ((n0 & 1) ^ wg) < N) qk(n0 + ((n0 & 1) ^ wg));
+            __syncwarp();
+            auto tile = [&](int i) -> bool {  // the weights of tile i; false: a wait gave up
                 const int n = n0 + i, x = n % KC_RING, v0 = (seg - cc.first + i) * KC_KEYS;
                 const bool edge = edge_of(v0);
                 float fac = fac0, ev = 0.0f;
                 if constexpr (P::QN) {
-                    if (!kc_wait_warp(&sh.xfull[x], (n / KC_RING) & 1, abort_flag, err)) break;
+                    if (!kc_wait_warp(&sh.xfull[x], (n / KC_RING) & 1, abort_flag, err)) return false;
                     fac *= exp2i(sh.ex[x][0]);
                     ev = (float)sh.ex[x][1];
                 }
-                if (!kc_wait_warp(&sh.sfull[wg], (n >> 1) & 1, abort_flag, err)) break;
-                if (edge && !kc_wait_warp(&sh.vfull[n % NS], (n / NS) & 1, abort_flag, err)) break;  // (the marks)
+                if (!kc_wait_warp(&sh.sfull[wg], (n >> 1) & 1, abort_flag, err)) return false;
+                if (edge && !kc_wait_warp(&sh.vfull[wg], (n >> 1) & 1, abort_flag, err)) return false;  // (the marks)
                 tc_fence_after();
                 // a chunk of 32 scores, what the row does not see taken out
                 auto chunk = [&](int ch, uint32_t* s) {
@@ -680,7 +685,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                     m = mt;
                 } else if (__any_sync(FULL, mt > m + KC_LAG)) {
                     // (warp-uniform: TMEM loads and stores are the whole warp's; a row that stays scales by 1)
-                    if (!kc_wait_warp(&sh.odone[wg], ((n >> 1) - 1) & 1, abort_flag, err)) break;
+                    if (!kc_wait_warp(&sh.odone[wg], ((n >> 1) - 1) & 1, abort_flag, err)) return false;
                     tc_fence_after();
                     const bool up = mt > m + KC_LAG;
                     const float f = up ? ex2(m - mt) : 1.0f;
@@ -719,14 +724,26 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 }
                 l = fmaf(sum[0] + sum[1], exp2i(P::QN ? -(int)ev : 0), l);
                 tmem_wait_st();
+                return true;
+            };
+            bool ok = true;  // (a warp that gave up still meets its group at every tile)
+            for (int i = (n0 & 1) ^ wg; i < N; i += 2) {
+                const int n = n0 + i;
+                ok = ok && tile(i);
                 tc_fence_before();
+                bar_sync(4 + wg, 128);
+                if (issues && ok) {
+                    tc_fence_after();
+                    pv(n, i < 2);
+                    // (P lies over S: its product is done before the next S)
+                    if (i + 2 < N && kc_wait(&sh.odone[wg], (n >> 1) & 1, abort_flag, err)) qk(n + 2);
+                }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.pfull[wg]);
             }
             sh.ml[wg][0][r] = m;
             sh.ml[wg][1][r] = l;
             // both groups' products are done: this group's last tile, and the other's
-            bool ok = __all_sync(FULL, *abort_flag == 0);
+            ok = __all_sync(FULL, ok && *abort_flag == 0);
 #pragma unroll
             for (int w = 0; w < 2; w++) {
                 const int last = n0 + N - 1 - ((n0 + N - 1 - w) & 1);  // the last tile of group w
@@ -813,7 +830,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 sh.last = last;
             }
             __syncthreads();
-            if (sh.last && tid < 512) {
+            if (sh.last) {
                 const int r = tid & 127, d0 = (tid >> 7) * (D / 4);
                 const float* parts = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.work) + KV_TICKETS);
                 auto of = [&](int i) { return parts + (size_t)(2 * i + (i == c0)) * P::PART; };
@@ -840,16 +857,13 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
         seg = seg_end;
     }
     // ---- every product complete before the TMEM is given back ----
-    if (warp == 16) {
-        if (lane == 0 && any_mma) {
-            mma_commit(&sh.mdone);
-            mbar_wait(&sh.mdone, 0, err);
-        }
-        __syncwarp();
+    if (warp < 8 && (tid & 127) == 0 && any_mma) {
+        mma_commit(&sh.mdone[warp >> 2]);
+        mbar_wait(&sh.mdone[warp >> 2], 0, err);
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 16) {
+    if (warp == 0) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
