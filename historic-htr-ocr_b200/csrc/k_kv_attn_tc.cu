@@ -6,7 +6,7 @@
 // the exponentials (f16 rows: 16 a clock and SM against 128 x 128 of a tile).
 //
 // Products: S = Q K^T (M = N = 128, both operands in shared memory), O += P V (A = P in TMEM, written over S in place;
-// B = V^T in shared memory), f16 operands, f32 sums in TMEM. Exactness: f32 queries and P are f16 hi + lo (22 bits);
+// B = V in shared memory, MN-major), f16 operands, f32 sums in TMEM. Exactness: f32 queries and P are f16 hi + lo (22 bits);
 // f16 queries are exact, and P is rounded to f16 as the output is. f16 keys and values are exact; a quantised value
 // q d (at most 19 bits) splits exactly into f16 hi + lo, so S = Q_hi K_hi + Q_lo K_hi + Q_hi K_lo, and P V alike, carry
 // the f32 product to 2^-22. A row's query is scaled by a power of two (its lo part stays in f16's range), a tile's
@@ -19,7 +19,7 @@
 //
 // Roles (512 threads, so that each has 128 registers): warps 0-3 and 4-7 the two softmax groups, a row per thread, one
 // thread of each issuing the group's products (P V of its tile, then Q K^T of its next); warps 8-15 stage K and V: raw
-// loads one tile ahead in registers, quants to f16, V transposed (every operand K-major, 128-byte swizzle). K runs a
+// loads one tile ahead in registers, quants to f16 (operands in the 128-byte swizzle). K runs a
 // tile ahead of V: the next K is staged during P V, V during Q K^T, so one stage of each keeps the tensor cores fed.
 // Every wait is bounded: a role that gives up sets a flag, the others follow, and no copy is in flight (the staging is
 // plain loads and stores).
@@ -67,6 +67,7 @@ struct KcPlan {
 // Barriers: a waiter must meet every completion of its barrier in turn (a parity tells only one from the next), so what
 // a softmax group waits for is kept per group (tile n is group n % 2's): kfull, vfull, sfull, odone. The staging meets
 // every tile: kempty and vempty are kept per stage.
+template <int NB>
 struct KcShared {
     uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], odone[2], xfull[KC_RING], mdone[2];
     uint32_t tmem;
@@ -76,7 +77,8 @@ struct KcShared {
     float ml[2][2][KC_M];        // the groups' references and sums
     int ex[KC_RING][2];          // the tiles' exponents of K and V
     uint32_t bad[KC_RING][4];    // keys of an edge tile whose values are not all finite
-    uint32_t red[2][KC_LOADERS];
+    uint32_t red[KC_RING][KC_LOADERS];
+    __align__(8) __half scale[KC_RING][2][KC_KEYS][NB];
     int parent[KV_TREE_MAX], depth[KV_TREE_MAX];
 };
 
@@ -120,39 +122,29 @@ __device__ __forceinline__ bool h2_not_finite(uint32_t w) {
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 // ---- the staging of a tile, by 256 threads: raw rows to registers, later to operands ------------------------------------
+// K and V alike: rows of 64 dims (128 bytes, swizzled) in D / 64 halves of 128 keys — K is read along the dims (K-major),
+// V along the keys (MN-major), from the same layout. A warp's load covers four whole 128-byte lines; the lanes stand so
+// that the eight of a store's phase (one or more keys, units side by side) meet all eight 16-byte pieces of a row.
 template <int TYPE, int D>
 struct KcRaw {
-    static constexpr int ROW = kv_row_bytes(TYPE, D), UPK = ROW / 16, KU = KC_KEYS * UPK / (KC_LOADERS * 32);
-    static constexpr int VW = TYPE == KV_F16 ? 4 : TYPE == KV_Q8_0 ? 2 : 1;  // words of a key in a thread's block of V
     static constexpr bool QN = TYPE != KV_F16;
-    static constexpr int NB = D / KV_BLOCK;
-    uint4 k[KU];
-    __half kd[KU];
-    uint32_t v[8][VW];
-    __half vd[8];
-    uint32_t ex[NB / 2];
+    static constexpr int NB = D / KV_BLOCK, ROW = kv_row_bytes(TYPE, D);
+    static constexpr int UPK = ROW / 16;                               // 16-byte units of a key
+    static constexpr int KU = KC_KEYS * UPK / (KC_LOADERS * 32);       // units of a thread
+    static constexpr int UG = TYPE == KV_F16 ? 8 : TYPE == KV_Q8_0 ? 4 : 2;  // units of a key among eight lanes
+    static constexpr int PC = 8 / UG;                                  // 16-byte pieces of f16 from a unit
+    static constexpr int KPW = 8 / UG * 4 / (D / 64);                  // keys of a warp's load
+    static constexpr int STEP = KC_LOADERS * KPW;                      // keys from one unit of a thread to its next
+    uint4 k[KU], v[KU];
+    uint32_t ex[QN ? NB / 2 : 1];  // the scales of one key: K's for threads 0 … 127, V's for the others
 
-    // the key and the 16-byte unit of the i-th piece of K: eight keys to a store's eight lanes
-    __device__ static __forceinline__ void unit(int i, int lw, int lane, int& key, int& u) {
-        const int w = i * KC_LOADERS + lw;
-        if (UPK >= 4) {
-            key = 8 * (w / (UPK >= 4 ? UPK / 4 : 1)) + (lane & 7);
-            u = w % (UPK >= 4 ? UPK / 4 : 1) * 4 + (lane >> 3);
-        } else {
-            key = 16 * w + (lane & 15);
-            u = lane >> 4;
-        }
+    __device__ static __forceinline__ void place(int lw, int lane, int& key, int& u) {  // of the thread's first unit
+        const int q = lane >> 3, l = lane & 7;
+        key = lw * KPW + 8 / UG * (q / (D / 64)) + l / UG;
+        u = UG * (q % (D / 64)) + l % UG;
     }
-    // the thread's 8 x 8 block of V: keys 64 half + 8 ka …, group b of eight dims
-    __device__ static __forceinline__ bool block(int lt, int& ka, int& b, int& half) {
-        ka = lt & 7;
-        b = (lt >> 3) % (D / 8);
-        half = (lt >> 3) / (D / 8);
-        return half < 2;
-    }
-
-    // Loads of the tile at key v0. Where its 128 rows lie one after another (all but the tiles at an end of the span, of
-    // the sinks or of a ring), the addresses are one base and constants.
+    // The tile at key v. Where its 128 rows lie one after another (all but the tiles at an end of the span, of the sinks
+    // or of a ring), the addresses are one base and constants.
     struct Tile {
         size_t row;  // of the first key
         int v0;
@@ -163,192 +155,84 @@ struct KcRaw {
             row = base + r;
         }
     };
-    __device__ __forceinline__ void load_k(const KvView& c, const KvSpan& s, size_t base, const Tile& t, int lw, int lane) {
-        const int ekey = (lw * 32 + lane) & (KC_KEYS - 1);  // threads 0 … 127: K's scales of a key, the others V's
-        const __half* es = lw < KC_LOADERS / 2 ? c.ks : c.vs;
+    __device__ __forceinline__ void load(uint4* x, const uint8_t* data, const KvView& c, const KvSpan& s, size_t base,
+                                         const Tile& t, int lw, int lane) {
+        int key, u;
+        place(lw, lane, key, u);
         if (t.run) {
-            int key, u;
-            unit(0, lw, lane, key, u);
-            constexpr int STEP = KC_KEYS / KU;  // keys from one piece of a thread to its next
-            const uint8_t* p = c.k + (t.row + key) * ROW + u * 16;
-            const __half* d = c.ks + (t.row + key) * NB + (TYPE == KV_Q8_0 ? u >> 1 : u);
+            const uint8_t* p = data + (t.row + key) * ROW + u * 16;
 #pragma unroll
-            for (int i = 0; i < KU; i++) {
-                k[i] = *reinterpret_cast<const uint4*>(p + i * STEP * ROW);
-                if constexpr (QN) kd[i] = d[i * STEP * NB];
-            }
-            if constexpr (QN) {
-                const uint32_t* e = reinterpret_cast<const uint32_t*>(es + (t.row + ekey) * NB);
-#pragma unroll
-                for (int j = 0; j < NB / 2; j++) ex[j] = e[j];
-            }
+            for (int i = 0; i < KU; i++) x[i] = *reinterpret_cast<const uint4*>(p + i * STEP * ROW);
             return;
         }
 #pragma unroll
         for (int i = 0; i < KU; i++) {
-            int key, u;
-            unit(i, lw, lane, key, u);
-            k[i] = make_uint4(0u, 0u, 0u, 0u);
-            kd[i] = __ushort_as_half(0);
-            if (t.v0 + key < s.nv) {
-                const size_t row = base + kv_row(c, s.position(t.v0 + key));
-                k[i] = *reinterpret_cast<const uint4*>(c.k + row * ROW + u * 16);
-                if constexpr (QN) kd[i] = c.ks[row * NB + (TYPE == KV_Q8_0 ? u >> 1 : u)];
-            }
+            const int w = t.v0 + key + i * STEP;
+            x[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (w < s.nv) x[i] = *reinterpret_cast<const uint4*>(data + (base + kv_row(c, s.position(w))) * ROW + u * 16);
         }
+    }
+    __device__ __forceinline__ void load_scales(const KvView& c, const KvSpan& s, size_t base, const Tile& t, int lt) {
         if constexpr (QN) {
+            const int w = t.v0 + (lt & (KC_KEYS - 1));
 #pragma unroll
             for (int j = 0; j < NB / 2; j++) ex[j] = 0u;
-            if (t.v0 + ekey < s.nv) {
-                const size_t row = base + kv_row(c, s.position(t.v0 + ekey));
+            if (w < s.nv) {
+                const size_t row = t.run ? t.row + (lt & (KC_KEYS - 1)) : base + kv_row(c, s.position(w));
+                const uint32_t* p = reinterpret_cast<const uint32_t*>((lt < KC_KEYS ? c.ks : c.vs) + row * NB);
 #pragma unroll
-                for (int j = 0; j < NB / 2; j++) ex[j] = reinterpret_cast<const uint32_t*>(es + row * NB)[j];
+                for (int j = 0; j < NB / 2; j++) ex[j] = p[j];
             }
         }
     }
-    __device__ __forceinline__ void load_v(const KvView& c, const KvSpan& s, size_t base, const Tile& t, int lt) {
-        int ka, b, half;
-        if (!block(lt, ka, b, half)) return;
-        const int key0 = 64 * half + 8 * ka;
-        auto one = [&](int i, const uint8_t* p, const __half* d) {
-            if constexpr (VW == 4) {
-                const uint4 x = *reinterpret_cast<const uint4*>(p);
-                v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
-            } else if constexpr (VW == 2) {
-                const uint2 x = *reinterpret_cast<const uint2*>(p);
-                v[i][0] = x.x, v[i][1] = x.y;
-            } else {
-                v[i][0] = *reinterpret_cast<const uint32_t*>(p);
-            }
-            if constexpr (QN) vd[i] = *d;
-        };
-        if (t.run) {
-            const uint8_t* p = c.v + (t.row + key0) * ROW + b * (VW * 4);
-            const __half* d = c.vs + (t.row + key0) * NB + b / 4;
-#pragma unroll
-            for (int i = 0; i < 8; i++) one(i, p + i * ROW, d + i * NB);
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-#pragma unroll
-            for (int j = 0; j < VW; j++) v[i][j] = 0u;
-            vd[i] = __ushort_as_half(0);
-            if (t.v0 + key0 + i < s.nv) {
-                const size_t row = base + kv_row(c, s.position(t.v0 + key0 + i));
-                one(i, c.v + row * ROW + b * (VW * 4), c.vs + row * NB + b / 4);
-            }
-        }
-    }
-    // K as the product's operand: rows of 64 dims (128 bytes) in D / 64 halves of 128 keys
-    __device__ __forceinline__ void store_k(uint8_t* hi, uint8_t* lo, int e, int lw, int lane) const {
+    // The operands, values times 2^-e. `bad` (an edge tile's V): what is not finite becomes zero and its key is marked.
+    __device__ static __forceinline__ void store(const uint4* x, uint8_t* hi, uint8_t* lo, const __half* scale, int e,
+                                                 uint32_t* bad, int lw, int lane) {
         const float down = exp2i(-e);
+        int key0, u;
+        place(lw, lane, key0, u);
 #pragma unroll
         for (int i = 0; i < KU; i++) {
-            int key, u;
-            unit(i, lw, lane, key, u);
-            const uint32_t w[4] = {k[i].x, k[i].y, k[i].z, k[i].w};
-            if constexpr (TYPE == KV_F16) {
-                *reinterpret_cast<uint4*>(hi + (u >> 3) * (KC_KEYS * 128) + kc_sw(key, u & 7)) = k[i];
+            const int key = key0 + i * STEP;
+            if constexpr (!QN) {
+                uint4 y = x[i];
+                if (bad && (h2_not_finite(y.x) || h2_not_finite(y.y) || h2_not_finite(y.z) || h2_not_finite(y.w))) {
+                    atomicOr(&bad[key >> 5], 1u << (key & 31));
+                    y = make_uint4(0u, 0u, 0u, 0u);
+                }
+                *reinterpret_cast<uint4*>(hi + (u >> 3) * (KC_KEYS * 128) + kc_sw(key, u & 7)) = y;
             } else {
-                const __half2 dh = __float2half2_rn(__half2float(kd[i]) * down);
-                const uint32_t d = *reinterpret_cast<const uint32_t*>(&dh);
-                uint32_t q[TYPE == KV_Q8_0 ? 8 : 16];  // pairs of dims in order
+                const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                float f = __half2float(scale[key * NB + (TYPE == KV_Q8_0 ? u >> 1 : u)]);
+                if (bad && !(fabsf(f) <= 65504.0f)) {
+                    atomicOr(&bad[key >> 5], 1u << (key & 31));
+                    f = 0.0f;
+                }
+                const uint32_t d = pack2(f * down, f * down);
+                uint32_t q[4 * PC];  // pairs of dims in order
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     if constexpr (TYPE == KV_Q8_0) {
                         q[2 * j] = bytes_h2(w[j] ^ 0x80808080u, 0x4140, H2_1152);
                         q[2 * j + 1] = bytes_h2(w[j] ^ 0x80808080u, 0x4342, H2_1152);
                     } else {
-                        const uint32_t x = __byte_perm(w[j], 0u, 0x4140), y = __byte_perm(w[j], 0u, 0x4342);
-                        q[2 * j] = nibbles_h2<false>(x), q[2 * j + 1] = nibbles_h2<false>(y);
-                        q[8 + 2 * j] = nibbles_h2<true>(x), q[8 + 2 * j + 1] = nibbles_h2<true>(y);
+                        const uint32_t a = __byte_perm(w[j], 0u, 0x4140), b = __byte_perm(w[j], 0u, 0x4342);
+                        q[2 * j] = nibbles_h2<false>(a), q[2 * j + 1] = nibbles_h2<false>(b);
+                        q[8 + 2 * j] = nibbles_h2<true>(a), q[8 + 2 * j + 1] = nibbles_h2<true>(b);
                     }
                 }
-                constexpr int PC = TYPE == KV_Q8_0 ? 2 : 4;  // 16-byte pieces of the unit
 #pragma unroll
                 for (int j = 0; j < PC; j++) {
                     const int pc = PC * u + j;
                     const uint32_t at = (pc >> 3) * (KC_KEYS * 128) + kc_sw(key, pc & 7);
                     uint32_t h[4], l[4];
 #pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        h[x] = h2mul(q[4 * j + x], d);
-                        l[x] = h2rest(q[4 * j + x], d, h[x]);
+                    for (int y = 0; y < 4; y++) {
+                        h[y] = h2mul(q[4 * j + y], d);
+                        l[y] = h2rest(q[4 * j + y], d, h[y]);
                     }
                     *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
                     *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
-                }
-            }
-        }
-    }
-    // V transposed: rows of 64 keys (128 bytes) in two halves of D dims. In an edge tile, what is not finite becomes
-    // zero and its key is marked.
-    __device__ __forceinline__ void store_v(uint8_t* hi, uint8_t* lo, int e, bool edge, uint32_t* bad, int lt) {
-        int ka, b, half;
-        if (!block(lt, ka, b, half)) return;
-        if (edge) {
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                bool x = false;
-                if constexpr (QN)
-                    x = h2_not_finite((uint32_t)__half_as_ushort(vd[i]));
-                else
-#pragma unroll
-                    for (int j = 0; j < VW; j++) x |= h2_not_finite(v[i][j]);
-                if (x) {
-                    atomicOr(&bad[2 * half + (ka >> 2)], 1u << (8 * (ka & 3) + i));
-                    vd[i] = __ushort_as_half(0);
-                    if constexpr (!QN)
-#pragma unroll
-                        for (int j = 0; j < VW; j++) v[i][j] = 0u;
-                }
-            }
-        }
-        uint8_t *h0 = hi + half * (D * 128), *l0 = lo + half * (D * 128);
-        if constexpr (TYPE == KV_F16) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-                const int w = j >> 1;
-                *reinterpret_cast<uint4*>(h0 + kc_sw(8 * b + j, ka)) =
-                    make_uint4(__byte_perm(v[0][w], v[1][w], sel), __byte_perm(v[2][w], v[3][w], sel),
-                               __byte_perm(v[4][w], v[5][w], sel), __byte_perm(v[6][w], v[7][w], sel));
-            }
-        } else {
-            const float down = exp2i(-e);
-            uint32_t d[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) d[i] = pack2(__half2float(vd[2 * i]) * down, __half2float(vd[2 * i + 1]) * down);
-#pragma unroll
-            for (int x = 0; x < 4; x++) {  // two dims at a time
-                uint32_t q[2][4];
-                int dim[2];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    if constexpr (TYPE == KV_Q8_0) {  // dims 8 b + 2 x, + 1: bytes 2 (x % 2) … of word x / 2
-                        const uint32_t m = __byte_perm(v[2 * i][x >> 1], v[2 * i + 1][x >> 1], x & 1 ? 0x7362 : 0x5140) ^
-                                           0x80808080u;
-                        q[0][i] = bytes_h2(m, 0x4140, H2_1152), q[1][i] = bytes_h2(m, 0x4342, H2_1152);
-                    } else {  // byte x of the word: dim 4 w + x (low) and 16 + 4 w + x (high) of the block
-                        const uint32_t m = __byte_perm(v[2 * i][0], v[2 * i + 1][0], x & 2 ? 0x7632 : 0x5410) >> (8 * (x & 1));
-                        q[0][i] = nibbles_h2<false>(m), q[1][i] = nibbles_h2<true>(m);
-                    }
-                }
-                if constexpr (TYPE == KV_Q8_0)
-                    dim[0] = 8 * b + 2 * x, dim[1] = dim[0] + 1;
-                else
-                    dim[0] = 32 * (b >> 2) + 4 * (b & 3) + x, dim[1] = dim[0] + 16;
-#pragma unroll
-                for (int y = 0; y < 2; y++) {
-                    uint32_t h[4], l[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        h[i] = h2mul(q[y][i], d[i]);
-                        l[i] = h2rest(q[y][i], d[i], h[i]);
-                    }
-                    *reinterpret_cast<uint4*>(h0 + kc_sw(dim[y], ka)) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4*>(l0 + kc_sw(dim[y], ka)) = make_uint4(l[0], l[1], l[2], l[3]);
                 }
             }
         }
@@ -361,7 +245,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
     using Raw = KcRaw<TYPE, D>;
     constexpr int NS = P::NS;
     extern __shared__ uint8_t sm_raw[];
-    __shared__ __align__(8) KcShared sh;
+    __shared__ __align__(8) KcShared<P::QN ? P::NB : 1> sh;
     volatile int* abort_flag = &sh.abort_flag;
     const KvView& c = a.c;
     int* err = a.err;
@@ -537,19 +421,22 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 int eK = 0, eV = 0;
                 if (lt < 4) sh.bad[x][lt] = 0u;
                 if constexpr (P::QN) {
-                    uint32_t big = raw.ex[0] & 0x7fff7fffu;
+                    uint32_t big = 0u;
 #pragma unroll
-                    for (int j = 1; j < P::NB / 2; j++) big = h2max(big, raw.ex[j] & 0x7fff7fffu);
+                    for (int j = 0; j < P::NB / 2; j++) {
+                        big = h2max(big, raw.ex[j] & 0x7fff7fffu);
+                        reinterpret_cast<uint32_t*>(sh.scale[x][lt >> 7][lt & 127])[j] = raw.ex[j];
+                    }
 #pragma unroll
                     for (int o = 16; o > 0; o >>= 1) big = h2max(big, __shfl_xor_sync(FULL, big, o));
-                    if (lane == 0) sh.red[n & 1][lw] = big;
+                    if (lane == 0) sh.red[x][lw] = big;
                 }
                 bar_sync(2, KC_LOADERS * 32);
                 if constexpr (P::QN) {
                     auto exponent = [&](int w) {
-                        uint32_t b = sh.red[n & 1][w];
+                        uint32_t b = sh.red[x][w];
 #pragma unroll
-                        for (int j = 1; j < KC_LOADERS / 2; j++) b = h2max(b, sh.red[n & 1][w + j]);
+                        for (int j = 1; j < KC_LOADERS / 2; j++) b = h2max(b, sh.red[x][w + j]);
                         const __half2 h = *reinterpret_cast<const __half2*>(&b);
                         const float f = fmaxf(__low2float(h), __high2float(h));
                         return f > 0.0f ? min(16, (int)(__float_as_uint(f) >> 23) - 127) : 0;
@@ -563,31 +450,36 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 }
                 ok = ok && (n < NS || kc_wait(&sh.kempty[st], (n / NS - 1) & 1, abort_flag, err));
                 uint8_t* kh = Kr + st * P::PARTS * P::T_BYTES;
-                if (ok) raw.store_k(kh, kh + P::T_BYTES, eK, lw, lane);
+                if (ok) Raw::store(raw.k, kh, kh + P::T_BYTES, sh.scale[x][0][0], eK, nullptr, lw, lane);
                 fence_proxy_async();
                 __syncwarp();
                 if (ok && lane == 0) mbar_arrive(&sh.kfull[n & 1]);
-                if (i + 1 < N)
-                    raw.load_k(c, sp, base, typename Raw::Tile(c, sp, base, vb + (i + 1) * KC_KEYS), lw, lane);
+                if (i + 1 < N) {
+                    const typename Raw::Tile t(c, sp, base, vb + (i + 1) * KC_KEYS);
+                    raw.load(raw.k, c.k, c, sp, base, t, lw, lane);
+                    raw.load_scales(c, sp, base, t, lt);
+                }
                 return eV;
             };
             {
                 const typename Raw::Tile first(c, sp, base, vb);
-                raw.load_k(c, sp, base, first, lw, lane);
-                raw.load_v(c, sp, base, first, lt);
+                raw.load_scales(c, sp, base, first, lt);
+                raw.load(raw.k, c.k, c, sp, base, first, lw, lane);
+                raw.load(raw.v, c.v, c, sp, base, first, lw, lane);
             }
             int eV = put_k(0);
             for (int i = 0; i < N; i++) {
-                const int n = n0 + i, st = n % NS, v0 = vb + i * KC_KEYS;
+                const int n = n0 + i, st = n % NS, x = n % KC_RING, v0 = vb + i * KC_KEYS;
                 const int e = eV;
                 if (i + 1 < N) eV = put_k(i + 1);
                 ok = ok && (n < NS || kc_wait(&sh.vempty[st], (n / NS - 1) & 1, abort_flag, err));
                 uint8_t* vh = Vr + st * P::PARTS * P::T_BYTES;
-                if (ok) raw.store_v(vh, vh + P::T_BYTES, e, edge_of(v0), sh.bad[n % KC_RING], lt);
+                if (ok)
+                    Raw::store(raw.v, vh, vh + P::T_BYTES, sh.scale[x][1][0], e, edge_of(v0) ? sh.bad[x] : nullptr, lw, lane);
                 fence_proxy_async();
                 __syncwarp();
                 if (ok && lane == 0) mbar_arrive(&sh.vfull[n & 1]);
-                if (i + 1 < N) raw.load_v(c, sp, base, typename Raw::Tile(c, sp, base, v0 + KC_KEYS), lt);
+                if (i + 1 < N) raw.load(raw.v, c.v, c, sp, base, typename Raw::Tile(c, sp, base, v0 + KC_KEYS), lw, lane);
             }
         } else {
             // ---- the rows: thread r of group wg owns pair r0 + r (TMEM lane r) ----
@@ -604,7 +496,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             float m = -INFINITY, l = 0.0f;
             // the group's products, by one thread
             const bool issues = (tid & 127) == 0;
-            constexpr uint32_t idS = bg_idesc(KC_KEYS), idO = bg_idesc(D);
+            constexpr uint32_t idS = bg_idesc(KC_KEYS), idO = bg_idesc_mn(D);
             auto qk = [&](int n) {
                 const int st = n % NS;
                 if (!kc_wait(&sh.kfull[wg], (n >> 1) & 1, abort_flag, err)) return;
@@ -635,10 +527,10 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
 #pragma unroll
                 for (int k = 0; k < KC_KEYS / 16; k++) {  // 32 keys' P: hi in 16 columns, lo in the next 16
                     const uint32_t p = tP + (k >> 1) * 32 + (k & 1) * 8;
-                    const uint32_t o = (k >> 2) * (D * 128) + (k & 3) * 32;
-                    mma_f16_ts(tD, p, bg_desc(vh + o), idO, (!fresh || k > 0) ? 1u : 0u);
-                    if constexpr (P::LO) mma_f16_ts(tD, p + 16, bg_desc(vh + o), idO, 1u);
-                    if constexpr (P::QN) mma_f16_ts(tD, p, bg_desc(vl + o), idO, 1u);
+                    const uint64_t bh = bg_desc_mn(vh + k * 2048, KC_KEYS * 128), bl = bg_desc_mn(vl + k * 2048, KC_KEYS * 128);
+                    mma_f16_ts(tD, p, bh, idO, (!fresh || k > 0) ? 1u : 0u);
+                    if constexpr (P::LO) mma_f16_ts(tD, p + 16, bh, idO, 1u);
+                    if constexpr (P::QN) mma_f16_ts(tD, p, bl, idO, 1u);
                 }
                 mma_commit(&sh.odone[wg]);
                 mma_commit(&sh.vempty[st]);

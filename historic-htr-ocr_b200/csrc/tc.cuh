@@ -20,6 +20,14 @@ __device__ __forceinline__ uint64_t bg_desc(uint32_t saddr) {
     return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
            (2ull << 61);
 }
+// The same for a B operand stored [k][n] (MN-major): 64 n to a 128-byte row, rows of consecutive k, atoms of 8 rows 1024
+// bytes apart (bit 32), the next 64 n `next` bytes on (bit 16, in 16-byte units). The instruction descriptor says so too
+// (bit 16).
+__device__ __forceinline__ uint64_t bg_desc_mn(uint32_t saddr, uint32_t next) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(next >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+__host__ __device__ constexpr uint32_t bg_idesc_mn(int n) { return bg_idesc(n) | (1u << 16); }
 __device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t cols) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst)), "r"(cols)
                  : "memory");
