@@ -24,9 +24,9 @@
 namespace ocr {
 
 constexpr int KA_ROWS = 32;          // (row, query head) pairs of a kv head up to which this kernel runs
-constexpr int KA_WARPS = 8;
+constexpr int KA_WARPS = 12;
 constexpr int KA_THREADS = KA_WARPS * 32;
-constexpr int KA_RING = 26112;       // a warp's share of the rings: three q8_0 tiles of 32 keys
+constexpr int KA_RING = 17408;       // a warp's share of the rings: two q8_0 tiles of 32 keys
 
 template <int TYPE, int D>
 struct KaTile {
@@ -70,6 +70,16 @@ __device__ __forceinline__ void ldmatrix4(uint32_t* r, uint32_t addr) {
                      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                      : "r"(addr));
 }
+// a key's NB scales
+template <int NB>
+__device__ __forceinline__ void load_scales(__half2* d, const uint8_t* scales, int key) {
+    if constexpr (NB == 4) {
+        const uint2 x = *reinterpret_cast<const uint2*>(scales + key * 8);
+        d[0] = *reinterpret_cast<const __half2*>(&x.x), d[1] = *reinterpret_cast<const __half2*>(&x.y);
+    } else {
+        d[0] = *reinterpret_cast<const __half2*>(scales + key * 4);
+    }
+}
 template <int N>
 __device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool live) {
     const int n = live ? N : 0;  // the rest is filled with zeros
@@ -83,20 +93,21 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-template <int TYPE, int D, int WR, class T>
+template <int TYPE, int D, int WR, bool PACK, class T>
 __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant__ KvAttnArgs a) {
     using KT = KaTile<TYPE, D>;
-    constexpr bool LO = sizeof(T) == 4;          // the lo halves of q and P
+    constexpr bool LO = sizeof(T) == 4 && !PACK;  // the lo halves of q and P in products of their own
     constexpr int TEAMS = KA_WARPS / WR;         // WR warps share a ring, eight rows each
     constexpr int STAGES = KT::STAGES * WR;
     constexpr int KEYS = KT::KEYS, MT = KEYS / 16, NB = KT::NB;
+    constexpr int ROWS = PACK ? 4 : 8;           // of a warp: PACK has four in columns 0 … 3, their lo halves in 4 … 7
     constexpr int KSTEPS = D / 16, DT = D / 16;  // 16-dim steps of S, 16-dim tiles of O
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int prefix[KV_LINE + 1];
     __shared__ int wsum[KA_WARPS];
     __shared__ int s_parent[KV_TREE_MAX], s_depth[KV_TREE_MAX];
     __shared__ KvSight s_sight[8 * WR];
-    __shared__ float s_ml[KA_WARPS][16];
+    __shared__ float s_ml[4][16];
     __shared__ int s_last;
     pdl_trigger();
     pdl_wait();
@@ -156,6 +167,8 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
     lc.at(begin, prefix, c.n_slot, c.n_kv);
     ls.set(a, lc.b, 0, a.r.T);
     int lt = begin + team, ln = 0;  // the next tile to copy, the copies so far
+    constexpr int PIECES = KT::ROW / 16, KEYS_PER = 32 * WR / PIECES;  // 16-byte pieces of a key; keys of one round
+    const int lkey = tl / PIECES, lpiece = tl % PIECES;
     auto load = [&]() {
         if (lt < end) {
             if (lt >= lc.first + lc.tiles) {
@@ -163,24 +176,44 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
                 ls.set(a, lc.b, 0, a.r.T);
             }
             const uint32_t dst = smem_u32(ring + ln % STAGES * KT::STAGE);
-            const int v0 = (lt - lc.first) * KEYS;
+            const int v0 = (lt - lc.first) * KEYS, v1 = v0 + KEYS - 1;
             const size_t base = kv_index(c, lc.b, lc.h, 0);
-            constexpr int PIECES = KT::ROW / 16;
+            const int r0 = kv_row(c, ls.position(v0));
+            // a tile whose rows lie one after another: one base, constant steps
+            if (v1 < ls.nv && (v0 >= ls.ns || v1 < ls.ns) && kv_row(c, ls.position(v1)) - r0 == KEYS - 1) {
+                const size_t row = base + r0;
+                const uint8_t *kp = c.k + (row + lkey) * KT::ROW + lpiece * 16, *vp = c.v + (row + lkey) * KT::ROW + lpiece * 16;
 #pragma unroll
-            for (int e = 0; e < KEYS * PIECES / 32; e += WR) {
-                const int x = e * 32 + tl, i = x / PIECES, p = x % PIECES;
-                if (KEYS * PIECES % (32 * WR) && x >= KEYS * PIECES) break;
-                const bool live = v0 + i < ls.nv;
-                const size_t row = base + (live ? kv_row(c, ls.position(v0 + i)) : 0);
-                cp_async<16>(dst + KT::off(i, p, false), c.k + row * KT::ROW + p * 16, live);
-                cp_async<16>(dst + KT::K_BYTES + KT::off(i, p, true), c.v + row * KT::ROW + p * 16, live);
-            }
-            if constexpr (NB > 0) {
-                for (int i = tl; i < KEYS; i += 32 * WR) {
+                for (int e = 0; e < KEYS / KEYS_PER; e++) {
+                    const int i = lkey + e * KEYS_PER;
+                    cp_async<16>(dst + KT::off(i, lpiece, false), kp + e * KEYS_PER * KT::ROW, true);
+                    cp_async<16>(dst + KT::K_BYTES + KT::off(i, lpiece, true), vp + e * KEYS_PER * KT::ROW, true);
+                }
+                if constexpr (NB > 0) {
+                    const __half *ks = c.ks + (row + tl) * NB, *vs = c.vs + (row + tl) * NB;
+#pragma unroll
+                    for (int i = 0; i < KEYS; i += 32 * WR) {
+                        if (i + tl >= KEYS) break;
+                        cp_async<NB * 2>(dst + 2 * KT::K_BYTES + (i + tl) * NB * 2, ks + i * NB, true);
+                        cp_async<NB * 2>(dst + 2 * KT::K_BYTES + KT::S_BYTES + (i + tl) * NB * 2, vs + i * NB, true);
+                    }
+                }
+            } else {
+#pragma unroll 1
+                for (int i = lkey; i < KEYS; i += KEYS_PER) {
                     const bool live = v0 + i < ls.nv;
                     const size_t row = base + (live ? kv_row(c, ls.position(v0 + i)) : 0);
-                    cp_async<NB * 2>(dst + 2 * KT::K_BYTES + i * NB * 2, c.ks + row * NB, live);
-                    cp_async<NB * 2>(dst + 2 * KT::K_BYTES + KT::S_BYTES + i * NB * 2, c.vs + row * NB, live);
+                    cp_async<16>(dst + KT::off(i, lpiece, false), c.k + row * KT::ROW + lpiece * 16, live);
+                    cp_async<16>(dst + KT::K_BYTES + KT::off(i, lpiece, true), c.v + row * KT::ROW + lpiece * 16, live);
+                }
+                if constexpr (NB > 0) {
+#pragma unroll 1
+                    for (int i = tl; i < KEYS; i += 32 * WR) {
+                        const bool live = v0 + i < ls.nv;
+                        const size_t row = base + (live ? kv_row(c, ls.position(v0 + i)) : 0);
+                        cp_async<NB * 2>(dst + 2 * KT::K_BYTES + i * NB * 2, c.ks + row * NB, live);
+                        cp_async<NB * 2>(dst + 2 * KT::K_BYTES + KT::S_BYTES + i * NB * 2, c.vs + row * NB, live);
+                    }
                 }
             }
             lt += TEAMS;
@@ -222,7 +255,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
         uint32_t qh[KSTEPS][2], ql[LO ? KSTEPS : 1][2];
         float sfac[2];
         {
-            const int r = 8 * wr + g;
+            const int r = ROWS * wr + (PACK ? g & 3 : g);
             const bool live = r < rows;
             const T* qp = static_cast<const T*>(a.q) + cc.b * a.q_slot + (r / G) * a.q_row + (cc.h * G + r % G) * a.q_head;
             float x[D / 4];  // the lane's dims: of step s, k = 2t, 2t + 1, 2t + 8, 2t + 9 at x[4 s …]
@@ -240,7 +273,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
                     x[4 * s + i] = live ? (float)qp[d] : 0.0f;
                 }
             float f = a.scale * LOG2E;
-            if constexpr (LO) {
+            if constexpr (sizeof(T) == 4) {
                 // the row times a power of two that brings its largest to 2^10 … 2^11 (an infinity or a NaN: 1)
                 float big = 0.0f;
 #pragma unroll
@@ -258,6 +291,10 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     qh[s][i] = pack2(x[4 * s + 2 * i], x[4 * s + 2 * i + 1]);
+                    if constexpr (PACK) {
+                        const uint32_t lo = rest2(x[4 * s + 2 * i], x[4 * s + 2 * i + 1], qh[s][i]);
+                        if (g >= 4) qh[s][i] = lo;
+                    }
                     if constexpr (LO) ql[s][i] = rest2(x[4 * s + 2 * i], x[4 * s + 2 * i + 1], qh[s][i]);
                 }
             // column 2t and 2t + 1's factor (held by the lanes of g = 2t, 2t + 1)
@@ -295,6 +332,8 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
                     const int kA = key(i, 0), kB = key(i, 1);
 #pragma unroll
                     for (int j = 0; j < 4; j++) p[i][j] = 0.0f;
+                    __half2 dk[2][NB / 2];
+                    load_scales<NB>(dk[0], kst, kA), load_scales<NB>(dk[1], kst, kB);
 #pragma unroll
                     for (int b = 0; b < NB; b++) {
                         uint32_t ka[2][4];
@@ -321,18 +360,21 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
                             mma16816(acc, ka[s], qh[2 * b + s][0], qh[2 * b + s][1]);
                             if constexpr (LO) mma16816(acc, ka[s], ql[2 * b + s][0], ql[2 * b + s][1]);
                         }
-                        const float dA = __half2float(reinterpret_cast<const __half*>(kst)[kA * NB + b]);
-                        const float dB = __half2float(reinterpret_cast<const __half*>(kst)[kB * NB + b]);
+                        const float dA = b & 1 ? __high2float(dk[0][b / 2]) : __low2float(dk[0][b / 2]);
+                        const float dB = b & 1 ? __high2float(dk[1][b / 2]) : __low2float(dk[1][b / 2]);
                         p[i][0] = fmaf(acc[0], dA, p[i][0]), p[i][1] = fmaf(acc[1], dA, p[i][1]);
                         p[i][2] = fmaf(acc[2], dB, p[i][2]), p[i][3] = fmaf(acc[3], dB, p[i][3]);
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < 4; j++) p[i][j] *= sfac[j & 1];
+                for (int j = 0; j < 4; j++) {
+                    if constexpr (PACK) p[i][j] += __shfl_xor_sync(FULL, p[i][j], 2);  // hi and lo
+                    p[i][j] *= sfac[j & 1];
+                }
             }
             // ---- the mask ----
             uint32_t bad = 0;       // (f16) keys of the tile whose values are not all finite
-            uint32_t seen = ~0u;    // this lane's scores that their rows see, bit 4 i + j
+            [[maybe_unused]] uint64_t col_seen = 0;  // those that column g's row sees
             if constexpr (EDGE) {
                 if (TYPE == KV_F16 && many) {
                     // a value that some rows see and some do not must not reach the latter as 0 * inf: such rows of V
@@ -347,23 +389,25 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
                         if (__any_sync(FULL, b)) bad |= 1u << i;
                     }
                 }
-                seen = 0;
+                auto sees = [&](int col, int v) {
+                    const int left = sp.nv - v;
+                    return many ? s_sight[ROWS * wr + (col & (ROWS - 1))].mask(v)
+                                : left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;
+                };
+                if constexpr (NB > 0)
+#pragma unroll
+                    for (int w = 0; w < (KEYS + 31) / 32; w++) col_seen |= (uint64_t)sees(g, v0 + 32 * w) << (32 * w);
                 uint32_t mask[2][(KEYS + 31) / 32];  // the tile's keys that the lane's two rows see
 #pragma unroll
                 for (int j = 0; j < 2; j++)
 #pragma unroll
-                    for (int w = 0; w < (KEYS + 31) / 32; w++) {
-                        const int v = v0 + 32 * w, left = sp.nv - v;
-                        mask[j][w] = many ? s_sight[8 * wr + 2 * t + j].mask(v)
-                                          : left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1u;
-                    }
+                    for (int w = 0; w < (KEYS + 31) / 32; w++) mask[j][w] = sees(2 * t + j, v0 + 32 * w);
 #pragma unroll
                 for (int i = 0; i < MT; i++)
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const int kk = key(i, j >> 1);
                         const bool s = (mask[j & 1][i / 2] >> (kk & 31)) & 1;
-                        if (s) seen |= 1u << (4 * i + j);
                         if (TYPE == KV_F16 && s && ((bad >> kk) & 1)) p[i][j] = NAN;
                         if (!s) p[i][j] = -INFINITY;
                     }
@@ -391,18 +435,27 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
                     p[i][j] = ex2(p[i][j] - ref[j & 1]);
                     l[j & 1] += p[i][j];
                 }
-            // ---- O = O alpha + V^T P ----
-            if constexpr (TYPE == KV_F16) {
-                uint32_t ph[MT][2];
-                [[maybe_unused]] uint32_t pl[LO ? MT : 1][2];
+            // ---- O = O alpha + V^T P: P as the B operand has column g, keys 2t, 2t + 1, 2t + 8, 2t + 9 of 16 ----
+            uint32_t ph[MT][2];
+            [[maybe_unused]] uint32_t pl[MT][2];
 #pragma unroll
-                for (int i = 0; i < MT; i++)
+            for (int i = 0; i < MT; i++)
 #pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const uint32_t h = pack2(p[i][2 * j], p[i][2 * j + 1]);
+                for (int j = 0; j < 2; j++) {
+                    const uint32_t h = pack2(p[i][2 * j], p[i][2 * j + 1]);
+                    if constexpr (sizeof(T) == 4) {
+                        const uint32_t r = rest2(p[i][2 * j], p[i][2 * j + 1], h);
+                        if (PACK && TYPE == KV_F16) {
+                            ph[i][j] = transpose8(t < 2 ? h : r);
+                        } else {
+                            ph[i][j] = transpose8(h);
+                            pl[i][j] = transpose8(r);
+                        }
+                    } else {
                         ph[i][j] = transpose8(h);
-                        if constexpr (LO) pl[i][j] = transpose8(rest2(p[i][2 * j], p[i][2 * j + 1], h));
                     }
+                }
+            if constexpr (TYPE == KV_F16) {
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
                     float acc[4] = {};
@@ -424,86 +477,108 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
                     for (int j = 0; j < 4; j++) o[d][j] = fmaf(o[d][j], alpha[j & 1], acc[j]);
                 }
             } else {
-                // the scales of this lane's two keys of each 16, and the tile's largest of each block
-                __half2 dv[MT][2][NB / 2], top[NB / 2];
+                // the weights again in 32 bits, the scales of the lane's four keys of each 16 (4t … 4t + 3), and the
+                // tile's largest of each block
+                float w[MT][4];
+                __half2 dv[MT][4][NB / 2], top[NB / 2];
 #pragma unroll
-                for (int i = 0; i < MT; i++)
+                for (int i = 0; i < MT; i++) {
 #pragma unroll
-                    for (int u = 0; u < 2; u++)
+                    for (int u = 0; u < 2; u++) {
+                        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&ph[i][u]));
+                        w[i][2 * u] = h.x, w[i][2 * u + 1] = h.y;
+                        if constexpr (sizeof(T) == 4) {
+                            const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&pl[i][u]));
+                            w[i][2 * u] += r.x, w[i][2 * u + 1] += r.y;
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        load_scales<NB>(dv[i][u], vst, 16 * i + 4 * t + u);
+                        // (0 times a scale that is no number is not 0)
+                        if (EDGE && !((col_seen >> (16 * i + 4 * t + u)) & 1))
+#pragma unroll
+                            for (int b = 0; b < NB / 2; b++) dv[i][u][b] = __float2half2_rn(0.0f);
 #pragma unroll
                         for (int b = 0; b < NB / 2; b++) {
-                            dv[i][u][b] = reinterpret_cast<const __half2*>(vst)[key(i, u) * (NB / 2) + b];
                             const __half2 x = __habs2(dv[i][u][b]);
                             top[b] = i + u == 0 ? x : __hmax2(top[b], x);
                         }
+                    }
+                }
+#pragma unroll
+                for (int b = 0; b < NB / 2; b++)
+#pragma unroll
+                    for (int s = 1; s <= 2; s <<= 1) {
+                        const uint32_t y = __shfl_xor_sync(FULL, *reinterpret_cast<uint32_t*>(&top[b]), s);
+                        top[b] = __hmax2(top[b], *reinterpret_cast<const __half2*>(&y));
+                    }
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
-                    if ((b & 1) == 0) {
-#pragma unroll
-                        for (int s = 4; s <= 16; s <<= 1) {
-                            const uint32_t y = __shfl_xor_sync(FULL, *reinterpret_cast<uint32_t*>(&top[b / 2]), s);
-                            top[b / 2] = __hmax2(top[b / 2], *reinterpret_cast<const __half2*>(&y));
-                        }
-                    }
                     const float big = b & 1 ? __high2float(top[b / 2]) : __low2float(top[b / 2]);
                     // 2^e <= big < 2^(e + 1); zero, or no finite scale: e = 0 or 16
                     const int e = big > 0.0f ? min(16, (int)(__float_as_uint(big) >> 23) - 127) : 0;
                     const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-                    const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+                    float up[2];  // of columns 2t, 2t + 1 (columns may see different keys)
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+                        up[j] = EDGE ? __uint_as_float((uint32_t)(127 + __shfl_sync(FULL, e, 8 * t + 4 * j)) << 23)
+                                     : __uint_as_float((uint32_t)(127 + e) << 23);
                     float acc[2][4] = {};
 #pragma unroll
                     for (int i = 0; i < MT; i++) {
-                        uint32_t ph[2];
-                        [[maybe_unused]] uint32_t pl[2];
+                        uint32_t bh[2];
+                        [[maybe_unused]] uint32_t bl[2];
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
-                            const float dd = (b & 1 ? __high2float(dv[i][u][b / 2]) : __low2float(dv[i][u][b / 2])) * down;
-                            float x = p[i][2 * u] * dd, y = p[i][2 * u + 1] * dd;
-                            if (EDGE) {  // (0 times a scale that is no number)
-                                if (!((seen >> (4 * i + 2 * u)) & 1)) x = 0.0f;
-                                if (!((seen >> (4 * i + 2 * u + 1)) & 1)) y = 0.0f;
+                            const __half2 *d0 = dv[i][2 * u], *d1 = dv[i][2 * u + 1];
+                            const float x = w[i][2 * u] * ((b & 1 ? __high2float(d0[b / 2]) : __low2float(d0[b / 2])) * down);
+                            const float y = w[i][2 * u + 1] * ((b & 1 ? __high2float(d1[b / 2]) : __low2float(d1[b / 2])) * down);
+                            bh[u] = pack2(x, y);
+                            if constexpr (LO) bl[u] = rest2(x, y, bh[u]);
+                            if constexpr (PACK) {
+                                const uint32_t r = rest2(x, y, bh[u]);
+                                if (g >= 4) bh[u] = r;
                             }
-                            const uint32_t h = pack2(x, y);
-                            ph[u] = transpose8(h);
-                            if constexpr (LO) pl[u] = transpose8(rest2(x, y, h));
                         }
                         uint32_t va[2][4];
                         if constexpr (TYPE == KV_Q8_0) {
-                            uint32_t w[4];
+                            uint32_t x4[4];
 #pragma unroll
                             for (int j = 0; j < 4; j++)
-                                w[j] = *reinterpret_cast<const uint32_t*>(
-                                           vt + KT::off(16 * i + 4 * t + j, 2 * b + (g >> 2), true) + (g & 3) * 4) ^
-                                       0x80808080u;
+                                x4[j] = *reinterpret_cast<const uint32_t*>(
+                                            vt + KT::off(16 * i + 4 * t + j, 2 * b + (g >> 2), true) + (g & 3) * 4) ^
+                                        0x80808080u;
 #pragma unroll
                             for (int u = 0; u < 2; u++) {  // keys 4t + 2u, 4t + 2u + 1; dims 4g … 4g + 3 of the block
-                                const uint32_t x = __byte_perm(w[2 * u], w[2 * u + 1], 0x5140);
-                                const uint32_t y = __byte_perm(w[2 * u], w[2 * u + 1], 0x7362);
+                                const uint32_t x = __byte_perm(x4[2 * u], x4[2 * u + 1], 0x5140);
+                                const uint32_t y = __byte_perm(x4[2 * u], x4[2 * u + 1], 0x7362);
                                 va[0][2 * u] = bytes_h2(x, 0x4140, H2_1152), va[0][2 * u + 1] = bytes_h2(x, 0x4342, H2_1152);
                                 va[1][2 * u] = bytes_h2(y, 0x4140, H2_1152), va[1][2 * u + 1] = bytes_h2(y, 0x4342, H2_1152);
                             }
                         } else {
-                            uint32_t w[4];
+                            uint32_t x4[4];
 #pragma unroll
                             for (int j = 0; j < 4; j++)
-                                w[j] = *reinterpret_cast<const uint16_t*>(vt + KT::off(16 * i + 4 * t + j, b, true) + g * 2);
+                                x4[j] = *reinterpret_cast<const uint16_t*>(vt + KT::off(16 * i + 4 * t + j, b, true) + g * 2);
 #pragma unroll
                             for (int u = 0; u < 2; u++) {  // dims 2g, 2g + 1 (low nibbles) and 16 + 2g, 17 + 2g (high)
-                                const uint32_t x = __byte_perm(w[2 * u], w[2 * u + 1], 0x5410);
+                                const uint32_t x = __byte_perm(x4[2 * u], x4[2 * u + 1], 0x5410);
                                 va[0][2 * u] = nibbles_h2<false>(x), va[0][2 * u + 1] = nibbles_h2<false>(x >> 8);
                                 va[1][2 * u] = nibbles_h2<true>(x), va[1][2 * u + 1] = nibbles_h2<true>(x >> 8);
                             }
                         }
 #pragma unroll
                         for (int s = 0; s < 2; s++) {
-                            mma16816(acc[s], va[s], ph[0], ph[1]);
-                            if constexpr (LO) mma16816(acc[s], va[s], pl[0], pl[1]);
+                            mma16816(acc[s], va[s], bh[0], bh[1]);
+                            if constexpr (LO) mma16816(acc[s], va[s], bl[0], bl[1]);
                         }
                     }
 #pragma unroll
                     for (int s = 0; s < 2; s++)
 #pragma unroll
-                        for (int j = 0; j < 4; j++) o[2 * b + s][j] = fmaf(o[2 * b + s][j], alpha[j & 1], acc[s][j] * up);
+                        for (int j = 0; j < 4; j++)
+                            o[2 * b + s][j] = fmaf(o[2 * b + s][j], alpha[j & 1], acc[s][j] * up[j & 1]);
                 }
             }
         };
@@ -530,12 +605,18 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
                 compute(ct, st, std::false_type{});
         }
 
-        // ---- the teams' parts joined: halves of them at a time, the upper into the lower ----
+        // ---- the teams' parts joined: the last teams' into the first's, at most four warps' at a time ----
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             l[j] += __shfl_xor_sync(FULL, l[j], 4);
             l[j] += __shfl_xor_sync(FULL, l[j], 8);
             l[j] += __shfl_xor_sync(FULL, l[j], 16);
+        }
+        if constexpr (PACK) {  // the lo halves' columns to the hi halves'
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[d][j] += __shfl_xor_sync(FULL, o[d][j], 2);
         }
         auto fold = [&](float* mo, float* lo, float f0[2], float f1[2]) {  // weights of the own and the other part
 #pragma unroll
@@ -546,10 +627,10 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
                 m[j] = mn;
             }
         };
-#pragma unroll
-        for (int half = TEAMS / 2; half >= 1; half /= 2) {
-            if (team >= half && team < 2 * half) {
-                const int w = warp - half * WR;
+        for (int n = TEAMS; n > 1;) {
+            const int give = min(n / 2, 4 / WR);  // teams n - give … n - 1 into teams 0 … give - 1
+            if (team >= n - give && team < n) {
+                const int w = warp - (n - give) * WR;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -560,7 +641,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
                 }
             }
             __syncthreads();
-            if (team < half) {
+            if (team < give) {
                 float mo[2] = {s_ml[warp][2 * t], s_ml[warp][2 * t + 1]};
                 float lo[2] = {s_ml[warp][8 + 2 * t], s_ml[warp][8 + 2 * t + 1]}, f0[2], f1[2];
                 fold(mo, lo, f0, f1);
@@ -571,6 +652,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
                         o[d][j] = o[d][j] * f0[j & 1] + joined[(warp * (D / 4) + 4 * d + j) * 32 + lane] * f1[j & 1];
             }
             __syncthreads();
+            n -= give;
         }
         // ---- the output, or this CTA's part of it ----
         auto dim = [&](int d, int up) {  // the dim of tile d's row g (up = 0) or g + 8
@@ -652,21 +734,23 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
     cp_wait<0>();
 }
 
-template <int TYPE, int D, int WR, class T>
+template <int TYPE, int D, int WR, bool PACK, class T>
 static cudaError_t launch_team(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
     constexpr int SMEM = KA_WARPS * KA_RING + 4 * D * 8 * 4;
     static PerDeviceOnce once;
     once([] {
-        cudaFuncSetAttribute(k_kv_attn<TYPE, D, WR, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        cudaFuncSetAttribute(k_kv_attn<TYPE, D, WR, PACK, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
     });
-    return kv_launch(k_kv_attn<TYPE, D, WR, T>, dim3(a.num_sms), KA_THREADS, SMEM, st, pdl, a);
+    return kv_launch(k_kv_attn<TYPE, D, WR, PACK, T>, dim3(a.num_sms), KA_THREADS, SMEM, st, pdl, a);
 }
 template <int TYPE, int D, class T>
 static cudaError_t launch_rows(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
     const int rows = a.r.T * (a.n_head / a.c.n_kv);
-    if (rows <= 8) return launch_team<TYPE, D, 1, T>(st, a, pdl);
-    if (rows <= 16) return launch_team<TYPE, D, 2, T>(st, a, pdl);
-    return launch_team<TYPE, D, 4, T>(st, a, pdl);
+    if constexpr (sizeof(T) == 4)
+        if (rows <= 4) return launch_team<TYPE, D, 1, true, T>(st, a, pdl);
+    if (rows <= 8) return launch_team<TYPE, D, 1, false, T>(st, a, pdl);
+    if (rows <= 16) return launch_team<TYPE, D, 2, false, T>(st, a, pdl);
+    return launch_team<TYPE, D, 4, false, T>(st, a, pdl);
 }
 template <int TYPE>
 static cudaError_t launch_type(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
