@@ -13,16 +13,17 @@
 // scales by a power of two 2^-e, e from the tile's largest: S takes 2^e back with the row's factor; for V the score
 // itself takes e as an addend, so that P carries 2^e and the row's reference bounds both.
 //
-// Softmax: online. Two warpgroups take the tiles in turn, each with sums, reference and O of its own (joined at the
-// end), so one's exponentials run beside the other's products. The reference moves when a tile's maximum passes it by
-// 2^6 (then O is rescaled in TMEM); weights stay below 2^14.
+// Softmax: online. Two warpgroups take 64 keys of every tile each, with sums, reference and O of their own (joined at the
+// end). S has two places: the next tile's Q K^T runs while the groups turn this tile's S into P, so a group goes from
+// one tile's exponentials to the next's without waiting for a product. The reference moves when a tile's maximum passes
+// it by 2^6 (then O is rescaled in TMEM); weights stay below 2^14.
 //
-// Roles (512 threads, so that each has 128 registers): warps 0-3 and 4-7 the two softmax groups, a row per thread, one
-// thread of each issuing the group's products (P V of its tile, then Q K^T of its next); warps 8-15 stage K and V: raw
-// loads one tile ahead in registers, quants to f16 (operands in the 128-byte swizzle). K runs a
-// tile ahead of V: the next K is staged during P V, V during Q K^T, so one stage of each keeps the tensor cores fed.
-// Every wait is bounded: a role that gives up sets a flag, the others follow, and no copy is in flight (the staging is
-// plain loads and stores).
+// Roles (512 threads, 128 registers each): warps 0-3 and 4-7 the two softmax groups, a row per thread; warps 8-14 stage K
+// and V: raw loads one tile ahead in registers, quants to f16 (operands in the 128-byte swizzle); one thread of warp 15
+// issues the products. K runs a tile ahead of V: the next K is staged during P V, V during Q K^T, so one stage of each
+// keeps the tensor cores fed. The staging runs on into the next triple while the softmax groups finish one. Every wait
+// is bounded: a role that gives up sets a flag and goes on without work, meeting every barrier, and no copy is in flight
+// (the staging is plain loads and stores).
 //
 // The work: as in k_kv_attn.cu, the tiles of all (slot, row block, kv head) triples form a line cut evenly over the
 // SMs, triples in several CTAs joined by the last to arrive; past KV_LINE (slot, row block) pairs a CTA takes one
@@ -33,9 +34,11 @@
 namespace ocr {
 
 constexpr int KC_M = 128, KC_KEYS = 128;
-constexpr int KC_LOADERS = 8;
-constexpr int KC_THREADS = (8 + KC_LOADERS) * 32;
-constexpr int KC_RING = 4;  // tiles whose exponents and marks are kept
+constexpr int KC_LOADERS = 7;
+constexpr int KC_THREADS = (8 + KC_LOADERS + 1) * 32;
+constexpr int KC_RING = 4;  // tiles whose exponents and scales are kept
+constexpr int KC_MARKS = 8;  // tiles whose marks are kept: looked at two tiles later
+constexpr int KC_PIECE = 3;
 constexpr float KC_LAG = 6.0f, KC_BIAS = 8.0f;
 
 template <int BYTES>
@@ -57,27 +60,30 @@ struct KcPlan {
     static constexpr bool LO = sizeof(T) == 4, QN = TYPE != KV_F16;
     static constexpr int NB = D / KV_BLOCK, ROW = kv_row_bytes(TYPE, D);
     static constexpr uint32_t Q_BYTES = KC_M * D * 2, T_BYTES = KC_KEYS * D * 2;  // one f16 operand of Q; of K or V
-    static constexpr int PARTS = QN ? 2 : 1;                                      // hi (and lo) of K and V
+    static constexpr bool VLO = QN && LO;  // f16 rows: V's rounding to f16 is P's and the output's
+    static constexpr int KPARTS = QN ? 2 : 1, VPARTS = VLO ? 2 : 1;               // hi (and lo) of K and of V
     static constexpr int NS = QN && D == 128 ? 1 : 2;                             // stages
-    static constexpr uint32_t SMEM = (LO ? 2 : 1) * Q_BYTES + 2 * NS * PARTS * T_BYTES + 1024;
+    static constexpr uint32_t SMEM = (LO ? 2 : 1) * Q_BYTES + NS * (KPARTS + VPARTS) * T_BYTES + 1024;
     // the joined parts: [D][128] sums, [128] references, [128] weights' sums
     static constexpr int PART = (D + 2) * KC_M;
 };
 
-// Barriers: a waiter must meet every completion of its barrier in turn (a parity tells only one from the next), so what
-// a softmax group waits for is kept per group (tile n is group n % 2's): kfull, vfull, sfull, odone. The staging meets
-// every tile: kempty and vempty are kept per stage.
+// Barriers: a parity tells one completion only from the next, so a waiter must know that the one before has come and that
+// the one after has not. Per stage: kfull, kempty, vempty (their waiters meet every tile in turn). Per place of S, tile
+// n's being n % 2: sfull, pfull of each group (a group may be a tile ahead of the products, not two: it needs S, which
+// needs both groups' P of two tiles before), odone, vfull.
 template <int NB>
 struct KcShared {
-    uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], odone[2], xfull[KC_RING], mdone[2];
+    uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2][2], odone[2],
+        xfull[KC_RING], qfull, mdone;
     uint32_t tmem;
     int abort_flag, last;
     int prefix[KV_LINE + 1], wsum[KC_THREADS / 32];
     float fac[KC_M];             // the rows' factors on S
     float ml[2][2][KC_M];        // the groups' references and sums
     int ex[KC_RING][2];          // the tiles' exponents of K and V
-    uint32_t bad[KC_RING][4];    // keys of an edge tile whose values are not all finite
-    uint32_t red[KC_RING][KC_LOADERS];
+    uint32_t bad[KC_MARKS][4];   // keys of an edge tile whose values are not all finite
+    __align__(8) uint32_t top[KC_RING][2];  // the largest scales of a tile's K and V (f16 bits)
     __align__(8) __half scale[KC_RING][2][KC_KEYS][NB];
     int parent[KV_TREE_MAX], depth[KV_TREE_MAX];
 };
@@ -130,13 +136,13 @@ struct KcRaw {
     static constexpr bool QN = TYPE != KV_F16;
     static constexpr int NB = D / KV_BLOCK, ROW = kv_row_bytes(TYPE, D);
     static constexpr int UPK = ROW / 16;                               // 16-byte units of a key
-    static constexpr int KU = KC_KEYS * UPK / (KC_LOADERS * 32);       // units of a thread
     static constexpr int UG = TYPE == KV_F16 ? 8 : TYPE == KV_Q8_0 ? 4 : 2;  // units of a key among eight lanes
     static constexpr int PC = 8 / UG;                                  // 16-byte pieces of f16 from a unit
     static constexpr int KPW = 8 / UG * 4 / (D / 64);                  // keys of a warp's load
     static constexpr int STEP = KC_LOADERS * KPW;                      // keys from one unit of a thread to its next
+    static constexpr int KU = (KC_KEYS + STEP - 1) / STEP;             // units of a thread, the last one of some warps
     uint4 k[KU], v[KU];
-    uint32_t ex[QN ? NB / 2 : 1];  // the scales of one key: K's for threads 0 … 127, V's for the others
+    uint32_t ex[2][QN ? NB / 2 : 1];  // threads 0 … 127: the scales of one key, K's and V's
 
     __device__ static __forceinline__ void place(int lw, int lane, int& key, int& u) {  // of the thread's first unit
         const int q = lane >> 3, l = lane & 7;
@@ -149,6 +155,7 @@ struct KcRaw {
         size_t row;  // of the first key
         int v0;
         bool run;
+        __device__ __forceinline__ Tile() {}
         __device__ __forceinline__ Tile(const KvView& c, const KvSpan& s, size_t base, int v) : v0(v) {
             const int r = kv_row(c, s.position(v)), last = v + KC_KEYS - 1;
             run = last < s.nv && (v >= s.ns || last < s.ns) && kv_row(c, s.position(last)) - r == KC_KEYS - 1;
@@ -162,30 +169,32 @@ struct KcRaw {
         if (t.run) {
             const uint8_t* p = data + (t.row + key) * ROW + u * 16;
 #pragma unroll
-            for (int i = 0; i < KU; i++) x[i] = *reinterpret_cast<const uint4*>(p + i * STEP * ROW);
+            for (int i = 0; i < KU; i++)
+                if (key + i * STEP < KC_KEYS) x[i] = *reinterpret_cast<const uint4*>(p + i * STEP * ROW);
             return;
         }
 #pragma unroll
         for (int i = 0; i < KU; i++) {
             const int w = t.v0 + key + i * STEP;
             x[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (w < s.nv) x[i] = *reinterpret_cast<const uint4*>(data + (base + kv_row(c, s.position(w))) * ROW + u * 16);
+            if (key + i * STEP < KC_KEYS && w < s.nv) x[i] = *reinterpret_cast<const uint4*>(data + (base + kv_row(c, s.position(w))) * ROW + u * 16);
         }
     }
     __device__ __forceinline__ void load_scales(const KvView& c, const KvSpan& s, size_t base, const Tile& t, int lt) {
-        if constexpr (QN) {
-            const int w = t.v0 + (lt & (KC_KEYS - 1));
+        if (QN && lt < KC_KEYS) {
+            const int w = t.v0 + lt;
+            const bool live = w < s.nv;
+            const size_t row = t.run ? t.row + lt : base + (live ? kv_row(c, s.position(w)) : 0);
 #pragma unroll
-            for (int j = 0; j < NB / 2; j++) ex[j] = 0u;
-            if (w < s.nv) {
-                const size_t row = t.run ? t.row + (lt & (KC_KEYS - 1)) : base + kv_row(c, s.position(w));
-                const uint32_t* p = reinterpret_cast<const uint32_t*>((lt < KC_KEYS ? c.ks : c.vs) + row * NB);
-#pragma unroll
-                for (int j = 0; j < NB / 2; j++) ex[j] = p[j];
+            for (int j = 0; j < NB / 2; j++) {
+                ex[0][j] = live ? reinterpret_cast<const uint32_t*>(c.ks + row * NB)[j] : 0u;
+                ex[1][j] = live ? reinterpret_cast<const uint32_t*>(c.vs + row * NB)[j] : 0u;
             }
         }
     }
     // The operands, values times 2^-e. `bad` (an edge tile's V): what is not finite becomes zero and its key is marked.
+    // Without LOW only the rounding to f16 is kept.
+    template <bool LOW>
     __device__ static __forceinline__ void store(const uint4* x, uint8_t* hi, uint8_t* lo, const __half* scale, int e,
                                                  uint32_t* bad, int lw, int lane) {
         const float down = exp2i(-e);
@@ -194,6 +203,7 @@ struct KcRaw {
 #pragma unroll
         for (int i = 0; i < KU; i++) {
             const int key = key0 + i * STEP;
+            if (key >= KC_KEYS) break;
             if constexpr (!QN) {
                 uint4 y = x[i];
                 if (bad && (h2_not_finite(y.x) || h2_not_finite(y.y) || h2_not_finite(y.z) || h2_not_finite(y.w))) {
@@ -229,10 +239,10 @@ struct KcRaw {
 #pragma unroll
                     for (int y = 0; y < 4; y++) {
                         h[y] = h2mul(q[4 * j + y], d);
-                        l[y] = h2rest(q[4 * j + y], d, h[y]);
+                        l[y] = LOW ? h2rest(q[4 * j + y], d, h[y]) : 0u;
                     }
                     *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
-                    *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+                    if constexpr (LOW) *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
                 }
             }
         }
@@ -254,7 +264,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
     uint8_t* Qh = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
     uint8_t* Ql = Qh + P::Q_BYTES;
     uint8_t* Kr = Qh + (P::LO ? 2 : 1) * P::Q_BYTES;
-    uint8_t* Vr = Kr + NS * P::PARTS * P::T_BYTES;
+    uint8_t* Vr = Kr + NS * P::KPARTS * P::T_BYTES;
     pdl_trigger();
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
@@ -263,10 +273,16 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             mbar_init(&sh.vfull[i], KC_LOADERS);
             mbar_init(&sh.vempty[i], 1);
             mbar_init(&sh.sfull[i], 1);
-            mbar_init(&sh.mdone[i], 1);
+            mbar_init(&sh.pfull[i][0], 4);
+            mbar_init(&sh.pfull[i][1], 4);
             mbar_init(&sh.odone[i], 1);
         }
-        for (int i = 0; i < KC_RING; i++) mbar_init(&sh.xfull[i], 1);
+        for (int i = 0; i < KC_RING; i++) {
+            mbar_init(&sh.xfull[i], 1);
+            sh.top[i][0] = sh.top[i][1] = 0u;
+        }
+        mbar_init(&sh.mdone, 1);
+        mbar_init(&sh.qfull, 8);
         sh.abort_flag = 0;
         mbar_fence_init();
     }
@@ -281,15 +297,16 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
     auto rows_of_block = [&](int blk, int& t0, int& t1) { t0 = blk * KC_M / G, t1 = (blk * KC_M + KC_M - 1) / G + 1; };
     bool idle_rows = false;
     for (int b = tid; b < c.n_slot; b += KC_THREADS) idle_rows |= a.r.rows(c, b, err) < a.r.T;
-    int total = 0;
+    int total = 0, longest = 0;
     if (line) {
-        int x = 0;
+        int x = 0, mine_tiles = 0;
         if (tid < entries) {  // (at most KV_LINE of them)
             int t0, t1;
             rows_of_block(tid % blocks, t0, t1);
             KvSpan s;
             s.set(a, tid / blocks, t0, t1);
-            x = (s.nv + KC_KEYS - 1) / KC_KEYS * c.n_kv;
+            mine_tiles = (s.nv + KC_KEYS - 1) / KC_KEYS;
+            x = mine_tiles * c.n_kv;
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -302,6 +319,11 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
         if (tid < entries) sh.prefix[tid + 1] = x;
         if (tid == 0) sh.prefix[0] = 0;
         for (int w = 0; w < KC_THREADS / 32; w++) total += sh.wsum[w];
+        longest = __reduce_max_sync(FULL, tid < entries ? mine_tiles : 0);
+        __syncthreads();
+        if (lane == 0) sh.wsum[warp] = longest;
+        __syncthreads();
+        for (int w = 0; w < KC_THREADS / 32; w++) longest = max(longest, sh.wsum[w]);
     }
     tc_fence_before();
     const bool some_idle = __syncthreads_or(idle_rows);
@@ -323,7 +345,23 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
     int begin = 0, end = 0;
     KvCursor cc;
     if (line) {
-        if (cta < n_cta) begin = cut.part(cta), end = cut.part(cta + 1);
+        // Even parts cut most triples in two, and each piece costs the time of about KC_PIECE tiles (the queries staged,
+        // the sums joined): where triples are short, CTAs take whole ones. (2214 rows in a window of 512, 280 triples of
+        // 6 tiles: 134 us whole, 155 us cut; 128 triples of 66 tiles: cut.)
+        const int triples = entries * c.n_kv, per = (triples + (int)gridDim.x - 1) / (int)gridDim.x;
+        const long share = total / (int)gridDim.x + 1;
+        const long whole_cost = (long)per * (longest + KC_PIECE);
+        const long cut_cost = share + KC_PIECE * (2 + share * triples / max(total, 1));
+        if (whole_cost <= cut_cost) {
+            auto start = [&](int t) {  // the first tile of triple t
+                if (t >= triples) return total;
+                const int e = t / c.n_kv, tiles = (sh.prefix[e + 1] - sh.prefix[e]) / c.n_kv;
+                return sh.prefix[e] + t % c.n_kv * tiles;
+            };
+            begin = start(cta * per), end = start((cta + 1) * per);
+        } else if (cta < n_cta) {
+            begin = cut.part(cta), end = cut.part(cta + 1);
+        }
     } else {  // one triple, the last row blocks (the longest) first
         const int per = c.n_slot * c.n_kv;
         const int blk = blocks - 1 - cta / per, b = cta % per / c.n_kv;
@@ -338,34 +376,241 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
         end = cc.tiles;
     }
 
-    int n0 = 0;          // tiles of this CTA before the triple
-    bool any_mma = false;  // (the issuing threads)
+    bool any_mma = false;  // (the issuing thread)
+    uint32_t qn = 0;
+    // a triple: its slot and row block, the keys it sees
+    struct Triple {
+        int slot, blk, t0, t1;
+        KvSpan sp;
+        size_t base;
+    };
+    auto triple = [&](const KvCursor& at) {
+        Triple x;
+        x.slot = at.b / blocks, x.blk = at.b % blocks;
+        rows_of_block(x.blk, x.t0, x.t1);
+        x.sp.set(a, x.slot, x.t0, x.t1);
+        x.base = kv_index(c, x.slot, at.h, 0);
+        return x;
+    };
+    // the tiles whose every key is seen by every row of the block: at v0 in the sinks, or from `from` to `to`
+    struct Plain {
+        int ns, from, to;
+        __device__ __forceinline__ bool edge(int v0) const { return v0 + KC_KEYS > ns && (v0 < from || v0 > to); }
+    };
+    auto plain_of = [&](const Triple& x) {
+        const KvSpan& sp = x.sp;
+        const int shift = sp.ns - sp.lo;  // key = position + shift
+        const int lowest = sp.pos + (a.parent ? -1 : x.t0), highest = sp.pos + (a.parent ? sp.m : min(x.t1, sp.m)) - 1;
+        // (with a window: past every row's window's start; sinks inside the window's part are left to the mask)
+        return Plain{sp.ns, max(sp.ns, c.window ? highest - c.window + 1 + shift : 0), min(sp.nv, lowest + 1 + shift) - KC_KEYS};
+    };
+    if (warp >= 8 && warp < 15) {
+        // ---- the staging: K of tile n + 1, then V of tile n, from the first of the CTA's tiles to the last ----
+        const int lw = warp - 8, lt = tid - 256, tiles = end - begin;
+        Raw raw{};
+        bool ok = true;  // (a thread that gave up still meets the others at every tile's barrier)
+        auto find = [&](KvCursor& at, int g) {
+            if (line) at.at(g, sh.prefix, entries, c.n_kv);
+        };
+        KvCursor kc = cc;
+        Triple kx;
+        Plain kp;
+        if (tiles > 0) {
+            find(kc, begin);
+            kx = triple(kc);
+            kp = plain_of(kx);
+        }
+        typename Raw::Tile tv;             // of the V tile to load next: K's of the tile before
+        bool next_edge = false, edge = false;
+        int plain = 0;                     // tiles that follow at 128 rows' distance, whole and seen by every row
+        auto load_k = [&](int n) {         // tile n's K and scales; its place is V's next
+            if (plain > 0) {
+                plain--;
+                tv.row += KC_KEYS, tv.v0 += KC_KEYS;
+            } else {
+                const int g = begin + n;
+                if (g >= kc.first + kc.tiles) {
+                    find(kc, g);
+                    kx = triple(kc);
+                    kp = plain_of(kx);
+                }
+                const KvSpan& sp = kx.sp;
+                tv = typename Raw::Tile(c, sp, kx.base, (g - kc.first) * KC_KEYS);
+                next_edge = kp.edge(tv.v0);
+                if (tv.run && !next_edge && tv.v0 >= sp.ns)
+                    plain = min(min((kp.to - tv.v0) / KC_KEYS, (c.n_rows - (int)(tv.row - kx.base)) / KC_KEYS - 1),
+                                min(end, kc.first + kc.tiles) - g - 1);
+            }
+            raw.load_scales(c, kx.sp, kx.base, tv, lt);
+            raw.load(raw.k, c.k, c, kx.sp, kx.base, tv, lw, lane);
+        };
+        auto load_v = [&](int n, const typename Raw::Tile& t, bool e) {
+            edge = e;
+            if (t.run) {
+                raw.load(raw.v, c.v, c, kx.sp, 0, t, lw, lane);
+            } else {  // (K may be in the next triple)
+                KvCursor at = kc;
+                if (begin + n < kc.first) find(at, begin + n);
+                const Triple x = triple(at);
+                raw.load(raw.v, c.v, c, x.sp, x.base, t, lw, lane);
+            }
+        };
+        auto put_k = [&](int n) {  // → the exponent of V's tile
+            const int st = n % NS, x = n % KC_RING;
+            int eK = 0, eV = 0;
+            if (lt < 4) sh.bad[n % KC_MARKS][lt] = 0u;
+            if (P::QN && lt < KC_KEYS) {
+#pragma unroll
+                for (int y = 0; y < 2; y++) {
+                    uint32_t big = 0u;
+#pragma unroll
+                    for (int j = 0; j < P::NB / 2; j++) {
+                        big = h2max(big, raw.ex[y][j] & 0x7fff7fffu);
+                        reinterpret_cast<uint32_t*>(sh.scale[x][y][lt])[j] = raw.ex[y][j];
+                    }
+                    big = __reduce_max_sync(FULL, max(big & 0xffffu, big >> 16));
+                    if (lane == 0) atomicMax(&sh.top[x][y], big);
+                }
+                if (lt < 2) sh.top[(x + 2) % KC_RING][lt] = 0u;  // (tile n - 2's, read by all before the last barrier)
+            }
+            bar_sync(2, KC_LOADERS * 32);
+            if constexpr (P::QN) {
+                auto exponent = [&](uint32_t bits) {
+                    const float f = __half2float(__ushort_as_half((unsigned short)bits));
+                    return f > 0.0f ? min(16, (int)(__float_as_uint(f) >> 23) - 127) : 0;
+                };
+                const uint2 top = *reinterpret_cast<const uint2*>(sh.top[x]);
+                eK = exponent(top.x), eV = exponent(top.y);
+                if (lt == 0) {
+                    sh.ex[x][0] = eK, sh.ex[x][1] = eV;
+                    mbar_arrive(&sh.xfull[x]);
+                }
+            }
+            ok = ok && (n < NS || kc_wait(&sh.kempty[st], (n / NS - 1) & 1, abort_flag, err));
+            uint8_t* kh = Kr + st * P::KPARTS * P::T_BYTES;
+            if (ok) Raw::template store<P::QN>(raw.k, kh, kh + P::T_BYTES, sh.scale[x][0][0], eK, nullptr, lw, lane);
+            fence_proxy_async();
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(&sh.kfull[st]);
+            return eV;
+        };
+        int eV = 0;
+        if (tiles > 0) {
+            load_k(0);
+            load_v(0, tv, next_edge);
+            eV = put_k(0);
+            if (tiles > 1) load_k(1);
+        }
+        for (int n = 0; n < tiles; n++) {
+            const int st = n % NS, x = n % KC_RING, e = eV;
+            const typename Raw::Tile t1 = tv;  // of tile n + 1
+            const bool e1 = next_edge;
+            if (n + 1 < tiles) {
+                eV = put_k(n + 1);
+                if (n + 2 < tiles) load_k(n + 2);
+            }
+            ok = ok && (n < NS || kc_wait(&sh.vempty[st], (n / NS - 1) & 1, abort_flag, err));
+            uint8_t* vh = Vr + st * P::VPARTS * P::T_BYTES;
+            if (ok)
+                Raw::template store<P::VLO>(raw.v, vh, vh + P::T_BYTES, sh.scale[x][1][0], e, edge ? sh.bad[n % KC_MARKS] : nullptr, lw, lane);
+            fence_proxy_async();
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(&sh.vfull[n & 1]);
+            if (n + 1 < tiles) load_v(n + 1, t1, e1);
+        }
+    } else if (warp == 15) {
+        // ---- the products: Q K^T of tile n + 1, then P V of tile n, the first group's and the second's ----
+        if (lane == 0) {
+            constexpr uint32_t idS = bg_idesc(KC_KEYS), idO = bg_idesc_mn(D);
+            constexpr int HALF = KC_KEYS / 2;
+            // the operands' descriptors; a step adds to their address field, in 16-byte units
+            const uint64_t qh = bg_desc(smem_u32(Qh)), ql = bg_desc(smem_u32(Ql));
+            const uint64_t kd = bg_desc(smem_u32(Kr)), vd = bg_desc_mn(smem_u32(Vr), KC_KEYS * 128);
+            constexpr uint64_t T16 = P::T_BYTES / 16;
+            auto qk = [&](int n, bool first) -> bool {
+                const int st = n % NS;
+                // (a triple's first: its Q is there, and every product of the one before is done)
+                if (first ? !kc_wait(&sh.qfull, qn++ & 1, abort_flag, err)
+                          // P of tile n - 2 lies over this S: its products are done
+                          : n >= 2 && !kc_wait(&sh.odone[n & 1], ((n >> 1) - 1) & 1, abort_flag, err))
+                    return false;
+                if (!kc_wait(&sh.kfull[st], (n / NS) & 1, abort_flag, err)) return false;
+                tc_fence_after();
+                const uint64_t kh = kd + st * P::KPARTS * T16, kl = kh + T16;
+                // the small products first: a sum loses what falls below its last bit at every product added
+                constexpr int SMALL = (P::LO ? 1 : 0) + (P::QN ? 1 : 0);
+#pragma unroll
+                for (int x = 0; x <= SMALL; x++)
+#pragma unroll
+                    for (int k = 0; k < D / 16; k++) {
+                        const uint64_t o = ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16;
+                        const bool lq = P::LO && x == 0, lk = P::QN && x == (P::LO ? 1 : 0);
+                        mma_f16(tmem + (n & 1) * KC_KEYS, (lq ? ql : qh) + o, (lk ? kl : kh) + o, idS, x + k > 0 ? 1u : 0u);
+                    }
+                mma_commit(&sh.sfull[n & 1]);
+                mma_commit(&sh.kempty[st]);
+                any_mma = true;
+                return true;
+            };
+            auto pv = [&](int n, bool fresh) -> bool {
+                const int st = n % NS;
+                if (!kc_wait(&sh.vfull[n & 1], (n >> 1) & 1, abort_flag, err)) return false;
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    if (!kc_wait(&sh.pfull[w][n & 1], (n >> 1) & 1, abort_flag, err)) return false;
+                    tc_fence_after();
+                    const uint64_t vh = vd + st * P::VPARTS * T16 + w * HALF * 128 / 16, vl = vh + T16;
+                    const uint32_t tP = tmem + (n & 1) * KC_KEYS + w * HALF, tD = tmem + 256 + w * 128;
+#pragma unroll
+                    for (int k = 0; k < HALF / 16; k++) {  // 32 keys' P: hi in 16 columns, lo in the next 16
+                        const uint32_t p = tP + (k >> 1) * 32 + (k & 1) * 8;
+                        const uint64_t o = k * 2048 / 16;
+                        mma_f16_ts(tD, p, vh + o, idO, (!fresh || k > 0) ? 1u : 0u);
+                        if constexpr (P::LO) mma_f16_ts(tD, p + 16, vh + o, idO, 1u);
+                        if constexpr (P::VLO) mma_f16_ts(tD, p, vl + o, idO, 1u);
+                    }
+                }
+                mma_commit(&sh.odone[n & 1]);
+                mma_commit(&sh.vempty[st]);
+                return true;
+            };
+            bool go = true;
+            int n = 0;
+            for (int seg = begin; seg < end && go;) {
+                if (line) cc.at(seg, sh.prefix, entries, c.n_kv);
+                const int seg_end = min(end, cc.first + cc.tiles), N = seg_end - seg;
+                go = qk(n, true);
+                for (int i = 0; i < N && go; i++, n++) {
+                    if (i + 1 < N) go = qk(n + 1, false);
+                    go = go && pv(n, i == 0);
+                }
+                seg = seg_end;
+            }
+            if (any_mma) {  // every product complete before the TMEM is given back
+                mma_commit(&sh.mdone);
+                mbar_wait(&sh.mdone, 0, err);
+            }
+        }
+        __syncwarp();
+    } else {
+    int n0 = 0;              // tiles of this CTA before the triple
+    bool ok = true;          // (a warp that gave up still meets its groups at every barrier)
     for (int seg = begin; seg < end;) {
         if (line) cc.at(seg, sh.prefix, entries, c.n_kv);
-        const int slot = cc.b / blocks, blk = cc.b % blocks;
-        int t0, t1;
-        rows_of_block(blk, t0, t1);
-        KvSpan sp;
-        sp.set(a, slot, t0, t1);
+        const Triple x3 = triple(cc);
+        const Plain plain = plain_of(x3);
+        const KvSpan& sp = x3.sp;
+        const int slot = x3.slot;
         const int seg_end = min(end, cc.first + cc.tiles), N = seg_end - seg;
-        const int r0 = blk * KC_M, rows = min(KC_M, sp.m * G - r0);
-        const size_t base = kv_index(c, slot, cc.h, 0);
-        // whether some row of the block does not see some key of the tile
-        auto edge_of = [&](int v0) {
-            if (v0 + KC_KEYS > sp.nv) return true;
-            if (v0 + KC_KEYS <= sp.ns) return false;
-            const int p0 = sp.position(v0), p1 = sp.position(v0 + KC_KEYS - 1);
-            const int lowest = sp.pos + (a.parent ? -1 : t0), highest = sp.pos + (a.parent ? sp.m : min(t1, sp.m)) - 1;
-            return v0 < sp.ns || p1 > lowest || (c.window && p0 <= highest - c.window && p1 >= c.sinks);
-        };
+        const int r0 = x3.blk * KC_M, rows = min(KC_M, sp.m * G - r0);
         if (a.parent && tid < sp.m) sh.parent[tid] = a.parent[(size_t)slot * a.r.T + tid];
         // ---- the queries: hi and lo, a row per warp at a time ----
         {
-            constexpr int R = KC_M / 16, V = D / 32;  // a lane's dims
+            constexpr int R = KC_M / 8, V = D / 32;  // a warp's rows; a lane's dims
             alignas(16) T q[R][V];
 #pragma unroll
             for (int i = 0; i < R; i++) {
-                const int r = warp + 16 * i, row = r0 + r;
+                const int r = warp + 8 * i, row = r0 + r;
                 const T* qp = static_cast<const T*>(a.q) + slot * a.q_slot + (row / G) * a.q_row +
                               (cc.h * G + row % G) * a.q_head + lane * V;
                 using Word = typename KcWord<V * sizeof(T)>::type;
@@ -375,7 +620,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             }
 #pragma unroll
             for (int i = 0; i < R; i++) {
-                const int r = warp + 16 * i;
+                const int r = warp + 8 * i;
                 float x[V];
                 float f = a.scale * LOG2E;
 #pragma unroll
@@ -401,91 +646,20 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 }
             }
             fence_proxy_async();
+            tc_fence_before();  // (the last triple's sums are read)
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.qfull);
         }
-        __syncthreads();
+        bar_sync(3, 256);
         if (a.parent) {
-            if (tid < sp.m) {
-                sh.depth[tid] = kv_depth(tid, sh.parent, err);
-            }
-            __syncthreads();
+            if (tid < sp.m) sh.depth[tid] = kv_depth(tid, sh.parent, err);
+            bar_sync(3, 256);
         }
-
-        if (warp >= 8 && warp < 16) {
-            // ---- the staging: K of tile i + 1, then V of tile i ----
-            const int lw = warp - 8, lt = tid - 256;
-            Raw raw{};
-            const int vb = (seg - cc.first) * KC_KEYS;
-            bool ok = true;  // (a thread that gave up still meets the others at every tile's barrier)
-            auto put_k = [&](int i) {  // → the exponent of V's tile
-                const int n = n0 + i, st = n % NS, x = n % KC_RING;
-                int eK = 0, eV = 0;
-                if (lt < 4) sh.bad[x][lt] = 0u;
-                if constexpr (P::QN) {
-                    uint32_t big = 0u;
-#pragma unroll
-                    for (int j = 0; j < P::NB / 2; j++) {
-                        big = h2max(big, raw.ex[j] & 0x7fff7fffu);
-                        reinterpret_cast<uint32_t*>(sh.scale[x][lt >> 7][lt & 127])[j] = raw.ex[j];
-                    }
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) big = h2max(big, __shfl_xor_sync(FULL, big, o));
-                    if (lane == 0) sh.red[x][lw] = big;
-                }
-                bar_sync(2, KC_LOADERS * 32);
-                if constexpr (P::QN) {
-                    auto exponent = [&](int w) {
-                        uint32_t b = sh.red[x][w];
-#pragma unroll
-                        for (int j = 1; j < KC_LOADERS / 2; j++) b = h2max(b, sh.red[x][w + j]);
-                        const __half2 h = *reinterpret_cast<const __half2*>(&b);
-                        const float f = fmaxf(__low2float(h), __high2float(h));
-                        return f > 0.0f ? min(16, (int)(__float_as_uint(f) >> 23) - 127) : 0;
-                    };
-                    eK = exponent(0);
-                    eV = exponent(KC_LOADERS / 2);
-                    if (lt == 0) {
-                        sh.ex[x][0] = eK, sh.ex[x][1] = eV;
-                        mbar_arrive(&sh.xfull[x]);
-                    }
-                }
-                ok = ok && (n < NS || kc_wait(&sh.kempty[st], (n / NS - 1) & 1, abort_flag, err));
-                uint8_t* kh = Kr + st * P::PARTS * P::T_BYTES;
-                if (ok) Raw::store(raw.k, kh, kh + P::T_BYTES, sh.scale[x][0][0], eK, nullptr, lw, lane);
-                fence_proxy_async();
-                __syncwarp();
-                if (ok && lane == 0) mbar_arrive(&sh.kfull[n & 1]);
-                if (i + 1 < N) {
-                    const typename Raw::Tile t(c, sp, base, vb + (i + 1) * KC_KEYS);
-                    raw.load(raw.k, c.k, c, sp, base, t, lw, lane);
-                    raw.load_scales(c, sp, base, t, lt);
-                }
-                return eV;
-            };
-            {
-                const typename Raw::Tile first(c, sp, base, vb);
-                raw.load_scales(c, sp, base, first, lt);
-                raw.load(raw.k, c.k, c, sp, base, first, lw, lane);
-                raw.load(raw.v, c.v, c, sp, base, first, lw, lane);
-            }
-            int eV = put_k(0);
-            for (int i = 0; i < N; i++) {
-                const int n = n0 + i, st = n % NS, x = n % KC_RING, v0 = vb + i * KC_KEYS;
-                const int e = eV;
-                if (i + 1 < N) eV = put_k(i + 1);
-                ok = ok && (n < NS || kc_wait(&sh.vempty[st], (n / NS - 1) & 1, abort_flag, err));
-                uint8_t* vh = Vr + st * P::PARTS * P::T_BYTES;
-                if (ok)
-                    Raw::store(raw.v, vh, vh + P::T_BYTES, sh.scale[x][1][0], e, edge_of(v0) ? sh.bad[x] : nullptr, lw, lane);
-                fence_proxy_async();
-                __syncwarp();
-                if (ok && lane == 0) mbar_arrive(&sh.vfull[n & 1]);
-                if (i + 1 < N) raw.load(raw.v, c.v, c, sp, base, typename Raw::Tile(c, sp, base, v0 + KC_KEYS), lw, lane);
-            }
-        } else {
-            // ---- the rows: thread r of group wg owns pair r0 + r (TMEM lane r) ----
+        {
+            // ---- the rows: thread r of group wg owns pair r0 + r (TMEM lane r), keys 64 wg … 64 wg + 63 of every tile ----
             const int wg = warp >> 2, r = tid & 127;
             const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-            const uint32_t tS = tmem + lanes + wg * KC_KEYS, tO = tmem + lanes + 256 + wg * 128;
+            const uint32_t tO = tmem + lanes + 256 + wg * 128;
             const int row = min((r0 + r) / G, sp.m - 1);
             KvSight sight;
             if (a.parent)
@@ -494,90 +668,53 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 sight.rows(c, sp, sp.pos + row, sp.pos + row);
             const float fac0 = sh.fac[r];
             float m = -INFINITY, l = 0.0f;
-            // the group's products, by one thread
-            const bool issues = (tid & 127) == 0;
-            constexpr uint32_t idS = bg_idesc(KC_KEYS), idO = bg_idesc_mn(D);
-            auto qk = [&](int n) {
-                const int st = n % NS;
-                if (!kc_wait(&sh.kfull[wg], (n >> 1) & 1, abort_flag, err)) return;
-                tc_fence_after();
-                const uint32_t qh = smem_u32(Qh), ql = smem_u32(Ql);
-                const uint32_t kh = smem_u32(Kr + st * P::PARTS * P::T_BYTES), kl = kh + P::T_BYTES;
-                // the small products first: a sum loses what falls below its last bit at every product added
-                constexpr int SMALL = (P::LO ? 1 : 0) + (P::QN ? 1 : 0);
+            constexpr int HALF = KC_KEYS / 2;
+            // an edge tile's values that are not finite were taken out of the product (a row that does not see them must not
+            // meet them as 0 times infinity); a row that sees one is spoilt as a whole
+            auto marks = [&](int i) {
+                const int v0 = (seg - cc.first + i) * KC_KEYS;
+                if (!plain.edge(v0)) return;
 #pragma unroll
-                for (int x = 0; x <= SMALL; x++)
-#pragma unroll
-                    for (int k = 0; k < D / 16; k++) {
-                        const uint32_t o = (k >> 2) * (128 * 128) + (k & 3) * 32;
-                        const bool lq = P::LO && x == 0, lk = P::QN && x == (P::LO ? 1 : 0);
-                        mma_f16(tmem + wg * KC_KEYS, bg_desc((lq ? ql : qh) + o), bg_desc((lk ? kl : kh) + o), idS,
-                                x + k > 0 ? 1u : 0u);
-                    }
-                mma_commit(&sh.sfull[wg]);
-                mma_commit(&sh.kempty[st]);
-                any_mma = true;
-            };
-            auto pv = [&](int n, bool fresh) {
-                const int st = n % NS;
-                if (!kc_wait(&sh.vfull[wg], (n >> 1) & 1, abort_flag, err)) return;
-                tc_fence_after();
-                const uint32_t vh = smem_u32(Vr + st * P::PARTS * P::T_BYTES), vl = vh + P::T_BYTES;
-                const uint32_t tP = tmem + wg * KC_KEYS, tD = tmem + 256 + wg * 128;
-#pragma unroll
-                for (int k = 0; k < KC_KEYS / 16; k++) {  // 32 keys' P: hi in 16 columns, lo in the next 16
-                    const uint32_t p = tP + (k >> 1) * 32 + (k & 1) * 8;
-                    const uint64_t bh = bg_desc_mn(vh + k * 2048, KC_KEYS * 128), bl = bg_desc_mn(vl + k * 2048, KC_KEYS * 128);
-                    mma_f16_ts(tD, p, bh, idO, (!fresh || k > 0) ? 1u : 0u);
-                    if constexpr (P::LO) mma_f16_ts(tD, p + 16, bh, idO, 1u);
-                    if constexpr (P::QN) mma_f16_ts(tD, p, bl, idO, 1u);
+                for (int ch = 0; ch < 2; ch++) {
+                    const uint32_t bad = sh.bad[(n0 + i) % KC_MARKS][2 * wg + ch];
+                    if (bad && (bad & sight.mask(v0 + HALF * wg + 32 * ch))) l = NAN;
                 }
-                mma_commit(&sh.odone[wg]);
-                mma_commit(&sh.vempty[st]);
             };
-            if (issues && ((n0 & 1) ^ wg) < N) qk(n0 + ((n0 & 1) ^ wg));
-            __syncwarp();
             auto tile = [&](int i) -> bool {  // the weights of tile i; false: a wait gave up
                 const int n = n0 + i, x = n % KC_RING, v0 = (seg - cc.first + i) * KC_KEYS;
-                const bool edge = edge_of(v0);
+                const uint32_t tS = tmem + lanes + (n & 1) * KC_KEYS + wg * HALF;
+                const bool edge = plain.edge(v0);
                 float fac = fac0, ev = 0.0f;
                 if constexpr (P::QN) {
                     if (!kc_wait_warp(&sh.xfull[x], (n / KC_RING) & 1, abort_flag, err)) return false;
                     fac *= exp2i(sh.ex[x][0]);
                     ev = (float)sh.ex[x][1];
                 }
-                if (!kc_wait_warp(&sh.sfull[wg], (n >> 1) & 1, abort_flag, err)) return false;
-                if (edge && !kc_wait_warp(&sh.vfull[wg], (n >> 1) & 1, abort_flag, err)) return false;  // (the marks)
+                if (!kc_wait_warp(&sh.sfull[n & 1], (n >> 1) & 1, abort_flag, err)) return false;
                 tc_fence_after();
-                // a chunk of 32 scores, what the row does not see taken out
-                auto chunk = [&](int ch, uint32_t* s) {
-                    tmem_ld32(tS + 32 * ch, s);
-                    tmem_wait_ld();
-                    if (!edge) return;
-                    const uint32_t see = sight.mask(v0 + 32 * ch), bad = sh.bad[x][ch] & see;
+                if (i >= 2) marks(i - 2);  // (S of this tile says that V of that one was used)
+                uint32_t s[HALF];
+                tmem_ld32(tS, s);
+                tmem_ld32(tS + 32, s + 32);
+                tmem_wait_ld();
+                if (edge) {  // what the row does not see is taken out
 #pragma unroll
-                    for (int j = 0; j < 32; j++)
-                        if (!((see >> j) & 1)) s[j] = 0xff800000u;
-                    if (bad) {
+                    for (int ch = 0; ch < 2; ch++) {
+                        const uint32_t see = sight.mask(v0 + HALF * wg + 32 * ch);
 #pragma unroll
                         for (int j = 0; j < 32; j++)
-                            if ((bad >> j) & 1) s[j] = 0x7fffffffu;
+                            if (!((see >> j) & 1)) s[32 * ch + j] = 0xff800000u;
                     }
-                };
-                float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-                for (int ch = 0; ch < 4; ch++) {
-                    uint32_t s[32];
-                    chunk(ch, s);
-#pragma unroll
-                    for (int j = 0; j < 32; j++) mq[j & 3] = fmaxf(mq[j & 3], __uint_as_float(s[j]));
                 }
+                float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < HALF; j++) mq[j & 3] = fmaxf(mq[j & 3], __uint_as_float(s[j]));
                 const float mt = fmaf(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])), fac, ev);
-                if (i < 2) {
+                if (i == 0) {
                     m = mt;
                 } else if (__any_sync(FULL, mt > m + KC_LAG)) {
                     // (warp-uniform: TMEM loads and stores are the whole warp's; a row that stays scales by 1)
-                    if (!kc_wait_warp(&sh.odone[wg], ((n >> 1) - 1) & 1, abort_flag, err)) return false;
+                    if (!kc_wait_warp(&sh.odone[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, err)) return false;
                     tc_fence_after();
                     const bool up = mt > m + KC_LAG;
                     const float f = up ? ex2(m - mt) : 1.0f;
@@ -595,109 +732,84 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 }
                 const float ref = ev + KC_BIAS - (m == -INFINITY ? 0.0f : m);
                 float sum[2] = {0.0f, 0.0f};
-#pragma unroll 1
-                for (int ch = 0; ch < 4; ch++) {
-                    uint32_t s[32], h[16];
-                    chunk(ch, s);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const float p = ex2(fmaf(__uint_as_float(s[j]), fac, ref));
-                        s[j] = __float_as_uint(p);
-                        sum[j & 1] += p;
-                    }
+                for (int ch = 0; ch < 2; ch++) {
+                    uint32_t h[16], lo[16];
 #pragma unroll
                     for (int j = 0; j < 16; j++) {
-                        const float p0 = __uint_as_float(s[2 * j]), p1 = __uint_as_float(s[2 * j + 1]);
+                        const float p0 = ex2(fmaf(__uint_as_float(s[32 * ch + 2 * j]), fac, ref));
+                        const float p1 = ex2(fmaf(__uint_as_float(s[32 * ch + 2 * j + 1]), fac, ref));
+                        sum[0] += p0, sum[1] += p1;
                         h[j] = pack2(p0, p1);
-                        if constexpr (P::LO) s[j] = rest2(p0, p1, h[j]);
+                        if constexpr (P::LO) lo[j] = rest2(p0, p1, h[j]);
                     }
                     tmem_st16(tS + 32 * ch, h);
-                    if constexpr (P::LO) tmem_st16(tS + 32 * ch + 16, s);
+                    if constexpr (P::LO) tmem_st16(tS + 32 * ch + 16, lo);
                 }
                 l = fmaf(sum[0] + sum[1], exp2i(P::QN ? -(int)ev : 0), l);
                 tmem_wait_st();
                 return true;
             };
-            bool ok = true;  // (a warp that gave up still meets its group at every tile)
-            for (int i = (n0 & 1) ^ wg; i < N; i += 2) {
+            for (int i = 0; i < N; i++) {
                 const int n = n0 + i;
                 ok = ok && tile(i);
                 tc_fence_before();
-                bar_sync(4 + wg, 128);
-                if (issues && ok) {
-                    tc_fence_after();
-                    pv(n, i < 2);
-                    // (P lies over S: its product is done before the next S)
-                    if (i + 2 < N && kc_wait(&sh.odone[wg], (n >> 1) & 1, abort_flag, err)) qk(n + 2);
-                }
                 __syncwarp();
+                if (ok && lane == 0) mbar_arrive(&sh.pfull[wg][n & 1]);
             }
+            // both groups' products are done
+            const int last = n0 + N - 1;
+            ok = __all_sync(FULL, ok && *abort_flag == 0);
+            ok = ok && kc_wait_warp(&sh.odone[last & 1], (last >> 1) & 1, abort_flag, err);
+            if (N > 1) marks(N - 2);
+            marks(N - 1);
             sh.ml[wg][0][r] = m;
             sh.ml[wg][1][r] = l;
-            // both groups' products are done: this group's last tile, and the other's
-            ok = __all_sync(FULL, ok && *abort_flag == 0);
-#pragma unroll
-            for (int w = 0; w < 2; w++) {
-                const int last = n0 + N - 1 - ((n0 + N - 1 - w) & 1);  // the last tile of group w
-                if (last >= n0 && ok) ok = kc_wait_warp(&sh.odone[w], (last >> 1) & 1, abort_flag, err);
-            }
             tc_fence_after();
             bar_sync(3, 256);
             // the row's sums: each group writes half of the dims
-            const int w0 = n0 & 1;
-            const bool two = N > 1;
-            const float ma = sh.ml[w0][0][r], mb = two ? sh.ml[w0 ^ 1][0][r] : -INFINITY;
+            const float ma = sh.ml[0][0][r], mb = sh.ml[1][0][r];
             const float mx = fmaxf(ma, mb), safe = mx == -INFINITY ? 0.0f : mx;
             const float fa = ex2(ma - safe), fb = ex2(mb - safe);
-            const float lt = sh.ml[w0][1][r] * fa + (two ? sh.ml[w0 ^ 1][1][r] * fb : 0.0f);
+            const float lt = sh.ml[0][1][r] * fa + sh.ml[1][1][r] * fb;
             const bool whole = N == cc.tiles;
             const int c0 = whole ? 0 : cut.owner(cc.first);
             float* mine = reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + KV_TICKETS) +
                           (size_t)(2 * cta + (cta == c0)) * P::PART;
             const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
             // (Q's memory is free: every product is done) the rows of the output, 16-byte pieces moved among eight
-            constexpr int ROW = D * sizeof(T);
+            constexpr int ROW = D * sizeof(T), E = 16 / sizeof(T);  // E elements of a piece
+            auto stage = [&](int d, const float* y) {  // dims d … d + 15 of the thread's row
+#pragma unroll
+                for (int j = 0; j < 16 / E; j++) {
+                    uint4 w;
+                    if constexpr (P::LO)
+                        w = make_uint4(__float_as_uint(y[4 * j]), __float_as_uint(y[4 * j + 1]), __float_as_uint(y[4 * j + 2]),
+                                       __float_as_uint(y[4 * j + 3]));
+                    else
+                        w = make_uint4(pack2(y[8 * j], y[8 * j + 1]), pack2(y[8 * j + 2], y[8 * j + 3]),
+                                       pack2(y[8 * j + 4], y[8 * j + 5]), pack2(y[8 * j + 6], y[8 * j + 7]));
+                    *reinterpret_cast<uint4*>(Qh + r * ROW + (((d / E + j) ^ (r & 7)) << 4)) = w;
+                }
+            };
+            bool emit = whole && ok;
             if (ok) {
 #pragma unroll 1
                 for (int d = wg * (D / 2); d < (wg + 1) * (D / 2); d += 16) {
                     uint32_t o[16], o2[16];
-                    tmem_ld16(tmem + lanes + 256 + w0 * 128 + d, o);
-                    if (two) tmem_ld16(tmem + lanes + 256 + (w0 ^ 1) * 128 + d, o2);
+                    tmem_ld16(tmem + lanes + 256 + d, o);
+                    tmem_ld16(tmem + lanes + 384 + d, o2);
                     tmem_wait_ld();
                     float y[16];
 #pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        y[j] = __uint_as_float(o[j]) * fa;
-                        if (two) y[j] = fmaf(__uint_as_float(o2[j]), fb, y[j]);
-                    }
-                    if (!whole) {
+                    for (int j = 0; j < 16; j++) y[j] = fmaf(__uint_as_float(o2[j]), fb, __uint_as_float(o[j]) * fa);
+                    if (whole) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++) y[j] = lt == 0.0f ? 0.0f : y[j] * inv;
+                        stage(d, y);
+                    } else {
 #pragma unroll
                         for (int j = 0; j < 16; j++) __stcg(&mine[(d + j) * KC_M + r], y[j]);
-                        continue;
-                    }
-#pragma unroll
-                    for (int j = 0; j < 16; j++) y[j] = lt == 0.0f ? 0.0f : y[j] * inv;
-                    constexpr int E = 16 / sizeof(T);  // elements of a piece
-#pragma unroll
-                    for (int j = 0; j < 16 / E; j++) {
-                        uint4 w;
-                        if constexpr (P::LO)
-                            w = make_uint4(__float_as_uint(y[4 * j]), __float_as_uint(y[4 * j + 1]),
-                                           __float_as_uint(y[4 * j + 2]), __float_as_uint(y[4 * j + 3]));
-                        else
-                            w = make_uint4(pack2(y[8 * j], y[8 * j + 1]), pack2(y[8 * j + 2], y[8 * j + 3]),
-                                           pack2(y[8 * j + 4], y[8 * j + 5]), pack2(y[8 * j + 6], y[8 * j + 7]));
-                        *reinterpret_cast<uint4*>(Qh + r * ROW + (((d / E + j) ^ (r & 7)) << 4)) = w;
-                    }
-                }
-                if (whole) {
-                    bar_sync(3, 256);
-                    constexpr int PC = ROW / 16;
-                    for (int e = tid; e < rows * PC; e += 256) {
-                        const int rr = e / PC, pc = e % PC;
-                        T* op = static_cast<T*>(a.out) + slot * a.o_slot + ((r0 + rr) / G) * a.o_row +
-                                (cc.h * G + (r0 + rr) % G) * a.o_head;
-                        reinterpret_cast<uint4*>(op)[pc] = *reinterpret_cast<const uint4*>(Qh + rr * ROW + ((pc ^ (rr & 7)) << 4));
                     }
                 }
                 if (!whole && wg == 0) {
@@ -707,51 +819,58 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 if (!whole) __threadfence();
             }
             tc_fence_before();
-        }
-        __syncthreads();
-        tc_fence_after();
-        if (*abort_flag) break;
-        // ---- a triple that lies in several CTAs: the last of them joins the parts in the CTAs' order ----
-        if (N != cc.tiles) {
-            const int c0 = cut.owner(cc.first), c1 = cut.owner(cc.first + cc.tiles - 1);
-            uint32_t* tickets = static_cast<uint32_t*>(a.work);
-            if (tid == 0) {
-                const bool last = atomicAdd(&tickets[c0], 1u) == (uint32_t)(c1 - c0);
-                if (last) tickets[c0] = 0;
-                __threadfence();
-                sh.last = last;
-            }
-            __syncthreads();
-            if (sh.last) {
-                const int r = tid & 127, d0 = (tid >> 7) * (D / 4);
-                const float* parts = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.work) + KV_TICKETS);
-                auto of = [&](int i) { return parts + (size_t)(2 * i + (i == c0)) * P::PART; };
-                float mx = -INFINITY, l = 0.0f, y[D / 4] = {};
-                for (int i = c0; i <= c1; i++) mx = fmaxf(mx, __ldcg(&of(i)[D * KC_M + r]));
-                if (mx == -INFINITY) mx = 0.0f;
-                for (int i = c0; i <= c1; i++) {
-                    const float* q = of(i);
-                    const float f = ex2(__ldcg(&q[D * KC_M + r]) - mx);
-                    l = fmaf(__ldcg(&q[(D + 1) * KC_M + r]), f, l);
-#pragma unroll
-                    for (int d = 0; d < D / 4; d++) y[d] = fmaf(__ldcg(&q[(d0 + d) * KC_M + r]), f, y[d]);
+            bar_sync(3, 256);
+            // ---- a triple that lies in several CTAs: the last of them joins the parts in the CTAs' order ----
+            if (!whole) {
+                const int c1 = cut.owner(cc.first + cc.tiles - 1);
+                uint32_t* tickets = static_cast<uint32_t*>(a.work);
+                if (tid == 0) {  // (after a wait that gave up nothing is joined; the host sets the tickets back)
+                    const bool last_one = *abort_flag == 0 && atomicAdd(&tickets[c0], 1u) == (uint32_t)(c1 - c0);
+                    if (last_one) tickets[c0] = 0;
+                    __threadfence();
+                    sh.last = last_one;
                 }
-                if (r < rows) {
-                    T* op = static_cast<T*>(a.out) + slot * a.o_slot + ((r0 + r) / G) * a.o_row +
-                            (cc.h * G + (r0 + r) % G) * a.o_head + d0;
-                    const float inv = 1.0f / l;
+                bar_sync(3, 256);
+                emit = sh.last;
+                if (emit) {
+                    const float* parts = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.work) + KV_TICKETS);
+                    auto of = [&](int i) { return parts + (size_t)(2 * i + (i == c0)) * P::PART; };
+                    float top = -INFINITY, sum = 0.0f;
+                    for (int i = c0; i <= c1; i++) top = fmaxf(top, __ldcg(&of(i)[D * KC_M + r]));
+                    if (top == -INFINITY) top = 0.0f;
+                    for (int i = c0; i <= c1; i++)
+                        sum = fmaf(__ldcg(&of(i)[(D + 1) * KC_M + r]), ex2(__ldcg(&of(i)[D * KC_M + r]) - top), sum);
+                    const float scale = 1.0f / sum;
+#pragma unroll 1
+                    for (int d = wg * (D / 2); d < (wg + 1) * (D / 2); d += 16) {
+                        float y[16] = {};
+#pragma unroll 1
+                        for (int i = c0; i <= c1; i++) {
+                            const float* q = of(i);
+                            const float f = ex2(__ldcg(&q[D * KC_M + r]) - top);
 #pragma unroll
-                    for (int d = 0; d < D / 4; d++) op[d] = (T)(l == 0.0f ? 0.0f : y[d] * inv);
+                            for (int j = 0; j < 16; j++) y[j] = fmaf(__ldcg(&q[(d + j) * KC_M + r]), f, y[j]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; j++) y[j] = sum == 0.0f ? 0.0f : y[j] * scale;
+                        stage(d, y);
+                    }
+                }
+                bar_sync(3, 256);
+            }
+            if (emit) {
+                constexpr int PC = ROW / 16;
+                for (int e = tid; e < rows * PC; e += 256) {
+                    const int rr = e / PC, pc = e % PC;
+                    T* op = static_cast<T*>(a.out) + slot * a.o_slot + ((r0 + rr) / G) * a.o_row + (cc.h * G + (r0 + rr) % G) * a.o_head;
+                    reinterpret_cast<uint4*>(op)[pc] = *reinterpret_cast<const uint4*>(Qh + rr * ROW + ((pc ^ (rr & 7)) << 4));
                 }
             }
+            bar_sync(3, 256);
         }
         n0 += N;
         seg = seg_end;
     }
-    // ---- every product complete before the TMEM is given back ----
-    if (warp < 8 && (tid & 127) == 0 && any_mma) {
-        mma_commit(&sh.mdone[warp >> 2]);
-        mbar_wait(&sh.mdone[warp >> 2], 0, err);
     }
     tc_fence_before();
     __syncthreads();
