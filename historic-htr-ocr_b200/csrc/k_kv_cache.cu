@@ -17,6 +17,7 @@
 namespace ocr {
 
 constexpr int KV_THREADS = 256;
+constexpr int KV_ROWS = 2;  // rows of a thread: K and V of each in flight together
 
 struct F4 {
     float x[4];
@@ -103,75 +104,75 @@ __device__ __forceinline__ F4 values4(const uint8_t* q, __half scale, int l) {
     return v;
 }
 
-template <int TYPE, bool WRITE, class T>
-__global__ void __launch_bounds__(KV_THREADS) k_kv_move(KvMoveArgs a) {
+template <int TYPE, int D, bool WRITE, class T>
+__global__ void __launch_bounds__(KV_THREADS) k_kv_move(const __grid_constant__ KvMoveArgs a, unsigned rows_step) {
     pdl_trigger();
     pdl_wait();
     const KvView& c = a.c;
+    constexpr int NB = D / KV_BLOCK;
     const int lane = threadIdx.x & 31, l = lane & 7;
-    const int nb = c.d / KV_BLOCK;
-    // the block of this thread's eight lanes, in the order [slot][row][head][block]
-    const long unit = ((long)blockIdx.x * KV_THREADS + threadIdx.x) >> 3;
-    const long per_slot = (long)a.r.T * c.n_kv * nb;
-    const int b = (int)(unit / per_slot);
-    bool live = b < c.n_slot;
-    int t = 0, h = 0, blk = 0;
-    size_t at = 0;
-    if (live) {
-        const int u = (int)(unit - b * per_slot);
-        blk = u % nb;
-        h = (u / nb) % c.n_kv;
-        t = u / (nb * c.n_kv);
-        const bool inside = t < a.r.rows(c, b, a.err);
-        if (!WRITE && !inside) {  // a row that is not in use reads as zeros
-            const F4 z = {};
-            store4(static_cast<T*>(a.k) + b * a.k_slot + t * a.k_row + h * a.k_head + blk * KV_BLOCK + 4 * l, z);
-            store4(static_cast<T*>(a.v) + b * a.v_slot + t * a.v_row + h * a.v_head + blk * KV_BLOCK + 4 * l, z);
-        }
-        live = inside;
-        if (live) at = kv_index(c, b, h, kv_row(c, a.r.pos[b] + t));
-    }
-    T* kp = static_cast<T*>(a.k) + b * a.k_slot + t * a.k_row + h * a.k_head + blk * KV_BLOCK + 4 * l;
-    T* vp = static_cast<T*>(a.v) + b * a.v_slot + t * a.v_row + h * a.v_head + blk * KV_BLOCK + 4 * l;
-    const size_t qo = at * kv_row_bytes(TYPE, c.d) + (size_t)blk * kv_row_bytes(TYPE, KV_BLOCK), so = at * nb + blk;
-    if (TYPE == KV_F16) {
-        if (!live) return;
-        __half* kc = reinterpret_cast<__half*>(c.k + qo) + 4 * l;
-        __half* vc = reinterpret_cast<__half*>(c.v + qo) + 4 * l;
+    // this thread's eight lanes take block blk of head h, of slot blockIdx.y's rows t, t + rows_step (one division here;
+    // the rows of a slot in one launch are few enough for 32 bits)
+    const unsigned unit = (blockIdx.x * KV_THREADS + threadIdx.x) >> 3;
+    const unsigned head = unit / NB, t0 = head / (unsigned)c.n_kv;
+    const int blk = unit % NB, h = (int)(head - t0 * c.n_kv), b = blockIdx.y;
+    const int n = a.r.rows(c, b, a.err), pos = a.r.pos[b];
+    const size_t base = kv_index(c, b, h, 0);
+    const long ko = b * a.k_slot + h * a.k_head + blk * KV_BLOCK + 4 * l, vo = b * a.v_slot + h * a.v_head + blk * KV_BLOCK + 4 * l;
+    constexpr int RB = kv_row_bytes(TYPE, D), BB = kv_row_bytes(TYPE, KV_BLOCK);
+    F4 x[KV_ROWS], y[KV_ROWS];
+    size_t at[KV_ROWS];
+    bool live[KV_ROWS];
+#pragma unroll
+    for (int i = 0; i < KV_ROWS; i++) {
+        const unsigned t = t0 + i * rows_step;
+        live[i] = t < (unsigned)n && (i > 0 || t < rows_step);  // (past the first share: the next thread's)
+        at[i] = base + (live[i] ? kv_row(c, pos + (int)t) : 0);
+        x[i] = y[i] = F4{};
         if (WRITE) {
-            const F4 x = load4(kp), y = load4(vp);
-            store4(kc, x);
-            store4(vc, y);
-        } else {
-            const F4 x = load4(kc), y = load4(vc);
-            store4(kp, x);
-            store4(vp, y);
+            if (live[i]) x[i] = load4(static_cast<const T*>(a.k) + ko + t * a.k_row), y[i] = load4(static_cast<const T*>(a.v) + vo + t * a.v_row);
+        } else if (live[i]) {
+            const uint8_t *kq = c.k + at[i] * RB + blk * BB, *vq = c.v + at[i] * RB + blk * BB;
+            if constexpr (TYPE == KV_F16) {
+                x[i] = load4(reinterpret_cast<const __half*>(kq) + 4 * l), y[i] = load4(reinterpret_cast<const __half*>(vq) + 4 * l);
+            } else {
+                x[i] = values4<TYPE>(kq, c.ks[at[i] * NB + blk], l), y[i] = values4<TYPE>(vq, c.vs[at[i] * NB + blk], l);
+            }
         }
-    } else if (WRITE) {  // (every lane takes part in the block's shuffles)
-        F4 x = {}, y = {};
-        if (live) x = load4(kp), y = load4(vp);
-        quantise4<TYPE>(x, lane, c.k + qo, c.ks + so, live);
-        quantise4<TYPE>(y, lane, c.v + qo, c.vs + so, live);
-    } else if (live) {
-        const F4 x = values4<TYPE>(c.k + qo, c.ks[so], l), y = values4<TYPE>(c.v + qo, c.vs[so], l);
-        store4(kp, x);
-        store4(vp, y);
+    }
+#pragma unroll
+    for (int i = 0; i < KV_ROWS; i++) {
+        const unsigned t = t0 + i * rows_step;
+        if (!WRITE) {  // (a row that is not in use reads as zeros)
+            if (t >= (unsigned)a.r.T || (i == 0 && t >= rows_step)) continue;
+            store4(static_cast<T*>(a.k) + ko + t * a.k_row, x[i]);
+            store4(static_cast<T*>(a.v) + vo + t * a.v_row, y[i]);
+        } else if constexpr (TYPE == KV_F16) {
+            if (!live[i]) continue;
+            store4(reinterpret_cast<__half*>(c.k + at[i] * RB + blk * BB) + 4 * l, x[i]);
+            store4(reinterpret_cast<__half*>(c.v + at[i] * RB + blk * BB) + 4 * l, y[i]);
+        } else {  // (every lane takes part in the block's shuffles)
+            quantise4<TYPE>(x[i], lane, c.k + at[i] * RB + blk * BB, c.ks + at[i] * NB + blk, live[i]);
+            quantise4<TYPE>(y[i], lane, c.v + at[i] * RB + blk * BB, c.vs + at[i] * NB + blk, live[i]);
+        }
     }
 }
 
-template <int TYPE, bool WRITE>
+template <int TYPE, int D, bool WRITE>
 static cudaError_t launch_move(cudaStream_t st, const KvMoveArgs& a, bool pdl) {
-    const long threads = (long)a.c.n_slot * a.r.T * a.c.n_kv * (a.c.d / KV_BLOCK) * 8;
-    const dim3 grid((unsigned)((threads + KV_THREADS - 1) / KV_THREADS));
-    return a.half ? kv_launch(k_kv_move<TYPE, WRITE, __half>, grid, KV_THREADS, 0, st, pdl, a)
-                  : kv_launch(k_kv_move<TYPE, WRITE, float>, grid, KV_THREADS, 0, st, pdl, a);
+    const unsigned step = (unsigned)(a.r.T + KV_ROWS - 1) / KV_ROWS;
+    const long threads = (long)step * a.c.n_kv * (D / KV_BLOCK) * 8;
+    const dim3 grid((unsigned)((threads + KV_THREADS - 1) / KV_THREADS), a.c.n_slot);
+    return a.half ? kv_launch(k_kv_move<TYPE, D, WRITE, __half>, grid, KV_THREADS, 0, st, pdl, a, step)
+                  : kv_launch(k_kv_move<TYPE, D, WRITE, float>, grid, KV_THREADS, 0, st, pdl, a, step);
 }
 template <bool WRITE>
 static cudaError_t launch_move_type(cudaStream_t st, const KvMoveArgs& a, bool pdl) {
+    const bool wide = a.c.d == 128;
     switch (a.c.type) {
-        case KV_F16: return launch_move<KV_F16, WRITE>(st, a, pdl);
-        case KV_Q8_0: return launch_move<KV_Q8_0, WRITE>(st, a, pdl);
-        default: return launch_move<KV_Q4_0, WRITE>(st, a, pdl);
+        case KV_F16: return wide ? launch_move<KV_F16, 128, WRITE>(st, a, pdl) : launch_move<KV_F16, 64, WRITE>(st, a, pdl);
+        case KV_Q8_0: return wide ? launch_move<KV_Q8_0, 128, WRITE>(st, a, pdl) : launch_move<KV_Q8_0, 64, WRITE>(st, a, pdl);
+        default: return wide ? launch_move<KV_Q4_0, 128, WRITE>(st, a, pdl) : launch_move<KV_Q4_0, 64, WRITE>(st, a, pdl);
     }
 }
 cudaError_t launch_kv_write(cudaStream_t st, const KvMoveArgs& a, bool pdl) { return launch_move_type<true>(st, a, pdl); }

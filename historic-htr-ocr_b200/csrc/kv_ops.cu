@@ -63,7 +63,7 @@ ocr_status move(ocr_ctx* ctx, const ocr_kv_cache* c, const ocr_rows* k, const oc
     OCR_TRY(check_rows(v, "v"));
     if (!k->half != !v->half) return fail(OCR_ERR_ARG, "k and v must be of one type");
     OCR_TRY(check_call(c, rows, d_pos));
-    if ((double)c->n_slot * rows * c->n_kv * (c->d_head / KV_BLOCK) / 32 > 2147483647.0)
+    if ((double)rows * c->n_kv * (c->d_head / KV_BLOCK) * 8 > 4294967295.0)  // (the kernel counts a slot's threads in 32 bits)
         return fail(OCR_ERR_ARG, "rows: more than one launch takes");
     OCR_CUDA(cudaSetDevice(ctx->device));
     const KvMoveArgs a{view(c),       {d_pos, d_n, rows}, k->data,        v->data,       k->half ? 1 : 0, k->slot_stride,

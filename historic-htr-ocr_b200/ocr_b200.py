@@ -835,19 +835,19 @@ def kv_cache_bytes(c: KvCacheC) -> tuple[int, int]:
 
 def rows_of(t, cache: KvCache, heads: Optional[int] = None) -> Rows:
     """a device tensor [n_slot][rows][heads][d_head], f32 or f16, of any strides but the last → ocr_rows"""
-    shape, stride, item = t.shape, t.stride(), t.element_size()
-    c = cache.c
+    shape, stride, item, c = t.shape, t.stride(), t.element_size(), cache.c
     if len(shape) != 4 or shape[0] != c.n_slot or shape[3] != c.d_head or stride[3] != 1 or \
-            (heads is not None and shape[2] != heads) or not t.is_floating_point() or \
-            str(t.dtype) not in ("torch.float32", "torch.float16"):
+            (heads is not None and shape[2] != heads) or str(t.dtype) not in ("torch.float32", "torch.float16"):
         raise OcrError(1, "rows must be an f32 or f16 tensor [n_slot][rows][heads][d_head], d_head contiguous")
-    return Rows(t.data_ptr(), int(item == 2), *(s if n > 1 else 0 for s, n in zip(stride[:3], shape)))
+    # (the stride of a dimension of one is anything)
+    return Rows(t.data_ptr(), item == 2, stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0,
+                stride[2] if shape[2] > 1 else 0)
 
 
 def _ints(t, *shape) -> Optional[int]:
     if t is None:
         return None
-    if tuple(t.shape) != shape or str(t.dtype) != "torch.int32" or not t.is_contiguous():
+    if t.shape != shape or str(t.dtype) != "torch.int32" or not t.is_contiguous():
         raise OcrError(1, f"positions, counts, parents and paths are contiguous int32 device tensors, here {list(shape)}")
     return t.data_ptr()
 
@@ -858,8 +858,8 @@ def op_kv_write(ctx: Context, cache: KvCache, k, v, pos, n=None) -> None:
     c = cache.c
     if k.shape != v.shape:
         raise OcrError(1, "k and v must be of one shape")
-    _check(lib().ocr_op_kv_write(ctx.h, C.byref(c), C.byref(rows_of(k, cache, c.n_kv)),
-                                 C.byref(rows_of(v, cache, c.n_kv)), k.shape[1], _ints(pos, c.n_slot),
+    _check(lib().ocr_op_kv_write(ctx.h, c, rows_of(k, cache, c.n_kv),
+                                 rows_of(v, cache, c.n_kv), k.shape[1], _ints(pos, c.n_slot),
                                  _ints(n, c.n_slot)))
 
 
@@ -868,8 +868,8 @@ def op_kv_read(ctx: Context, cache: KvCache, k, v, pos, n=None) -> None:
     c = cache.c
     if k.shape != v.shape:
         raise OcrError(1, "k and v must be of one shape")
-    _check(lib().ocr_op_kv_read(ctx.h, C.byref(c), C.byref(rows_of(k, cache, c.n_kv)),
-                                C.byref(rows_of(v, cache, c.n_kv)), k.shape[1], _ints(pos, c.n_slot),
+    _check(lib().ocr_op_kv_read(ctx.h, c, rows_of(k, cache, c.n_kv),
+                                rows_of(v, cache, c.n_kv), k.shape[1], _ints(pos, c.n_slot),
                                 _ints(n, c.n_slot)))
 
 
@@ -879,9 +879,8 @@ def op_attention_window(ctx: Context, cache: KvCache, q, out, pos, scale: float,
     c = cache.c
     if q.shape != out.shape:
         raise OcrError(1, "q and out must be of one shape")
-    _check(lib().ocr_op_attention_window(ctx.h, C.byref(c), C.byref(rows_of(q, cache)), q.shape[2], q.shape[1],
-                                         _ints(pos, c.n_slot), _ints(n, c.n_slot), scale,
-                                         C.byref(rows_of(out, cache))))
+    _check(lib().ocr_op_attention_window(ctx.h, c, rows_of(q, cache), q.shape[2], q.shape[1],
+                                         _ints(pos, c.n_slot), _ints(n, c.n_slot), scale, rows_of(out, cache)))
 
 
 def op_attention_tree(ctx: Context, cache: KvCache, q, out, pos, parent, scale: float, n=None) -> None:
@@ -890,9 +889,9 @@ def op_attention_tree(ctx: Context, cache: KvCache, q, out, pos, parent, scale: 
     c = cache.c
     if q.shape != out.shape:
         raise OcrError(1, "q and out must be of one shape")
-    _check(lib().ocr_op_attention_tree(ctx.h, C.byref(c), C.byref(rows_of(q, cache)), q.shape[2], q.shape[1],
+    _check(lib().ocr_op_attention_tree(ctx.h, c, rows_of(q, cache), q.shape[2], q.shape[1],
                                        _ints(pos, c.n_slot), _ints(n, c.n_slot), _ints(parent, c.n_slot, q.shape[1]),
-                                       scale, C.byref(rows_of(out, cache))))
+                                       scale, rows_of(out, cache)))
 
 
 def op_kv_keep(ctx: Context, caches: Sequence[KvCache], pos, path, n) -> None:

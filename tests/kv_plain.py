@@ -80,20 +80,41 @@ def sees(pos: int, t: int, j: int, window: int, sinks: int, parent=None) -> bool
     return window == 0 or theirs > mine - window or theirs < sinks
 
 
+def mask_of(pos: int, T: int, window: int, sinks: int, parent=None) -> torch.Tensor:
+    """sees() of every row and position at once"""
+    where = torch.arange(pos + T)
+    if parent is None:
+        mine = where[pos:]
+        seen = where[None] <= mine[:, None]
+    else:
+        d = torch.tensor(depths(parent))
+        where = torch.cat([where[:pos], pos + d])
+        mine = pos + d
+        seen = torch.zeros(T, pos + T, dtype=torch.bool)
+        for t, p in enumerate(parent):
+            seen[t, :pos] = True
+            if p >= 0:
+                seen[t, pos:] = seen[p, pos:]
+            seen[t, pos + t] = True
+    if window:
+        seen &= (where[None] > mine[:, None] - window) | (where[None] < sinks)
+    return seen
+
+
 def attend(q, keys, values, pos: int, scale: float, window: int = 0, sinks: int = 0, parent=None):
     """q [T][n_head][d]; keys, values [n_kv][positions][d] in order of position (the call's own rows last), f64 → [T][n_head][d]"""
     T, H, d = q.shape
     G = H // keys.shape[0]
     n = pos + T
-    mask = torch.tensor([[sees(pos, t, j, window, sinks, parent) for j in range(n)] for t in range(T)])
+    mask = mask_of(pos, T, window, sinks, parent)
     out = torch.zeros(T, H, d, dtype=torch.float64)
     for h in range(H):
         k, v = keys[h // G, :n], values[h // G, :n]
-        for t in range(T):
-            m = mask[t]
-            if not m.any():
-                continue
-            s = (k[m] @ q[t, h]) * scale
-            p = torch.exp(s - s.max())
-            out[t, h] = (p / p.sum()) @ v[m]
+        bad = ~torch.isfinite(v)
+        s = torch.where(mask, (q[:, h] @ k.T) * scale, -math.inf)
+        p = torch.exp(s - s.max(-1, keepdim=True).values)
+        p = torch.where(mask, p, 0.0)  # (a row that sees nothing)
+        o = p @ torch.where(bad, 0.0, v) / p.sum(-1, keepdim=True)
+        o[(mask.double() @ bad.double()) > 0] = math.nan
+        out[:, h] = torch.where(mask.any(-1, keepdim=True), o, 0.0)
     return out

@@ -214,6 +214,41 @@ def test_attention_matches_the_formula(ocr, ctx, kind, item, shape):
     assert torch.equal(got, call())  # the same bits again
 
 
+# many tiles to a CTA, triples cut in pieces and taken whole, more (slot, row block) pairs than the line holds, more slots
+LONG = [
+    (3, 8, 2, 128, 1, [5000, 3000, 4100], 0, 0, False, False),
+    (2, 8, 4, 64, 1, [9000, 8700], 6000, 64, True, False),
+    (600, 1, 2, 64, 1, list(range(600)), 0, 0, False, False),
+    (1, 8, 2, 128, 16, [2303], 0, 0, False, True),
+    (2, 8, 2, 128, 8, [3000, 2900], 0, 0, False, True),
+    (2, 8, 4, 128, 61, [3000, 2000], 1024, 16, False, True),
+    (1, 8, 2, 128, 700, [1500], 0, 0, False, False),
+    (2, 4, 4, 64, 300, [3100, 2500], 0, 0, False, False),
+    (1, 8, 2, 128, 1500, [0], 300, 5, False, False),
+    (1, 4, 2, 64, 500, [2000], 700, 9, True, False),
+    (40, 1, 1, 64, 1700, [0, 7] * 20, 0, 0, False, False),
+]
+
+
+@pytest.mark.parametrize("shape", LONG, ids=lambda s: "-".join(map(str, s)).replace(" ", "")[:60])
+@pytest.mark.parametrize("item", ["f32", "f16"])
+@pytest.mark.parametrize("kind", TYPES)
+def test_long_attention_matches_the_formula(ocr, ctx, kind, item, shape):
+    if shape[0] > 8 and (kind, item) not in (("f16", "f32"), ("q4_0", "f16")):
+        pytest.skip("the schedule is the same for every type")
+    call, want, top = case(ocr, ctx, kind, item, shape)
+    got = call()
+    err = float((got - want).abs().max()) / top
+    assert err <= TOL[item], f"{err:.2e} of the largest value"
+    assert torch.equal(got, call())
+
+
+def test_the_plain_mask_is_its_definition():
+    for pos, T, window, sinks, parent in ((7, 5, 0, 0, None), (20, 6, 8, 3, None), (3, 9, 4, 5, tree(1, 9)), (30, 12, 10, 2, tree(2, 12))):
+        m = P.mask_of(pos, T, window, sinks, parent)
+        assert m.tolist() == [[P.sees(pos, t, j, window, sinks, parent) for j in range(pos + T)] for t in range(T)]
+
+
 @pytest.mark.parametrize("kind", TYPES)
 def test_rows_not_in_use_are_zeros(ocr, ctx, kind):
     for shape, n in (((3, 2, 2, 128, 6, [100, 40, -1], 0, 0, False, False), [4, 0, 6]),
