@@ -19,34 +19,13 @@
 // are split into f16 hi + lo (22 bits); f16 queries are exact, and P is rounded to f16 like the output. A row's query
 // is scaled by a power of two so that its lo part does not fall below f16's range, P likewise by the tile's largest
 // scale.
-#include "kv_attn.cuh"
+#include "kv_tile.cuh"
 
 namespace ocr {
 
 constexpr int KA_ROWS = 32;          // (row, query head) pairs of a kv head up to which this kernel runs
 constexpr int KA_WARPS = 12;
 constexpr int KA_THREADS = KA_WARPS * 32;
-constexpr int KA_RING = 17408;       // a warp's share of the rings: two q8_0 tiles of 32 keys
-
-template <int TYPE, int D>
-struct KaTile {
-    static constexpr int ROW = kv_row_bytes(TYPE, D);
-    static constexpr int NB = TYPE == KV_F16 ? 0 : D / KV_BLOCK;
-    static constexpr int KEYS = TYPE == KV_F16 ? 2048 / D : TYPE == KV_Q8_0 ? 4096 / D : D == 128 ? 32 : 64;
-    static constexpr int K_BYTES = KEYS * ROW, S_BYTES = KEYS * NB * 2;
-    static constexpr int STAGE = 2 * (K_BYTES + S_BYTES);  // K, V, K scales, V scales
-    static constexpr int STAGES = KA_RING / STAGE;         // per warp
-    // the byte offset of 16-byte piece c of key i: permuted so that the eight (K) or four (V) keys that a warp reads at
-    // once lie in different banks
-    __device__ static __forceinline__ int off(int i, int c, bool v) {
-        if (TYPE == KV_F16) return i * ROW + ((c ^ (i & 7)) << 4);
-        if (TYPE == KV_Q8_0 && D == 128)
-            return i * ROW + ((c ^ ((v ? (i >> 2) & 3 : (i & 1) | ((i >> 1) & 2)) << 1)) << 4);
-        if (TYPE == KV_Q8_0) return (i ^ ((i >> 3) & 1)) * ROW + ((c ^ (((i >> 2) & 1) << 1)) << 4);
-        if (D == 128) return i * ROW + ((c ^ ((i >> 2) & 3)) << 4);
-        return (i ^ (((i >> 3) & 1) << 1)) * ROW + ((c ^ ((i >> 2) & 1)) << 4);
-    }
-};
 
 __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm volatile(
@@ -70,35 +49,12 @@ __device__ __forceinline__ void ldmatrix4(uint32_t* r, uint32_t addr) {
                      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                      : "r"(addr));
 }
-// a key's NB scales
-template <int NB>
-__device__ __forceinline__ void load_scales(__half2* d, const uint8_t* scales, int key) {
-    if constexpr (NB == 4) {
-        const uint2 x = *reinterpret_cast<const uint2*>(scales + key * 8);
-        d[0] = *reinterpret_cast<const __half2*>(&x.x), d[1] = *reinterpret_cast<const __half2*>(&x.y);
-    } else {
-        d[0] = *reinterpret_cast<const __half2*>(scales + key * 4);
-    }
-}
-template <int N>
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src, bool live) {
-    const int n = live ? N : 0;  // the rest is filled with zeros
-    if (N == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-    else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 template <int TYPE, int D, int WR, bool PACK, class T>
 __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant__ KvAttnArgs a) {
     using KT = KaTile<TYPE, D>;
     constexpr bool LO = sizeof(T) == 4 && !PACK;  // the lo halves of q and P in products of their own
     constexpr int TEAMS = KA_WARPS / WR;         // WR warps share a ring, eight rows each
-    constexpr int STAGES = KT::STAGES * WR;
+    constexpr int STAGES = KaStream<TYPE, D, WR, TEAMS>::STAGES;
     constexpr int KEYS = KT::KEYS, MT = KEYS / 16, NB = KT::NB;
     constexpr int ROWS = PACK ? 4 : 8;           // of a warp: PACK has four in columns 0 … 3, their lo halves in 4 … 7
     constexpr int KSTEPS = D / 16, DT = D / 16;  // 16-dim steps of S, 16-dim tiles of O
@@ -116,40 +72,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
     const int team = warp / WR, wr = warp % WR, tl = tid - team * WR * 32;
     const int G = a.n_head / c.n_kv;
 
-    // ---- the line: exclusive sums of the slots' tiles ----
-    bool idle_rows = false;
-    int total = 0;
-    for (int b0 = 0; b0 < c.n_slot; b0 += KA_THREADS) {
-        const int b = b0 + tid;
-        KvSpan s;
-        s.nv = 0;
-        if (b < c.n_slot) {
-            s.set(a, b, 0, a.r.T);
-            idle_rows |= s.m < a.r.T;
-        }
-        int x = (s.nv + KEYS - 1) / KEYS * c.n_kv;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(FULL, x, o);
-            if (lane >= o) x += y;
-        }
-        if (lane == 31) wsum[warp] = x;
-        __syncthreads();
-        for (int w = 0; w < warp; w++) x += wsum[w];
-        if (b < c.n_slot) prefix[b + 1] = total + x;
-        for (int w = 0; w < KA_WARPS; w++) total += wsum[w];
-        __syncthreads();
-    }
-    if (tid == 0) prefix[0] = 0;
-    if (__syncthreads_or(idle_rows)) {  // rows that are not in use are zeros
-        const long n = (long)c.n_slot * a.r.T * a.n_head;
-        for (long i = (long)blockIdx.x * KA_WARPS + warp; i < n; i += (long)gridDim.x * KA_WARPS) {
-            const int h = (int)(i % a.n_head), r = (int)(i / a.n_head % a.r.T), b = (int)(i / a.n_head / a.r.T);
-            if (r < a.r.rows(c, b, nullptr)) continue;
-            T* o = static_cast<T*>(a.out) + b * a.o_slot + r * a.o_row + h * a.o_head;
-            for (int d = lane; d < D; d += 32) o[d] = (T)0.0f;
-        }
-    }
+    const int total = kv_line_sums<KEYS, D, T, KA_THREADS>(a, prefix, wsum);
     // parts of at least a tile per team: a short line takes fewer CTAs, and fewer parts to join
     const int n_cta = min((int)gridDim.x, (total + TEAMS - 1) / TEAMS);
     const int cta = blockIdx.x;
@@ -162,65 +85,8 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
     float* joined = reinterpret_cast<float*>(smem + KA_WARPS * KA_RING);  // [4 warps][D / 4 registers][32 lanes]
 
     // ---- the copies of a tile, by the team's threads ----
-    KvCursor lc;
-    KvSpan ls;
-    lc.at(begin, prefix, c.n_slot, c.n_kv);
-    ls.set(a, lc.b, 0, a.r.T);
-    int lt = begin + team, ln = 0;  // the next tile to copy, the copies so far
-    constexpr int PIECES = KT::ROW / 16, KEYS_PER = 32 * WR / PIECES;  // 16-byte pieces of a key; keys of one round
-    const int lkey = tl / PIECES, lpiece = tl % PIECES;
-    auto load = [&]() {
-        if (lt < end) {
-            if (lt >= lc.first + lc.tiles) {
-                lc.at(lt, prefix, c.n_slot, c.n_kv);
-                ls.set(a, lc.b, 0, a.r.T);
-            }
-            const uint32_t dst = smem_u32(ring + ln % STAGES * KT::STAGE);
-            const int v0 = (lt - lc.first) * KEYS, v1 = v0 + KEYS - 1;
-            const size_t base = kv_index(c, lc.b, lc.h, 0);
-            const int r0 = kv_row(c, ls.position(v0));
-            // a tile whose rows lie one after another: one base, constant steps
-            if (v1 < ls.nv && (v0 >= ls.ns || v1 < ls.ns) && kv_row(c, ls.position(v1)) - r0 == KEYS - 1) {
-                const size_t row = base + r0;
-                const uint8_t *kp = c.k + (row + lkey) * KT::ROW + lpiece * 16, *vp = c.v + (row + lkey) * KT::ROW + lpiece * 16;
-#pragma unroll
-                for (int e = 0; e < KEYS / KEYS_PER; e++) {
-                    const int i = lkey + e * KEYS_PER;
-                    cp_async<16>(dst + KT::off(i, lpiece, false), kp + e * KEYS_PER * KT::ROW, true);
-                    cp_async<16>(dst + KT::K_BYTES + KT::off(i, lpiece, true), vp + e * KEYS_PER * KT::ROW, true);
-                }
-                if constexpr (NB > 0) {
-                    const __half *ks = c.ks + (row + tl) * NB, *vs = c.vs + (row + tl) * NB;
-#pragma unroll
-                    for (int i = 0; i < KEYS; i += 32 * WR) {
-                        if (i + tl >= KEYS) break;
-                        cp_async<NB * 2>(dst + 2 * KT::K_BYTES + (i + tl) * NB * 2, ks + i * NB, true);
-                        cp_async<NB * 2>(dst + 2 * KT::K_BYTES + KT::S_BYTES + (i + tl) * NB * 2, vs + i * NB, true);
-                    }
-                }
-            } else {
-#pragma unroll 1
-                for (int i = lkey; i < KEYS; i += KEYS_PER) {
-                    const bool live = v0 + i < ls.nv;
-                    const size_t row = base + (live ? kv_row(c, ls.position(v0 + i)) : 0);
-                    cp_async<16>(dst + KT::off(i, lpiece, false), c.k + row * KT::ROW + lpiece * 16, live);
-                    cp_async<16>(dst + KT::K_BYTES + KT::off(i, lpiece, true), c.v + row * KT::ROW + lpiece * 16, live);
-                }
-                if constexpr (NB > 0) {
-#pragma unroll 1
-                    for (int i = tl; i < KEYS; i += 32 * WR) {
-                        const bool live = v0 + i < ls.nv;
-                        const size_t row = base + (live ? kv_row(c, ls.position(v0 + i)) : 0);
-                        cp_async<NB * 2>(dst + 2 * KT::K_BYTES + i * NB * 2, c.ks + row * NB, live);
-                        cp_async<NB * 2>(dst + 2 * KT::K_BYTES + KT::S_BYTES + i * NB * 2, c.vs + row * NB, live);
-                    }
-                }
-            }
-            lt += TEAMS;
-            ln++;
-        }
-        cp_commit();
-    };
+    KaStream<TYPE, D, WR, TEAMS> stream(a, prefix, begin, end, team, tl, ring);
+    auto load = [&]() { stream.load(); };
 #pragma unroll 1
     for (int i = 0; i < STAGES - 1; i++) load();
 
@@ -763,7 +629,9 @@ static size_t few_work(const KvAttnArgs& a) { return KV_TICKETS + (size_t)a.num_
 static cudaError_t launch_few(cudaStream_t st, const KvAttnArgs& all, bool pdl) {
     for (int b = 0; b < all.c.n_slot; b += KV_LINE) {
         const KvAttnArgs a = kv_slots(all, b, min(KV_LINE, all.c.n_slot - b));
-        const cudaError_t e = a.c.type == KV_F16    ? launch_type<KV_F16>(st, a, pdl)
+        const bool one = a.c.type != KV_F16 && a.r.T * (a.n_head / a.c.n_kv) <= KV_ONE_ROWS;
+        const cudaError_t e = one                   ? launch_kv_attention_one(st, a, pdl)
+                              : a.c.type == KV_F16  ? launch_type<KV_F16>(st, a, pdl)
                               : a.c.type == KV_Q8_0 ? launch_type<KV_Q8_0>(st, a, pdl)
                                                     : launch_type<KV_Q4_0>(st, a, pdl);
         if (e != cudaSuccess) return e;

@@ -112,6 +112,8 @@ inline KvAttnArgs kv_slots(const KvAttnArgs& all, int b, int n) {
     return a;
 }
 cudaError_t launch_kv_attention(cudaStream_t st, const KvAttnArgs& a, bool pdl);
+constexpr int KV_ONE_ROWS = 2;  // (row, query head) pairs of a kv head up to which k_kv_attn_one.cu serves a quantised cache
+cudaError_t launch_kv_attention_one(cudaStream_t st, const KvAttnArgs& a, bool pdl);
 cudaError_t launch_kv_attention_many(cudaStream_t st, const KvAttnArgs& a, bool pdl);
 size_t kv_attention_many_work(const KvAttnArgs& a);
 size_t kv_attention_work_bytes(const KvAttnArgs& a);
