@@ -73,8 +73,8 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
     const int G = a.n_head / c.n_kv;
 
     const int total = kv_line_sums<KEYS, D, T, KA_THREADS>(a, prefix, wsum);
-    // parts of at least a tile per team: a short line takes fewer CTAs, and fewer parts to join
-    const int n_cta = min((int)gridDim.x, (total + TEAMS - 1) / TEAMS);
+    // a short line takes fewer CTAs, and fewer parts to join
+    const int share = kv_least_share(total, c.n_slot * c.n_kv, TEAMS), n_cta = min((int)gridDim.x, (total + share - 1) / share);
     const int cta = blockIdx.x;
     if (cta >= n_cta) return;
     KvLine cut;
@@ -574,11 +574,13 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
                     const int r = w / DT, d = w % DT;
                     float mx[2] = {-INFINITY, -INFINITY}, ll[2] = {0.0f, 0.0f}, x[4] = {};
                     auto ml_of = [&](int i) { return parts + (size_t)(2 * i + (i == c0)) * PART + WR * D * 8 + r * 16; };
+#pragma unroll 8
                     for (int i = c0; i <= c1; i++)
 #pragma unroll
                         for (int j = 0; j < 2; j++) mx[j] = fmaxf(mx[j], __ldcg(&ml_of(i)[2 * t + j]));
 #pragma unroll
                     for (int j = 0; j < 2; j++) mx[j] = mx[j] == -INFINITY ? 0.0f : mx[j];
+#pragma unroll 4  // (the loads of several parts in flight)
                     for (int i = c0; i <= c1; i++) {
                         const float* q = parts + (size_t)(2 * i + (i == c0)) * PART + (r * (D / 4) + 4 * d) * 32 + lane;
                         float f[2];

@@ -61,7 +61,8 @@ __global__ void __launch_bounds__(KO_THREADS, 1) k_kv_attn_one(const __grid_cons
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int G = a.n_head / c.n_kv;
     const int total = kv_line_sums<KEYS, D, T, KO_THREADS>(a, prefix, wsum);
-    const int n_cta = min((int)gridDim.x, (total + KO_WARPS - 1) / KO_WARPS), cta = blockIdx.x;
+    const int share = kv_least_share(total, c.n_slot * c.n_kv, KO_WARPS);
+    const int n_cta = min((int)gridDim.x, (total + share - 1) / share), cta = blockIdx.x;
     if (cta >= n_cta) return;
     KvLine cut;
     cut.cut(total, n_cta);
@@ -413,8 +414,10 @@ __global__ void __launch_bounds__(KO_THREADS, 1) k_kv_attn_one(const __grid_cons
             __syncthreads();
             if (s_last && r < KO_ROWS) {
                 float top = -INFINITY, sum = 0.0f, y = 0.0f;
+#pragma unroll 8
                 for (int i = c0; i <= c1; i++) top = fmaxf(top, __ldcg(&of(i)[KO_ROWS * D + 2 * r]));
                 if (top == -INFINITY) top = 0.0f;
+#pragma unroll 8  // (the loads of several parts in flight)
                 for (int i = c0; i <= c1; i++) {
                     const float* q = of(i);
                     const float f = ex2(__ldcg(&q[KO_ROWS * D + 2 * r]) - top);

@@ -338,7 +338,8 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
         }
     }
     const uint32_t tmem = sh.tmem;
-    const int n_cta = line ? min((int)gridDim.x, total) : (int)gridDim.x;
+    const int least = kv_least_share(total, entries * c.n_kv, 1);
+    const int n_cta = line ? min((int)gridDim.x, (total + least - 1) / least) : (int)gridDim.x;
     const int cta = blockIdx.x;
     KvLine cut;
     cut.cut(total, n_cta);
@@ -779,7 +780,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
             // (Q's memory is free: every product is done) the rows of the output, 16-byte pieces moved among eight
             constexpr int ROW = D * sizeof(T), E = 16 / sizeof(T);  // E elements of a piece
-            auto stage = [&](int d, const float* y) {  // dims d … d + 15 of the thread's row
+            auto stage = [&](int r, int d, const float* y) {  // dims d … d + 15 of row r
 #pragma unroll
                 for (int j = 0; j < 16 / E; j++) {
                     uint4 w;
@@ -806,7 +807,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                     if (whole) {
 #pragma unroll
                         for (int j = 0; j < 16; j++) y[j] = lt == 0.0f ? 0.0f : y[j] * inv;
-                        stage(d, y);
+                        stage(r, d, y);
                     } else {
 #pragma unroll
                         for (int j = 0; j < 16; j++) __stcg(&mine[(d + j) * KC_M + r], y[j]);
@@ -835,25 +836,27 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 if (emit) {
                     const float* parts = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.work) + KV_TICKETS);
                     auto of = [&](int i) { return parts + (size_t)(2 * i + (i == c0)) * P::PART; };
-                    float top = -INFINITY, sum = 0.0f;
-                    for (int i = c0; i <= c1; i++) top = fmaxf(top, __ldcg(&of(i)[D * KC_M + r]));
-                    if (top == -INFINITY) top = 0.0f;
-                    for (int i = c0; i <= c1; i++)
-                        sum = fmaf(__ldcg(&of(i)[(D + 1) * KC_M + r]), ex2(__ldcg(&of(i)[D * KC_M + r]) - top), sum);
-                    const float scale = 1.0f / sum;
+                    // (row, dim) pairs of the rows in use, a warp's side by side; each thread's several in flight at once
+                    const int R = (rows + 31) & ~31;
 #pragma unroll 1
-                    for (int d = wg * (D / 2); d < (wg + 1) * (D / 2); d += 16) {
-                        float y[16] = {};
-#pragma unroll 1
+                    for (int e0 = tid; e0 < R * (D / 16); e0 += 256) {
+                        const int rr = e0 % R, d = e0 / R * 16;
+                        float top = -INFINITY, sum = 0.0f, y[16] = {};
+#pragma unroll 8
+                        for (int i = c0; i <= c1; i++) top = fmaxf(top, __ldcg(&of(i)[D * KC_M + rr]));
+                        if (top == -INFINITY) top = 0.0f;
+#pragma unroll 2
                         for (int i = c0; i <= c1; i++) {
                             const float* q = of(i);
-                            const float f = ex2(__ldcg(&q[D * KC_M + r]) - top);
+                            const float f = ex2(__ldcg(&q[D * KC_M + rr]) - top);
+                            sum = fmaf(__ldcg(&q[(D + 1) * KC_M + rr]), f, sum);
 #pragma unroll
-                            for (int j = 0; j < 16; j++) y[j] = fmaf(__ldcg(&q[(d + j) * KC_M + r]), f, y[j]);
+                            for (int j = 0; j < 16; j++) y[j] = fmaf(__ldcg(&q[(d + j) * KC_M + rr]), f, y[j]);
                         }
+                        const float scale = 1.0f / sum;
 #pragma unroll
                         for (int j = 0; j < 16; j++) y[j] = sum == 0.0f ? 0.0f : y[j] * scale;
-                        stage(d, y);
+                        stage(rr, d, y);
                     }
                 }
                 bar_sync(3, 256);

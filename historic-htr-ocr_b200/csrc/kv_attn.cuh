@@ -104,6 +104,11 @@ __device__ __forceinline__ int kv_depth(int row, const int* parent, int* err) {
     return d;
 }
 
+// The least tiles of a part. A pair in p parts takes its tiles' time / p and p parts to join, a part's join about a
+// quarter of a tile's time for `at_once` tiles side by side: p near the root of the pair's tiles.
+__device__ __forceinline__ int kv_least_share(int total, int pairs, int at_once) {
+    return at_once * max(1, (int)(0.75f * sqrtf((float)total / (float)max(pairs, 1) / (float)at_once)));
+}
 // the line of tiles cut into parts of one size, or one more: CTA i takes tiles part(i) … part(i + 1) - 1
 struct KvLine {
     int n, size, more;  // parts, tiles of each, the first `more` of them have another
