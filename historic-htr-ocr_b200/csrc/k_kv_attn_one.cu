@@ -4,16 +4,17 @@
 // Bound: memory, if the instructions fit beside it: a key of 128 dims is 272 bytes in q8_0, so an SM gets 32 of them in
 // about 380 cycles, and turning their quants into f16 alone takes longer than that. So the quants stay what they are:
 // int8 operands of m16n8k32 (s8 x s8 → s32, the same 8 cycles as the f16 product of half its depth).
-//   S: the query becomes three signed digits to base 256 of a whole number q 2^k (its largest value just below 2^21),
-//      one digit to a column: rows 0, 1 in columns 0, 1 (lowest digit), 2, 3 and 4, 5 (highest). Each block of 32 dims is
-//      one product; its exact sums, times the key's block scale, add up in f32; the three columns of a row are added.
-//   O: a weight times its value's block scale, p d 2^-e (e from the tile's largest scale; p <= 1), becomes a whole
-//      number below 2^21 by one fused multiply-add onto 1.5 2^23, and its three bytes the digits, again a column each. V is the
-//      other operand, four keys' bytes to a word (a 4 x 4 transposition by byte permutes).
+//   S: the query becomes four signed digits to base 256 of a whole number q 2^k (its largest value just below 2^29), a
+//      digit to a column: rows 0, 1 in columns 0, 1 (lowest digit), … 6, 7 (highest). Each block of 32 dims is one
+//      product; its exact sums, times the key's block scale, add up in f32; a row's four columns are added.
+//   O: a weight times its value's block scale, p d 2^(29 - e) (e from the tile's largest scale; p <= 1), becomes a whole
+//      number, and its bytes the digits, again a column each. V is the other operand, four keys' bytes to a word (a
+//      4 x 4 transposition by byte permutes).
 // A q4_0 nibble n becomes the byte 16 (n - 8) by a shift and one logic operation. The accumulators start at the bits of
 // 1.5 2^23, so a sum comes out as a float less a constant (|sums| stay below 2^22: 32 products of 7 bits each, at most
-// two of those). Rounding: 2^-21 of a row's largest query value, 2^-21 of the tile's largest scale (on weights whose largest is 1).
-//
+// two of those). Rounding: 2^-30 of a row's largest query value, 2^-30 of the tile's largest scale (on weights whose
+// largest is 1), and 2^-24 of each. (Three digits of 21 bits: errors of 2 to 6 10^-6 of the output, three times the
+// f32 formula's own.)
 #include "kv_tile.cuh"
 
 namespace ocr {
@@ -22,7 +23,7 @@ constexpr int KO_WARPS = 12, KO_THREADS = KO_WARPS * 32;
 constexpr int KO_ROWS = 2;
 constexpr int KO_MAGIC = 0x4B400000;       // 1.5 2^23
 constexpr float KO_MAGIC_F = 12582912.0f;
-constexpr float KO_DIGITS = 12582912.0f + 32896.0f;  // with half a digit in each of the two lower places: signed digits
+constexpr float KO_DIGITS = 8421504.0f;    // 0x808080: half a digit in each of the three lower places: signed digits
 
 __device__ __forceinline__ void mma16832(int* d, const uint32_t* a, uint32_t b0, uint32_t b1, const int* c) {
     asm volatile(
@@ -73,16 +74,13 @@ __global__ void __launch_bounds__(KO_THREADS, 1) k_kv_attn_one(const __grid_cons
 #pragma unroll 1
     for (int i = 0; i < STAGES - 1; i++) stream.load();
 
-    // column g's digit and row, and how its digit leaves four integers' bytes: ((w | or) - sub) ^ flip
+    // column g's digit and row: that byte of four whole numbers, the lower three digits 128 less
     const int digit = g >> 1, grow = g & 1;
-    const uint32_t sel = (uint32_t)(digit & 3) * 0x11u + 0x40u;  // that byte of two words
-    const uint32_t fix_or = digit == 3 ? ~0u : digit == 2 ? 0x80808080u : 0u, fix_sub = digit == 2 ? 0x40404040u : 0u;
-    const uint32_t fix_flip = digit == 3 ? ~0u : 0x80808080u;
-    auto pick = [&](uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3) {
-        const uint32_t w = __byte_perm(__byte_perm(x0, x1, sel), __byte_perm(x2, x3, sel), 0x5410);
-        return ((w | fix_or) - fix_sub) ^ fix_flip;
+    const uint32_t sel = (uint32_t)digit * 0x11u + 0x40u, flip = digit == 3 ? 0u : 0x80808080u;
+    auto pick = [&](int x0, int x1, int x2, int x3) {
+        return __byte_perm(__byte_perm(x0, x1, sel), __byte_perm(x2, x3, sel), 0x5410) ^ flip;
     };
-    const float place = t == 0 ? 1.0f : t == 1 ? 256.0f : t == 2 ? 65536.0f : 0.0f;  // of this lane's columns 2t, 2t + 1
+    const float place = __uint_as_float((uint32_t)(127 + 8 * t) << 23);  // 256^t, of this lane's columns 2t, 2t + 1
     const int zero[4] = {KO_MAGIC, KO_MAGIC, KO_MAGIC, KO_MAGIC};
     // where the lane reads its keys: S takes rows g, g + 8 of 16 keys (keys kA and kA + 2), V keys 4t … 4t + 3
     const int kA = 4 * (g >> 1) + (g & 1);
@@ -130,24 +128,23 @@ __global__ void __launch_bounds__(KO_THREADS, 1) k_kv_attn_one(const __grid_cons
 #pragma unroll
             for (int o = 1; o <= 2; o <<= 1) big = fmaxf(big, __shfl_xor_sync(FULL, big, o));
             const bool fine = big <= 3.4028234e38f;
-            // 2^(e - 1) <= big < 2^e: times 2^(21 - e)
+            // 2^(e - 1) <= big < 2^e: times 2^(29 - e)
             const int e = big > 0.0f && fine ? max(-100, (int)(__float_as_uint(big) >> 23) - 126) : 0;
-            const float up = __uint_as_float((uint32_t)(127 + min(21 - e, 120)) << 23);
-            const float down = __uint_as_float((uint32_t)(127 - min(21 - e, 120)) << 23);
+            const float up = __uint_as_float((uint32_t)(127 + min(29 - e, 120)) << 23);
+            const float down = __uint_as_float((uint32_t)(127 - min(29 - e, 120)) << 23);
             // (a query that is not finite makes its scores NaN)
             const float f = fine ? a.scale * LOG2E * Q4 * down : NAN;
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    uint32_t n[4];
+                    int n[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) n[i] = __float_as_uint(fmaf(fine ? x[b][4 * u + i] : 0.0f, up, KO_DIGITS));
+                    for (int i = 0; i < 4; i++) n[i] = __float2int_rn(fmaf(fine ? x[b][4 * u + i] : 0.0f, up, KO_DIGITS));
                     qd[b][u] = pick(n[0], n[1], n[2], n[3]);
                 }
             sfac[0] = __shfl_sync(FULL, f, 0) * place;   // row 0 is column 0's
             sfac[1] = __shfl_sync(FULL, f, 4) * place;
-            if (t == 3) sfac[0] = sfac[1] = 0.0f;        // (columns 6 and 7 hold nothing)
         }
         float o[D / 16][4] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
@@ -281,11 +278,11 @@ __global__ void __launch_bounds__(KO_THREADS, 1) k_kv_attn_one(const __grid_cons
 #pragma unroll
             for (int b = 0; b < NB; b++) {
                 const float big = half_of(top[b / 2], b & 1);
-                // 2^(e - 1) <= big < 2^e: p d 2^(21 - e) < 2^21
+                // 2^(e - 1) <= big < 2^e: p d 2^(29 - e) < 2^29
                 const int e = big > 0.0f ? min(17, (int)(__float_as_uint(big) >> 23) - 126) : 0;
-                const float down = __uint_as_float((uint32_t)(127 + 21 - e) << 23);
+                const float down = __uint_as_float((uint32_t)(127 + 29 - e) << 23);
                 float up[2];  // of columns 2t, 2t + 1 (the rows may see different keys)
-                up[0] = up[1] = __uint_as_float((uint32_t)(127 - 21 + e) << 23);
+                up[0] = up[1] = __uint_as_float((uint32_t)(127 - 29 + e) << 23);
                 if (EDGE && many) up[0] = __shfl_sync(FULL, up[0], 0), up[1] = __shfl_sync(FULL, up[1], 4);
                 up[0] *= place * Q4, up[1] *= place * Q4;
                 int acc[2][4];
@@ -295,11 +292,12 @@ __global__ void __launch_bounds__(KO_THREADS, 1) k_kv_attn_one(const __grid_cons
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
                         const int i = 2 * k + u;
-                        uint32_t n[4], x[4];
+                        int n[4];
+                        uint32_t x[4];
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             const float d = b & 1 ? __high2float(dv[i][j][b / 2]) : __low2float(dv[i][j][b / 2]);
-                            n[j] = __float_as_uint(fmaf(w[i][j], d * down, KO_DIGITS));
+                            n[j] = __float2int_rn(fmaf(w[i][j], d * down, KO_DIGITS));
                         }
                         pd[u] = pick(n[0], n[1], n[2], n[3]);
                         if constexpr (TYPE == KV_Q8_0) {

@@ -60,10 +60,9 @@ struct KcPlan {
     static constexpr bool LO = sizeof(T) == 4, QN = TYPE != KV_F16;
     static constexpr int NB = D / KV_BLOCK, ROW = kv_row_bytes(TYPE, D);
     static constexpr uint32_t Q_BYTES = KC_M * D * 2, T_BYTES = KC_KEYS * D * 2;  // one f16 operand of Q; of K or V
-    static constexpr bool VLO = QN && LO;  // f16 rows: V's rounding to f16 is P's and the output's
-    static constexpr int KPARTS = QN ? 2 : 1, VPARTS = VLO ? 2 : 1;               // hi (and lo) of K and of V
+    static constexpr int PARTS = QN ? 2 : 1;                                      // hi (and lo) of K and V
     static constexpr int NS = QN && D == 128 ? 1 : 2;                             // stages
-    static constexpr uint32_t SMEM = (LO ? 2 : 1) * Q_BYTES + NS * (KPARTS + VPARTS) * T_BYTES + 1024;
+    static constexpr uint32_t SMEM = (LO ? 2 : 1) * Q_BYTES + 2 * NS * PARTS * T_BYTES + 1024;
     // the joined parts: [D][128] sums, [128] references, [128] weights' sums
     static constexpr int PART = (D + 2) * KC_M;
 };
@@ -193,8 +192,6 @@ struct KcRaw {
         }
     }
     // The operands, values times 2^-e. `bad` (an edge tile's V): what is not finite becomes zero and its key is marked.
-    // Without LOW only the rounding to f16 is kept.
-    template <bool LOW>
     __device__ static __forceinline__ void store(const uint4* x, uint8_t* hi, uint8_t* lo, const __half* scale, int e,
                                                  uint32_t* bad, int lw, int lane) {
         const float down = exp2i(-e);
@@ -239,10 +236,10 @@ struct KcRaw {
 #pragma unroll
                     for (int y = 0; y < 4; y++) {
                         h[y] = h2mul(q[4 * j + y], d);
-                        l[y] = LOW ? h2rest(q[4 * j + y], d, h[y]) : 0u;
+                        l[y] = h2rest(q[4 * j + y], d, h[y]);
                     }
                     *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
-                    if constexpr (LOW) *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+                    *reinterpret_cast<uint4*>(lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
                 }
             }
         }
@@ -264,7 +261,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
     uint8_t* Qh = sm_raw + ((1024u - (smem_u32(sm_raw) & 1023u)) & 1023u);
     uint8_t* Ql = Qh + P::Q_BYTES;
     uint8_t* Kr = Qh + (P::LO ? 2 : 1) * P::Q_BYTES;
-    uint8_t* Vr = Kr + NS * P::KPARTS * P::T_BYTES;
+    uint8_t* Vr = Kr + NS * P::PARTS * P::T_BYTES;
     pdl_trigger();
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
@@ -488,8 +485,8 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 }
             }
             ok = ok && (n < NS || kc_wait(&sh.kempty[st], (n / NS - 1) & 1, abort_flag, err));
-            uint8_t* kh = Kr + st * P::KPARTS * P::T_BYTES;
-            if (ok) Raw::template store<P::QN>(raw.k, kh, kh + P::T_BYTES, sh.scale[x][0][0], eK, nullptr, lw, lane);
+            uint8_t* kh = Kr + st * P::PARTS * P::T_BYTES;
+            if (ok) Raw::store(raw.k, kh, kh + P::T_BYTES, sh.scale[x][0][0], eK, nullptr, lw, lane);
             fence_proxy_async();
             __syncwarp();
             if (ok && lane == 0) mbar_arrive(&sh.kfull[st]);
@@ -511,9 +508,9 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 if (n + 2 < tiles) load_k(n + 2);
             }
             ok = ok && (n < NS || kc_wait(&sh.vempty[st], (n / NS - 1) & 1, abort_flag, err));
-            uint8_t* vh = Vr + st * P::VPARTS * P::T_BYTES;
+            uint8_t* vh = Vr + st * P::PARTS * P::T_BYTES;
             if (ok)
-                Raw::template store<P::VLO>(raw.v, vh, vh + P::T_BYTES, sh.scale[x][1][0], e, edge ? sh.bad[n % KC_MARKS] : nullptr, lw, lane);
+                Raw::store(raw.v, vh, vh + P::T_BYTES, sh.scale[x][1][0], e, edge ? sh.bad[n % KC_MARKS] : nullptr, lw, lane);
             fence_proxy_async();
             __syncwarp();
             if (ok && lane == 0) mbar_arrive(&sh.vfull[n & 1]);
@@ -537,7 +534,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                     return false;
                 if (!kc_wait(&sh.kfull[st], (n / NS) & 1, abort_flag, err)) return false;
                 tc_fence_after();
-                const uint64_t kh = kd + st * P::KPARTS * T16, kl = kh + T16;
+                const uint64_t kh = kd + st * P::PARTS * T16, kl = kh + T16;
                 // the small products first: a sum loses what falls below its last bit at every product added
                 constexpr int SMALL = (P::LO ? 1 : 0) + (P::QN ? 1 : 0);
 #pragma unroll
@@ -560,7 +557,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 for (int w = 0; w < 2; w++) {
                     if (!kc_wait(&sh.pfull[w][n & 1], (n >> 1) & 1, abort_flag, err)) return false;
                     tc_fence_after();
-                    const uint64_t vh = vd + st * P::VPARTS * T16 + w * HALF * 128 / 16, vl = vh + T16;
+                    const uint64_t vh = vd + st * P::PARTS * T16 + w * HALF * 128 / 16, vl = vh + T16;
                     const uint32_t tP = tmem + (n & 1) * KC_KEYS + w * HALF, tD = tmem + 256 + w * 128;
 #pragma unroll
                     for (int k = 0; k < HALF / 16; k++) {  // 32 keys' P: hi in 16 columns, lo in the next 16
@@ -568,7 +565,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                         const uint64_t o = k * 2048 / 16;
                         mma_f16_ts(tD, p, vh + o, idO, (!fresh || k > 0) ? 1u : 0u);
                         if constexpr (P::LO) mma_f16_ts(tD, p + 16, vh + o, idO, 1u);
-                        if constexpr (P::VLO) mma_f16_ts(tD, p, vl + o, idO, 1u);
+                        if constexpr (P::QN) mma_f16_ts(tD, p, vl + o, idO, 1u);
                     }
                 }
                 mma_commit(&sh.odone[n & 1]);
