@@ -38,7 +38,7 @@ constexpr int KC_LOADERS = 7;
 constexpr int KC_THREADS = (8 + KC_LOADERS + 1) * 32;
 constexpr int KC_RING = 4;  // tiles whose exponents and scales are kept
 constexpr int KC_MARKS = 8;  // tiles whose marks are kept: looked at two tiles later
-constexpr int KC_PIECE = 3;
+constexpr int KC_PIECE = 10;
 constexpr float KC_LAG = 6.0f, KC_BIAS = 8.0f;
 
 template <int BYTES>
@@ -343,9 +343,10 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
     int begin = 0, end = 0;
     KvCursor cc;
     if (line) {
-        // Even parts cut most triples in two, and each piece costs the time of about KC_PIECE tiles (the queries staged,
-        // the sums joined): where triples are short, CTAs take whole ones. (2214 rows in a window of 512, 280 triples of
-        // 6 tiles: 134 us whole, 155 us cut; 128 triples of 66 tiles: cut.)
+        // Even parts cut most triples in two, and each piece costs the time of some KC_PIECE tiles beside its own (the
+        // queries staged, the sums joined); whole ones leave SMs idle. 2214 rows in a window of 512 (280 triples of 6
+        // tiles on 148 SMs): 72 us whole, 129 cut; 666 rows by 2214 keys twice (96 of 18): 62 and 71; 512 rows by 16896
+        // keys four times (256 of 132): 422 and 299.
         const int triples = entries * c.n_kv, per = (triples + (int)gridDim.x - 1) / (int)gridDim.x;
         const long share = total / (int)gridDim.x + 1;
         const long whole_cost = (long)per * (longest + KC_PIECE);
@@ -627,7 +628,8 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                     float big = 0.0f;
 #pragma unroll
                     for (int j = 0; j < V; j++) big = fmaxf(big, fabsf(x[j]));
-                    big = warp_max(big);
+                    // (of floats that are not negative, the bits' order is theirs)
+                    big = __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(big)));
                     const int e = big > 0.0f && big <= 3.4028234e38f ? min(100, 137 - (int)(__float_as_uint(big) >> 23)) : 0;
                     f *= exp2i(-e);
 #pragma unroll
