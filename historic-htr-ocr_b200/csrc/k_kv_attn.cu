@@ -59,8 +59,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
     constexpr int ROWS = PACK ? 4 : 8;           // of a warp: PACK has four in columns 0 … 3, their lo halves in 4 … 7
     constexpr int KSTEPS = D / 16, DT = D / 16;  // 16-dim steps of S, 16-dim tiles of O
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int prefix[KV_LINE + 1];
-    __shared__ int wsum[KA_WARPS];
+    __shared__ KaLine line;
     __shared__ int s_parent[KV_TREE_MAX], s_depth[KV_TREE_MAX];
     __shared__ KvSight s_sight[8 * WR];
     __shared__ float s_ml[4][16];
@@ -72,20 +71,21 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
     const int team = warp / WR, wr = warp % WR, tl = tid - team * WR * 32;
     const int G = a.n_head / c.n_kv;
 
-    const int total = kv_line_sums<KEYS, D, T, KA_THREADS>(a, prefix, wsum);
+    const int total = kv_line_sums<KEYS, D, T, KA_THREADS>(a, line);
     // a short line takes fewer CTAs, and fewer parts to join
     const int share = kv_least_share(total, c.n_slot * c.n_kv, TEAMS), n_cta = min((int)gridDim.x, (total + share - 1) / share);
     const int cta = blockIdx.x;
-    if (cta >= n_cta) return;
     KvLine cut;
     cut.cut(total, n_cta);
-    const int begin = cut.part(cta), end = cut.part(cta + 1);
+    int begin, end;
+    kv_share(cut, cta, line.prefix, c.n_slot, c.n_kv, total, line.longest, (int)gridDim.x, KA_PIECE, KA_PIECE, begin, end);
+    if (begin >= end) return;
 
     uint8_t* ring = smem + team * WR * KA_RING;
     float* joined = reinterpret_cast<float*>(smem + KA_WARPS * KA_RING);  // [4 warps][D / 4 registers][32 lanes]
 
     // ---- the copies of a tile, by the team's threads ----
-    KaStream<TYPE, D, WR, TEAMS> stream(a, prefix, begin, end, team, tl, ring);
+    KaStream<TYPE, D, WR, TEAMS> stream(a, line, begin, end, team, tl, ring);
     auto load = [&]() { stream.load(); };
 #pragma unroll 1
     for (int i = 0; i < STAGES - 1; i++) load();
@@ -95,8 +95,8 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
     for (int seg = begin; seg < end;) {
         KvCursor cc;
         KvSpan sp;
-        cc.at(seg, prefix, c.n_slot, c.n_kv);
-        sp.set(a, cc.b, 0, a.r.T);
+        cc.at(seg, line.prefix, c.n_slot, c.n_kv);
+        sp.set(a, line.pos[cc.b], line.m[cc.b], 0, a.r.T);
         const int seg_end = min(end, cc.first + cc.tiles);
         const int rows = sp.m * G;
         const bool many = a.r.T > 1;
@@ -629,8 +629,8 @@ static cudaError_t launch_type(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
 
 static size_t few_work(const KvAttnArgs& a) { return KV_TICKETS + (size_t)a.num_sms * 2 * 4 * (a.c.d * 8 + 16) * 4; }
 static cudaError_t launch_few(cudaStream_t st, const KvAttnArgs& all, bool pdl) {
-    for (int b = 0; b < all.c.n_slot; b += KV_LINE) {
-        const KvAttnArgs a = kv_slots(all, b, min(KV_LINE, all.c.n_slot - b));
+    for (int b = 0; b < all.c.n_slot; b += KA_LINE) {
+        const KvAttnArgs a = kv_slots(all, b, min(KA_LINE, all.c.n_slot - b));
         const bool one = a.c.type != KV_F16 && a.r.T * (a.n_head / a.c.n_kv) <= KV_ONE_ROWS;
         const cudaError_t e = one                   ? launch_kv_attention_one(st, a, pdl)
                               : a.c.type == KV_F16  ? launch_type<KV_F16>(st, a, pdl)

@@ -50,8 +50,7 @@ __global__ void __launch_bounds__(KO_THREADS, 1) k_kv_attn_one(const __grid_cons
     constexpr int KEYS = KT::KEYS, MT = KEYS / 16, NB = KT::NB, NH = NB / 2, STAGES = Stream::STAGES;
     constexpr float Q4 = TYPE == KV_Q4_0 ? 1.0f / 16 : 1.0f;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int prefix[KV_LINE + 1];
-    __shared__ int wsum[KO_WARPS];
+    __shared__ KaLine line;
     __shared__ KvSight s_sight[KO_ROWS];
     __shared__ int s_parent[KO_ROWS], s_depth[KO_ROWS];
     __shared__ float s_ml[2][KO_ROWS][KO_WARPS];
@@ -61,16 +60,17 @@ __global__ void __launch_bounds__(KO_THREADS, 1) k_kv_attn_one(const __grid_cons
     const KvView& c = a.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int G = a.n_head / c.n_kv;
-    const int total = kv_line_sums<KEYS, D, T, KO_THREADS>(a, prefix, wsum);
+    const int total = kv_line_sums<KEYS, D, T, KO_THREADS>(a, line);
     const int share = kv_least_share(total, c.n_slot * c.n_kv, KO_WARPS);
     const int n_cta = min((int)gridDim.x, (total + share - 1) / share), cta = blockIdx.x;
-    if (cta >= n_cta) return;
     KvLine cut;
     cut.cut(total, n_cta);
-    const int begin = cut.part(cta), end = cut.part(cta + 1);
+    int begin, end;
+    kv_share(cut, cta, line.prefix, c.n_slot, c.n_kv, total, line.longest, (int)gridDim.x, KA_PIECE, KA_PIECE, begin, end);
+    if (begin >= end) return;
     uint8_t* ring = smem + warp * KA_RING;
     float* joined = reinterpret_cast<float*>(smem + KO_WARPS * KA_RING);  // [warp][row][dim]
-    Stream stream(a, prefix, begin, end, warp, lane, ring);
+    Stream stream(a, line, begin, end, warp, lane, ring);
 #pragma unroll 1
     for (int i = 0; i < STAGES - 1; i++) stream.load();
 
@@ -89,8 +89,8 @@ __global__ void __launch_bounds__(KO_THREADS, 1) k_kv_attn_one(const __grid_cons
     for (int seg = begin; seg < end;) {
         KvCursor cc;
         KvSpan sp;
-        cc.at(seg, prefix, c.n_slot, c.n_kv);
-        sp.set(a, cc.b, 0, a.r.T);
+        cc.at(seg, line.prefix, c.n_slot, c.n_kv);
+        sp.set(a, line.pos[cc.b], line.m[cc.b], 0, a.r.T);
         const int seg_end = min(end, cc.first + cc.tiles), rows = sp.m * G;
         const bool many = a.r.T > 1;
         if (many) {
@@ -443,7 +443,7 @@ static cudaError_t launch_type(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
     if (a.c.d == 128) return a.half ? launch_one<TYPE, 128, __half>(st, a, pdl) : launch_one<TYPE, 128, float>(st, a, pdl);
     return a.half ? launch_one<TYPE, 64, __half>(st, a, pdl) : launch_one<TYPE, 64, float>(st, a, pdl);
 }
-// at most KV_LINE slots
+// at most KA_LINE slots
 cudaError_t launch_kv_attention_one(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
     return a.c.type == KV_Q8_0 ? launch_type<KV_Q8_0>(st, a, pdl) : launch_type<KV_Q4_0>(st, a, pdl);
 }

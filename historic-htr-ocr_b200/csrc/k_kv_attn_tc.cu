@@ -347,20 +347,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
         // queries staged, the sums joined); whole ones leave SMs idle. 2214 rows in a window of 512 (280 triples of 6
         // tiles on 148 SMs): 72 us whole, 129 cut; 666 rows by 2214 keys twice (96 of 18): 62 and 71; 512 rows by 16896
         // keys four times (256 of 132): 422 and 299.
-        const int triples = entries * c.n_kv, per = (triples + (int)gridDim.x - 1) / (int)gridDim.x;
-        const long share = total / (int)gridDim.x + 1;
-        const long whole_cost = (long)per * (longest + KC_PIECE);
-        const long cut_cost = share + KC_PIECE * (2 + share * triples / max(total, 1));
-        if (whole_cost <= cut_cost) {
-            auto start = [&](int t) {  // the first tile of triple t
-                if (t >= triples) return total;
-                const int e = t / c.n_kv, tiles = (sh.prefix[e + 1] - sh.prefix[e]) / c.n_kv;
-                return sh.prefix[e] + t % c.n_kv * tiles;
-            };
-            begin = start(cta * per), end = start((cta + 1) * per);
-        } else if (cta < n_cta) {
-            begin = cut.part(cta), end = cut.part(cta + 1);
-        }
+        kv_share(cut, cta, sh.prefix, entries, c.n_kv, total, longest, (int)gridDim.x, KC_PIECE, KC_PIECE / 2, begin, end);
     } else {  // one triple, the last row blocks (the longest) first
         const int per = c.n_slot * c.n_kv;
         const int blk = blocks - 1 - cta / per, b = cta % per / c.n_kv;

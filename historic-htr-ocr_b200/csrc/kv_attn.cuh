@@ -7,7 +7,8 @@
 
 namespace ocr {
 
-constexpr int KV_LINE = 512;      // entries (slots, or slots x row blocks) whose prefix sums a CTA holds
+constexpr int KV_LINE = 512;      // (slot, row block) pairs whose prefix sums a CTA holds (k_kv_attn_tc.cu)
+constexpr int KA_LINE = 256;      // slots of a launch of the attentions of few rows
 constexpr int KV_TICKETS = 4096;  // bytes of the workspace before the partial results: a ticket per CTA
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -50,8 +51,10 @@ __device__ __forceinline__ uint32_t nibbles_h2(uint32_t w) {
 struct KvSpan {
     int pos, m, lo, ns, nv;  // m: the slot's rows in use
     __device__ __forceinline__ void set(const KvAttnArgs& a, int b, int t0, int t1) {
-        pos = a.r.pos[b];
-        m = a.r.rows(a.c, b, a.err);
+        set(a, a.r.pos[b], a.r.rows(a.c, b, a.err), t0, t1);
+    }
+    __device__ __forceinline__ void set(const KvAttnArgs& a, int pos_, int m_, int t0, int t1) {
+        pos = pos_, m = m_;
         const int first = pos + (a.parent ? 0 : t0);
         lo = a.c.window ? max(0, first - a.c.window + 1) : 0;
         ns = min(a.c.sinks, lo);
@@ -119,6 +122,26 @@ struct KvLine {
         return t < 0 ? tile / (size + 1) : more + t / size;
     }
 };
+
+// The tiles begin … end - 1 of CTA i: an even part of the line, or whole pairs (`per` to an entry of prefix) where those
+// take less. Costs in tiles: `piece` for a pair or a piece of one beside its tiles, `join` for the two that are cut.
+__device__ __forceinline__ void kv_share(const KvLine& cut, int i, const int* prefix, int entries, int per, int total, int longest,
+                                         int grid, int piece, int join, int& begin, int& end) {
+    const int pairs = entries * per, each = (pairs + grid - 1) / grid, share = total / grid + 1;
+    const long whole_cost = (long)each * (longest + piece);
+    const long cut_cost = share + (long)piece * (1 + (long)share * pairs / max(total, 1)) + 2L * join;
+    begin = end = 0;
+    if (whole_cost <= cut_cost) {
+        auto start = [&](int t) {  // the first tile of pair t
+            if (t >= pairs) return total;
+            const int e = t / per;
+            return prefix[e] + t % per * ((prefix[e + 1] - prefix[e]) / per);
+        };
+        begin = start(i * each), end = start((i + 1) * each);
+    } else if (i < cut.n) {
+        begin = cut.part(i), end = cut.part(i + 1);
+    }
+}
 
 // where a CTA stands in the line of tiles
 struct KvCursor {

@@ -51,6 +51,13 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
+// Short pairs are taken whole: a pair costs the time of some KA_PIECE tiles beside its own (queries, the teams joined), as
+// much again where it is cut (parts written, counted, joined).
+constexpr int KA_PIECE = 14;
+struct KaLine {
+    int prefix[KA_LINE + 1], pos[KA_LINE], m[KA_LINE];  // of the slots: tiles before, position, rows in use
+    int wsum[32], longest;                              // the most tiles of a pair
+};
 // The copies of a team's tiles (WR warps share a ring; team i of TEAMS takes tiles begin + i, begin + i + TEAMS, …).
 template <int TYPE, int D, int WR, int TEAMS>
 struct KaStream {
@@ -58,25 +65,25 @@ struct KaStream {
     static constexpr int STAGES = KT::STAGES * WR, KEYS = KT::KEYS, NB = KT::NB;
     static constexpr int PIECES = KT::ROW / 16, KEYS_PER = 32 * WR / PIECES;  // 16-byte pieces of a key; keys of one round
     const KvAttnArgs& a;
-    const int* prefix;
+    const KaLine& line;
     KvCursor at;
     KvSpan s;
     uint32_t ring;
     int next, end, count = 0, tl, lkey, lpiece;  // the next tile to copy, the copies so far
-    __device__ __forceinline__ KaStream(const KvAttnArgs& a_, const int* prefix_, int begin, int end_, int team, int tl_,
+    __device__ __forceinline__ KaStream(const KvAttnArgs& a_, const KaLine& line_, int begin, int end_, int team, int tl_,
                                         const uint8_t* ring_)
-        : a(a_), prefix(prefix_), ring(smem_u32(ring_)), next(begin + team), end(end_), tl(tl_), lkey(tl_ / PIECES),
+        : a(a_), line(line_), ring(smem_u32(ring_)), next(begin + team), end(end_), tl(tl_), lkey(tl_ / PIECES),
           lpiece(tl_ % PIECES) {
-        at.at(begin, prefix, a.c.n_slot, a.c.n_kv);
-        s.set(a, at.b, 0, a.r.T);
+        go(begin);
+    }
+    __device__ __forceinline__ void go(int tile) {
+        at.at(tile, line.prefix, a.c.n_slot, a.c.n_kv);
+        s.set(a, line.pos[at.b], line.m[at.b], 0, a.r.T);
     }
     __device__ __forceinline__ void load() {  // the next tile, if there is one; a group of copies either way
         if (next < end) {
             const KvView& c = a.c;
-            if (next >= at.first + at.tiles) {
-                at.at(next, prefix, c.n_slot, c.n_kv);
-                s.set(a, at.b, 0, a.r.T);
-            }
+            if (next >= at.first + at.tiles) go(next);
             const uint32_t dst = ring + count % STAGES * KT::STAGE;
             const int v0 = (next - at.first) * KEYS, v1 = v0 + KEYS - 1;
             const size_t base = kv_index(c, at.b, at.h, 0);
@@ -125,37 +132,43 @@ struct KaStream {
     }
 };
 
-// The line of tiles of all (slot, kv head) pairs, by THREADS threads: exclusive sums of the slots' tiles in prefix
-// [n_slot + 1]; rows that are not in use are set to zeros on the way. → the line's length
+// The line of tiles of all (slot, kv head) pairs; rows that are not in use are set to zeros on the way. → the line's
+// length
 template <int KEYS, int D, class T, int THREADS>
-__device__ __forceinline__ int kv_line_sums(const KvAttnArgs& a, int* prefix, int* wsum) {
+__device__ __forceinline__ int kv_line_sums(const KvAttnArgs& a, KaLine& line) {
+    static_assert(THREADS >= KA_LINE, "a thread per slot");
     const KvView& c = a.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    KvSpan span;
+    span.nv = 0;
     bool idle_rows = false;
-    int total = 0;
-    for (int b0 = 0; b0 < c.n_slot; b0 += THREADS) {
-        const int b = b0 + tid;
-        KvSpan s;
-        s.nv = 0;
-        if (b < c.n_slot) {
-            s.set(a, b, 0, a.r.T);
-            idle_rows |= s.m < a.r.T;
-        }
-        int x = (s.nv + KEYS - 1) / KEYS * c.n_kv;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(FULL, x, o);
-            if (lane >= o) x += y;
-        }
-        if (lane == 31) wsum[warp] = x;
-        __syncthreads();
-        for (int w = 0; w < warp; w++) x += wsum[w];
-        if (b < c.n_slot) prefix[b + 1] = total + x;
-        for (int w = 0; w < THREADS / 32; w++) total += wsum[w];
-        __syncthreads();
+    if (tid < c.n_slot) {
+        span.set(a, tid, 0, a.r.T);
+        idle_rows = span.m < a.r.T;
+        line.pos[tid] = span.pos, line.m[tid] = span.m;
     }
-    if (tid == 0) prefix[0] = 0;
-    if (__syncthreads_or(idle_rows)) {
+    if (tid == 0) line.longest = 0;
+    const int tiles = (span.nv + KEYS - 1) / KEYS;
+    int x = tiles * c.n_kv;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(FULL, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) line.wsum[warp] = x;
+    idle_rows = __syncthreads_or(idle_rows);
+    const int most = __reduce_max_sync(FULL, tiles);
+    if (lane == 0 && most) atomicMax(&line.longest, most);
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; w++) {
+        if (w < warp) x += line.wsum[w];
+        total += line.wsum[w];
+    }
+    if (tid < c.n_slot) line.prefix[tid + 1] = x;
+    if (tid == 0) line.prefix[0] = 0;
+    __syncthreads();
+    if (idle_rows) {
         const long n = (long)c.n_slot * a.r.T * a.n_head;
         for (long i = (long)blockIdx.x * (THREADS / 32) + warp; i < n; i += (long)gridDim.x * (THREADS / 32)) {
             const int h = (int)(i % a.n_head), r = (int)(i / a.n_head % a.r.T), b = (int)(i / a.n_head / a.r.T);
