@@ -15,6 +15,9 @@
 // two of those). Rounding: 2^-30 of a row's largest query value, 2^-30 of the tile's largest scale (on weights whose
 // largest is 1), and 2^-24 of each. (Three digits of 21 bits: errors of 2 to 6 10^-6 of the output, three times the
 // f32 formula's own.)
+// Measured: 32 slots of some 3100 keys, 8 kv heads, two query heads each, q8_0: 55 us, 3.9 TB/s (60 % of a copy's rate; issue
+// 52 % busy, ALU 35, loads and stores 28: the digits' packing and the joins, no single unit); the same in a q4_0 ring of 1028
+// keys 25 us; one slot of 2304 keys 13 us, latency.
 #include "kv_tile.cuh"
 
 namespace ocr {

@@ -2,8 +2,10 @@
 // (kv.cuh), on the 5th-generation tensor cores. The formula is k_kv_attn.cu's.
 //
 // A CTA takes 128 (row, query head) pairs of a kv head (the pairs of a row side by side, so K and V are read once for
-// the whole group) against the keys that any of them sees, in tiles of 128 keys. Bound: the tensor cores (f32 rows),
-// the exponentials (f16 rows: 16 a clock and SM against 128 x 128 of a tile).
+// the whole group) against the keys that any of them sees, in tiles of 128 keys. Floor: the tensor cores. What bounds it now
+// is the chain S → P → O of one triple (one fits an SM) with the softmax's instructions in it: tensor pipe 16 to 20 % busy,
+// issue 32 to 43 %. Measured: 512 f16 rows by 16896 f16 keys, 16 heads of 64, four slots: 308 us, 342 TFLOP/s; 2214 f32 rows
+// in a window of 512, q8_0, 16 heads of 128: 73 us; 8 trees of 61 drafts in windows of 8192, q4_0, f16 rows, 32 heads: 245 us.
 //
 // Products: S = Q K^T (M = N = 128, both operands in shared memory), O += P V (A = P in TMEM, written over S in place;
 // B = V in shared memory, MN-major), f16 operands, f32 sums in TMEM. Exactness: f32 queries and P are f16 hi + lo (22 bits);
@@ -25,9 +27,14 @@
 // is bounded: a role that gives up sets a flag and goes on without work, meeting every barrier, and no copy is in flight
 // (the staging is plain loads and stores).
 //
+// The sums in TMEM lose what falls below their last bit at every product added (about 1.7 10^-8 of a sum each time, towards
+// zero). For f32 rows a group adds its O to a sum of its own in memory after KcPlan::FLUSH tiles and starts O afresh —
+// between a tile's weights and the word that they are there, when the products of the tile before are nearly done. 666 rows
+// by 2214 f16 keys twice: errors of 1.6 10^-6 of the output instead of 2.3, for 7 us of 70. For f16 rows nothing is
+// moved: 40000 keys lose 4 10^-5 of a sum, a sixth of the output's rounding.
+//
 // The work: as in k_kv_attn.cu, the tiles of all (slot, row block, kv head) triples form a line cut evenly over the
-// SMs, triples in several CTAs joined by the last to arrive; past KV_LINE (slot, row block) pairs a CTA takes one
-// triple, longest first.
+// SMs, triples in several CTAs joined by the last to arrive.
 #include "kv_attn.cuh"
 #include "tc.cuh"
 
@@ -63,6 +70,8 @@ struct KcPlan {
     static constexpr int PARTS = QN ? 2 : 1;                                      // hi (and lo) of K and V
     static constexpr int NS = QN && D == 128 ? 1 : 2;                             // stages
     static constexpr uint32_t SMEM = (LO ? 2 : 1) * Q_BYTES + 2 * NS * PARTS * T_BYTES + 1024;
+    // f32 rows: tiles between two moves of O, at most 64 products added to each of its sums in between
+    static constexpr int FLUSH = QN ? 5 : 8;
     // the joined parts: [D][128] sums, [128] references, [128] weights' sums
     static constexpr int PART = (D + 2) * KC_M;
 };
@@ -76,10 +85,10 @@ struct KcShared {
     uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2][2], odone[2],
         xfull[KC_RING], qfull, mdone;
     uint32_t tmem;
-    int abort_flag, last;
+    int abort_flag, last, longest;
     int prefix[KV_LINE + 1], wsum[KC_THREADS / 32];
     float fac[KC_M];             // the rows' factors on S
-    float ml[2][2][KC_M];        // the groups' references and sums
+    float ml[2][3][KC_M];        // the groups' references, sums, and factors on their sums in memory
     int ex[KC_RING][2];          // the tiles' exponents of K and V
     uint32_t bad[KC_MARKS][4];   // keys of an edge tile whose values are not all finite
     __align__(8) uint32_t top[KC_RING][2];  // the largest scales of a tile's K and V (f16 bits)
@@ -247,7 +256,7 @@ struct KcRaw {
 };
 
 template <int TYPE, int D, class T>
-__global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_constant__ KvAttnArgs a, int blocks, int line) {
+__global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_constant__ KvAttnArgs a, int blocks) {
     using P = KcPlan<TYPE, D, T>;
     using Raw = KcRaw<TYPE, D>;
     constexpr int NS = P::NS;
@@ -295,33 +304,36 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
     bool idle_rows = false;
     for (int b = tid; b < c.n_slot; b += KC_THREADS) idle_rows |= a.r.rows(c, b, err) < a.r.T;
     int total = 0, longest = 0;
-    if (line) {
-        int x = 0, mine_tiles = 0;
-        if (tid < entries) {  // (at most KV_LINE of them)
+    if (tid == 0) sh.longest = sh.prefix[0] = 0;
+    for (int e0 = 0; e0 < entries; e0 += KC_THREADS) {
+        const int e = e0 + tid;
+        int sum = 0;
+        if (e < entries) {
             int t0, t1;
-            rows_of_block(tid % blocks, t0, t1);
+            rows_of_block(e % blocks, t0, t1);
             KvSpan s;
-            s.set(a, tid / blocks, t0, t1);
-            mine_tiles = (s.nv + KC_KEYS - 1) / KC_KEYS;
-            x = mine_tiles * c.n_kv;
+            s.set(a, e / blocks, t0, t1);
+            const int tiles = (s.nv + KC_KEYS - 1) / KC_KEYS;
+            longest = max(longest, tiles);
+            sum = tiles * c.n_kv;
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(FULL, x, o);
-            if (lane >= o) x += y;
+            const int y = __shfl_up_sync(FULL, sum, o);
+            if (lane >= o) sum += y;
         }
-        if (lane == 31) sh.wsum[warp] = x;
+        if (lane == 31) sh.wsum[warp] = sum;
         __syncthreads();
-        for (int w = 0; w < warp; w++) x += sh.wsum[w];
-        if (tid < entries) sh.prefix[tid + 1] = x;
-        if (tid == 0) sh.prefix[0] = 0;
-        for (int w = 0; w < KC_THREADS / 32; w++) total += sh.wsum[w];
-        longest = __reduce_max_sync(FULL, tid < entries ? mine_tiles : 0);
+        sum += total;
+        for (int w = 0; w < KC_THREADS / 32; w++) {
+            if (w < warp) sum += sh.wsum[w];
+            total += sh.wsum[w];
+        }
+        if (e < entries) sh.prefix[e + 1] = sum;
         __syncthreads();
-        if (lane == 0) sh.wsum[warp] = longest;
-        __syncthreads();
-        for (int w = 0; w < KC_THREADS / 32; w++) longest = max(longest, sh.wsum[w]);
     }
+    longest = __reduce_max_sync(FULL, longest);
+    if (lane == 0 && longest) atomicMax(&sh.longest, longest);
     tc_fence_before();
     const bool some_idle = __syncthreads_or(idle_rows);
     tc_fence_after();
@@ -336,32 +348,17 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
     }
     const uint32_t tmem = sh.tmem;
     const int least = kv_least_share(total, entries * c.n_kv, 1);
-    const int n_cta = line ? min((int)gridDim.x, (total + least - 1) / least) : (int)gridDim.x;
+    const int n_cta = min((int)gridDim.x, (total + least - 1) / least);
     const int cta = blockIdx.x;
     KvLine cut;
     cut.cut(total, n_cta);
-    int begin = 0, end = 0;
+    int begin, end;
+    // Even parts cut most triples in two, and each piece costs the time of some KC_PIECE tiles beside its own (the
+    // queries staged, the sums joined); whole ones leave SMs idle. 2214 rows in a window of 512 (280 triples of 6
+    // tiles on 148 SMs): 72 us whole, 129 cut; 666 pairs by 2214 keys twice (96 of 18): 62 and 71; 2048 by 16896
+    // keys four times (256 of 132): 422 and 299. (Before sums of f32 rows were moved out of TMEM.)
+    kv_share(cut, cta, sh.prefix, entries, c.n_kv, total, sh.longest, (int)gridDim.x, KC_PIECE, KC_PIECE / 2, begin, end);
     KvCursor cc;
-    if (line) {
-        // Even parts cut most triples in two, and each piece costs the time of some KC_PIECE tiles beside its own (the
-        // queries staged, the sums joined); whole ones leave SMs idle. 2214 rows in a window of 512 (280 triples of 6
-        // tiles on 148 SMs): 72 us whole, 129 cut; 666 rows by 2214 keys twice (96 of 18): 62 and 71; 512 rows by 16896
-        // keys four times (256 of 132): 422 and 299.
-        kv_share(cut, cta, sh.prefix, entries, c.n_kv, total, longest, (int)gridDim.x, KC_PIECE, KC_PIECE / 2, begin, end);
-    } else {  // one triple, the last row blocks (the longest) first
-        const int per = c.n_slot * c.n_kv;
-        const int blk = blocks - 1 - cta / per, b = cta % per / c.n_kv;
-        int t0, t1;
-        rows_of_block(blk, t0, t1);
-        KvSpan s;
-        s.set(a, b, t0, t1);
-        cc.b = b * blocks + blk;
-        cc.h = cta % c.n_kv;
-        cc.first = 0;
-        cc.tiles = (s.nv + KC_KEYS - 1) / KC_KEYS;
-        end = cc.tiles;
-    }
-
     bool any_mma = false;  // (the issuing thread)
     uint32_t qn = 0;
     // a triple: its slot and row block, the keys it sees
@@ -396,9 +393,9 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
         Raw raw{};
         bool ok = true;  // (a thread that gave up still meets the others at every tile's barrier)
         auto find = [&](KvCursor& at, int g) {
-            if (line) at.at(g, sh.prefix, entries, c.n_kv);
+            at.at(g, sh.prefix, entries, c.n_kv);
         };
-        KvCursor kc = cc;
+        KvCursor kc;
         Triple kx;
         Plain kp;
         if (tiles > 0) {
@@ -563,12 +560,12 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             bool go = true;
             int n = 0;
             for (int seg = begin; seg < end && go;) {
-                if (line) cc.at(seg, sh.prefix, entries, c.n_kv);
+                cc.at(seg, sh.prefix, entries, c.n_kv);
                 const int seg_end = min(end, cc.first + cc.tiles), N = seg_end - seg;
                 go = qk(n, true);
                 for (int i = 0; i < N && go; i++, n++) {
                     if (i + 1 < N) go = qk(n + 1, false);
-                    go = go && pv(n, i == 0);
+                    go = go && pv(n, P::LO ? i % P::FLUSH == 0 : i == 0);
                 }
                 seg = seg_end;
             }
@@ -582,7 +579,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
     int n0 = 0;              // tiles of this CTA before the triple
     bool ok = true;          // (a warp that gave up still meets its groups at every barrier)
     for (int seg = begin; seg < end;) {
-        if (line) cc.at(seg, sh.prefix, entries, c.n_kv);
+        cc.at(seg, sh.prefix, entries, c.n_kv);
         const Triple x3 = triple(cc);
         const Plain plain = plain_of(x3);
         const KvSpan& sp = x3.sp;
@@ -655,6 +652,10 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 sight.rows(c, sp, sp.pos + row, sp.pos + row);
             const float fac0 = sh.fac[r];
             float m = -INFINITY, l = 0.0f;
+            // the group's sums in memory, [D][128]: their reference
+            float m_kept = -INFINITY;
+            float* kept = reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + KV_TICKETS) +
+                          (size_t)gridDim.x * 2 * P::PART + (size_t)(2 * cta + wg) * D * KC_M + r;
             constexpr int HALF = KC_KEYS / 2;
             // an edge tile's values that are not finite were taken out of the product (a row that does not see them must not
             // meet them as 0 times infinity); a row that sees one is spoilt as a whole
@@ -697,8 +698,13 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
 #pragma unroll
                 for (int j = 0; j < HALF; j++) mq[j & 3] = fmaxf(mq[j & 3], __uint_as_float(s[j]));
                 const float mt = fmaf(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])), fac, ev);
+                const bool flush = P::LO && i > 0 && i % P::FLUSH == 0;
+                const float m_was = m;
                 if (i == 0) {
                     m = mt;
+                } else if (flush) {  // (O starts afresh)
+                    m = fmaxf(m, mt);
+                    if (m_was != -INFINITY) l *= ex2(m_was - m);
                 } else if (__any_sync(FULL, mt > m + KC_LAG)) {
                     // (warp-uniform: TMEM loads and stores are the whole warp's; a row that stays scales by 1)
                     if (!kc_wait_warp(&sh.odone[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, err)) return false;
@@ -735,6 +741,24 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 }
                 l = fmaf(sum[0] + sum[1], exp2i(P::QN ? -(int)ev : 0), l);
                 tmem_wait_st();
+                if (flush) {
+                    if (!kc_wait_warp(&sh.odone[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, err)) return false;
+                    tc_fence_after();
+                    const float f = m_kept == -INFINITY ? 0.0f : ex2(m_kept - m_was);
+                    const bool more = i > P::FLUSH;
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 32) {
+                        uint32_t o[32];
+                        float k[32];
+                        tmem_ld32(tO + d, o);
+#pragma unroll
+                        for (int j = 0; j < 32; j++) k[j] = more ? __ldcg(&kept[(d + j) * KC_M]) : 0.0f;
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; j++) __stcg(&kept[(d + j) * KC_M], fmaf(k[j], f, __uint_as_float(o[j])));
+                    }
+                    m_kept = m_was;
+                }
                 return true;
             };
             for (int i = 0; i < N; i++) {
@@ -752,6 +776,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             marks(N - 1);
             sh.ml[wg][0][r] = m;
             sh.ml[wg][1][r] = l;
+            sh.ml[wg][2][r] = m_kept == -INFINITY ? 0.0f : ex2(m_kept - m);
             tc_fence_after();
             bar_sync(3, 256);
             // the row's sums: each group writes half of the dims
@@ -786,10 +811,16 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                     uint32_t o[16], o2[16];
                     tmem_ld16(tmem + lanes + 256 + d, o);
                     tmem_ld16(tmem + lanes + 384 + d, o2);
-                    tmem_wait_ld();
-                    float y[16];
+                    float y[16] = {};
+                    if (P::LO && N > P::FLUSH) {
+                        const float *k0 = kept - wg * D * KC_M, *k1 = k0 + D * KC_M;
+                        const float ga = fa * sh.ml[0][2][r], gb = fb * sh.ml[1][2][r];
 #pragma unroll
-                    for (int j = 0; j < 16; j++) y[j] = fmaf(__uint_as_float(o2[j]), fb, __uint_as_float(o[j]) * fa);
+                        for (int j = 0; j < 16; j++) y[j] = fmaf(__ldcg(&k1[(d + j) * KC_M]), gb, __ldcg(&k0[(d + j) * KC_M]) * ga);
+                    }
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 16; j++) y[j] = fmaf(__uint_as_float(o2[j]), fb, fmaf(__uint_as_float(o[j]), fa, y[j]));
                     if (whole) {
 #pragma unroll
                         for (int j = 0; j < 16; j++) y[j] = lt == 0.0f ? 0.0f : y[j] * inv;
@@ -870,28 +901,34 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
 }
 
 template <int TYPE, int D, class T>
-static cudaError_t launch_tc(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
+static cudaError_t launch_tc(cudaStream_t st, const KvAttnArgs& a, int blocks, bool pdl) {
     using P = KcPlan<TYPE, D, T>;
     static PerDeviceOnce once;
     once([] { cudaFuncSetAttribute(k_kv_attn_tc<TYPE, D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::SMEM); });
-    const int blocks = (int)(((long)a.r.T * (a.n_head / a.c.n_kv) + KC_M - 1) / KC_M);
-    const bool line = (long)a.c.n_slot * blocks <= KV_LINE;
-    const long grid = line ? a.num_sms : (long)a.c.n_slot * blocks * a.c.n_kv;
-    return kv_launch(k_kv_attn_tc<TYPE, D, T>, dim3((unsigned)grid), KC_THREADS, P::SMEM, st, pdl, a, blocks, line ? 1 : 0);
+    return kv_launch(k_kv_attn_tc<TYPE, D, T>, dim3(a.num_sms), KC_THREADS, P::SMEM, st, pdl, a, blocks);
 }
 template <int TYPE>
-static cudaError_t launch_type(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
-    if (a.c.d == 128) return a.half ? launch_tc<TYPE, 128, __half>(st, a, pdl) : launch_tc<TYPE, 128, float>(st, a, pdl);
-    return a.half ? launch_tc<TYPE, 64, __half>(st, a, pdl) : launch_tc<TYPE, 64, float>(st, a, pdl);
+static cudaError_t launch_type(cudaStream_t st, const KvAttnArgs& a, int blocks, bool pdl) {
+    if (a.c.d == 128)
+        return a.half ? launch_tc<TYPE, 128, __half>(st, a, blocks, pdl) : launch_tc<TYPE, 128, float>(st, a, blocks, pdl);
+    return a.half ? launch_tc<TYPE, 64, __half>(st, a, blocks, pdl) : launch_tc<TYPE, 64, float>(st, a, blocks, pdl);
 }
-// tickets, and two parts for each CTA
-size_t kv_attention_many_work(const KvAttnArgs& a) { return KV_TICKETS + (size_t)a.num_sms * 2 * (a.c.d + 2) * KC_M * 4; }
-cudaError_t launch_kv_attention_many(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
-    switch (a.c.type) {
-        case KV_F16: return launch_type<KV_F16>(st, a, pdl);
-        case KV_Q8_0: return launch_type<KV_Q8_0>(st, a, pdl);
-        default: return launch_type<KV_Q4_0>(st, a, pdl);
+// tickets, two parts for each CTA, the groups' sums
+size_t kv_attention_many_work(const KvAttnArgs& a) {
+    return KV_TICKETS + (size_t)a.num_sms * 2 * ((a.c.d + 2) + a.c.d) * KC_M * 4;
+}
+// (row, query head) pairs of a kv head in one slot that one call takes
+long kv_attention_many_rows() { return (long)KV_LINE * KC_M; }
+cudaError_t launch_kv_attention_many(cudaStream_t st, const KvAttnArgs& all, bool pdl) {
+    const int blocks = (int)(((long)all.r.T * (all.n_head / all.c.n_kv) + KC_M - 1) / KC_M), slots = KV_LINE / blocks;
+    for (int b = 0; b < all.c.n_slot; b += slots) {
+        const KvAttnArgs a = kv_slots(all, b, min(slots, all.c.n_slot - b));
+        const cudaError_t e = a.c.type == KV_F16    ? launch_type<KV_F16>(st, a, blocks, pdl)
+                              : a.c.type == KV_Q8_0 ? launch_type<KV_Q8_0>(st, a, blocks, pdl)
+                                                    : launch_type<KV_Q4_0>(st, a, blocks, pdl);
+        if (e != cudaSuccess) return e;
     }
+    return cudaSuccess;
 }
 
 }  // namespace ocr

@@ -56,8 +56,6 @@ __device__ __forceinline__ size_t kv_index(const KvView& c, int b, int h, int ro
     return ((size_t)b * c.n_kv + h) * c.n_rows + row;
 }
 
-__device__ __forceinline__ float kv_finite_or_zero(float x) { return fabsf(x) <= 3.4028234e38f ? x : 0.0f; }
-
 // ---- launchers ----
 struct KvMoveArgs {
     KvView c;
@@ -112,10 +110,14 @@ inline KvAttnArgs kv_slots(const KvAttnArgs& all, int b, int n) {
     return a;
 }
 cudaError_t launch_kv_attention(cudaStream_t st, const KvAttnArgs& a, bool pdl);
-constexpr int KV_ONE_ROWS = 2;  // (row, query head) pairs of a kv head up to which k_kv_attn_one.cu serves a quantised cache
+// (row, query head) pairs of a kv head up to which k_kv_attn_one.cu serves a quantised cache: with 2, 32 slots of some 3100
+// keys in q8_0 take 55 us there and 73 in k_kv_attn.cu, in a q4_0 ring of 1028 keys 32 and 41 (cut evenly). Its digits take
+// four columns of eight a pair, so two pairs are what one product holds.
+constexpr int KV_ONE_ROWS = 2;
 cudaError_t launch_kv_attention_one(cudaStream_t st, const KvAttnArgs& a, bool pdl);
 cudaError_t launch_kv_attention_many(cudaStream_t st, const KvAttnArgs& a, bool pdl);
 size_t kv_attention_many_work(const KvAttnArgs& a);
+long kv_attention_many_rows();
 size_t kv_attention_work_bytes(const KvAttnArgs& a);
 
 // a launch that may start while its predecessor on the stream still runs: the kernel calls pdl_wait() before it

@@ -243,6 +243,29 @@ def test_long_attention_matches_the_formula(ocr, ctx, kind, item, shape):
     assert torch.equal(got, call())
 
 
+# a slot's rows past one launch's share of (slot, row block) pairs
+def test_more_slots_than_a_launch_takes(ocr, ctx):
+    shape = (4100, 1, 1, 64, 33, [i % 50 for i in range(4100)], 0, 0, False, False)
+    call, want, top = case(ocr, ctx, "f16", "f16", shape)
+    assert float((call() - want).abs().max()) / top <= TOL["f16"]
+
+
+# many tiles to a whole (row block, kv head), the scores rising (so the reference moves between tiles) or falling
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rising", [True, False])
+def test_scores_that_rise_along_a_long_cache(ocr, ctx, kind, rising):
+    shape = (1, 8, 2, 128, 700, [3000], 0, 0, False, False)
+
+    def change(k, v):
+        f = np.linspace(0.05, 3.0, k.shape[1], dtype=np.float32)
+        k *= (f if rising else f[::-1])[None, :, None, None]
+
+    call, want, top = case(ocr, ctx, kind, "f32", shape, change=change)
+    got = call()
+    assert float((got - want).abs().max()) / top <= TOL["f32"]
+    assert torch.equal(got, call())
+
+
 def test_the_plain_mask_is_its_definition():
     for pos, T, window, sinks, parent in ((7, 5, 0, 0, None), (20, 6, 8, 3, None), (3, 9, 4, 5, tree(1, 9)), (30, 12, 10, 2, tree(2, 12))):
         m = P.mask_of(pos, T, window, sinks, parent)
@@ -510,6 +533,9 @@ def test_arguments_are_refused(ocr, ctx):
                                                                                     device="cuda"), 0.1)
     refused("at most 64", ocr.op_kv_keep, ctx, [long], ps, torch.zeros(2, 65, dtype=torch.int32, device="cuda"), ps)
     refused("one shape", ocr.op_kv_keep, ctx, [long, cache], ps, torch.zeros(2, 4, dtype=torch.int32, device="cuda"), ps)
+    wide = torch.zeros(1, 65537, 8, 64, dtype=torch.float16, device="cuda")
+    refused("more than one launch", ocr.op_attention_window, ctx, make_cache(ocr, "q4_0", 1, 1, 65537, 64), wide, wide,
+            i32([0]), 0.1)
     ring = make_cache(ocr, "q8_0", 2, 2, 32, 128, window=20, sinks=4, ring=True)
     refused("more than the cache", ocr.op_kv_write, ctx, ring, rows(T=10), rows(T=10), ps)
     refused("ring cache", ocr.op_kv_write, ctx, make_cache(ocr, "q8_0", 2, 2, 32, 128, ring=True), k, k, ps)
