@@ -4,8 +4,8 @@
 // A CTA takes 128 (row, query head) pairs of a kv head (the pairs of a row side by side, so K and V are read once for
 // the whole group) against the keys that any of them sees, in tiles of 128 keys. Floor: the tensor cores. What bounds it now
 // is the chain S → P → O of one triple (one fits an SM) with the softmax's instructions in it: tensor pipe 16 to 20 % busy,
-// issue 32 to 43 %. Measured: 512 f16 rows by 16896 f16 keys, 16 heads of 64, four slots: 308 us, 342 TFLOP/s; 2214 f32 rows
-// in a window of 512, q8_0, 16 heads of 128: 73 us; 8 trees of 61 drafts in windows of 8192, q4_0, f16 rows, 32 heads: 245 us.
+// issue 32 to 43 %. Measured: 512 f16 rows by 16896 f16 keys, 16 heads of 64, four slots: 307 us, 343 TFLOP/s; 2214 f32 rows
+// in a window of 512, q8_0, 16 heads of 128: 72 us; 8 trees of 61 drafts in windows of 8192, q4_0, f16 rows, 32 heads: 234 us.
 //
 // Products: S = Q K^T (M = N = 128, both operands in shared memory), O += P V (A = P in TMEM, written over S in place;
 // B = V in shared memory, MN-major), f16 operands, f32 sums in TMEM. Exactness: f32 queries and P are f16 hi + lo (22 bits);
@@ -30,7 +30,7 @@
 // The sums in TMEM lose what falls below their last bit at every product added (about 1.7 10^-8 of a sum each time, towards
 // zero). For f32 rows a group adds its O to a sum of its own in memory after KcPlan::FLUSH tiles and starts O afresh —
 // between a tile's weights and the word that they are there, when the products of the tile before are nearly done. 666 rows
-// by 2214 f16 keys twice: errors of 1.6 10^-6 of the output instead of 2.3, for 7 us of 70. For f16 rows nothing is
+// by 2214 f16 keys twice: errors of 1.6 10^-6 of the output instead of 2.3, for 7 us of 69. For f16 rows nothing is
 // moved: 40000 keys lose 4 10^-5 of a sum, a sixth of the output's rounding.
 //
 // The work: as in k_kv_attn.cu, the tiles of all (slot, row block, kv head) triples form a line cut evenly over the
@@ -478,28 +478,25 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             return eV;
         };
         int eV = 0;
-        if (tiles > 0) {
-            load_k(0);
-            load_v(0, tv, next_edge);
-            eV = put_k(0);
-            if (tiles > 1) load_k(1);
-        }
-        for (int n = 0; n < tiles; n++) {
+        // (from -2: one copy of each step's code — the instruction cache is short of room)
+#pragma unroll 1
+        for (int n = -2; n < tiles; n++) {
             const int st = n % NS, x = n % KC_RING, e = eV;
             const typename Raw::Tile t1 = tv;  // of tile n + 1
             const bool e1 = next_edge;
-            if (n + 1 < tiles) {
-                eV = put_k(n + 1);
-                if (n + 2 < tiles) load_k(n + 2);
+            const bool next = n + 1 >= 0 && n + 1 < tiles;
+            if (next) eV = put_k(n + 1);
+            if (n + 2 < tiles) load_k(n + 2);
+            if (n >= 0) {
+                ok = ok && (n < NS || kc_wait(&sh.vempty[st], (n / NS - 1) & 1, abort_flag, err));
+                uint8_t* vh = Vr + st * P::PARTS * P::T_BYTES;
+                if (ok)
+                    Raw::store(raw.v, vh, vh + P::T_BYTES, sh.scale[x][1][0], e, edge ? sh.bad[n % KC_MARKS] : nullptr, lw, lane);
+                fence_proxy_async();
+                __syncwarp();
+                if (ok && lane == 0) mbar_arrive(&sh.vfull[n & 1]);
             }
-            ok = ok && (n < NS || kc_wait(&sh.vempty[st], (n / NS - 1) & 1, abort_flag, err));
-            uint8_t* vh = Vr + st * P::PARTS * P::T_BYTES;
-            if (ok)
-                Raw::store(raw.v, vh, vh + P::T_BYTES, sh.scale[x][1][0], e, edge ? sh.bad[n % KC_MARKS] : nullptr, lw, lane);
-            fence_proxy_async();
-            __syncwarp();
-            if (ok && lane == 0) mbar_arrive(&sh.vfull[n & 1]);
-            if (n + 1 < tiles) load_v(n + 1, t1, e1);
+            if (next) load_v(n + 1, t1, e1);
         }
     } else if (warp == 15) {
         // ---- the products: Q K^T of tile n + 1, then P V of tile n, the first group's and the second's ----
