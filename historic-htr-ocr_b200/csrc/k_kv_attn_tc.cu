@@ -4,8 +4,8 @@
 // A CTA takes 128 (row, query head) pairs of a kv head (the pairs of a row side by side, so K and V are read once for
 // the whole group) against the keys that any of them sees, in tiles of 128 keys. Floor: the tensor cores. What bounds it now
 // is the chain S → P → O of one triple (one fits an SM) with the softmax's instructions in it: tensor pipe 16 to 20 % busy,
-// issue 32 to 43 %. Measured: 512 f16 rows by 16896 f16 keys, 16 heads of 64, four slots: 307 us, 343 TFLOP/s; 2214 f32 rows
-// in a window of 512, q8_0, 16 heads of 128: 72 us; 8 trees of 61 drafts in windows of 8192, q4_0, f16 rows, 32 heads: 234 us.
+// issue 32 to 43 %. Measured: 512 f16 rows by 16896 f16 keys, 16 heads of 64, four slots: 278 us, 379 TFLOP/s; 2214 f32 rows
+// in a window of 512, q8_0, 16 heads of 128: 64 us; 8 trees of 61 drafts in windows of 8192, q4_0, f16 rows, 32 heads: 217 us.
 //
 // Products: S = Q K^T (M = N = 128, both operands in shared memory), O += P V (A = P in TMEM, written over S in place;
 // B = V in shared memory, MN-major), f16 operands, f32 sums in TMEM. Exactness: f32 queries and P are f16 hi + lo (22 bits);
@@ -30,7 +30,7 @@
 // The sums in TMEM lose what falls below their last bit at every product added (about 1.7 10^-8 of a sum each time, towards
 // zero). For f32 rows a group adds its O to a sum of its own in memory after KcPlan::FLUSH tiles and starts O afresh —
 // between a tile's weights and the word that they are there, when the products of the tile before are nearly done. 666 rows
-// by 2214 f16 keys twice: errors of 1.6 10^-6 of the output instead of 2.3, for 7 us of 69. For f16 rows nothing is
+// by 2214 f16 keys twice: errors of 1.6 10^-6 of the output instead of 2.3, for 6 us of 63. For f16 rows nothing is
 // moved: 40000 keys lose 4 10^-5 of a sum, a sixth of the output's rounding.
 //
 // The work: as in k_kv_attn.cu, the tiles of all (slot, row block, kv head) triples form a line cut evenly over the
@@ -114,6 +114,11 @@ __device__ __forceinline__ bool kc_wait_warp(uint64_t* bar, uint32_t parity, vol
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t* r) {
     tmem_ld16(taddr, r);
     tmem_ld16(taddr + 16, r + 16);
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t x;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(x));
+    return x != 0;
 }
 __device__ __forceinline__ uint32_t h2mul(uint32_t a, uint32_t b) {
     const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
@@ -500,7 +505,8 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
         }
     } else if (warp == 15) {
         // ---- the products: Q K^T of tile n + 1, then P V of tile n, the first group's and the second's ----
-        if (lane == 0) {
+        // one thread by election, not by its number: the compiler then knows that it is one (10 % of the whole kernel's time)
+        if (elect_one()) {
             constexpr uint32_t idS = bg_idesc(KC_KEYS), idO = bg_idesc_mn(D);
             constexpr int HALF = KC_KEYS / 2;
             // the operands' descriptors; a step adds to their address field, in 16-byte units
@@ -519,14 +525,17 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 const uint64_t kh = kd + st * P::PARTS * T16, kl = kh + T16;
                 // the small products first: a sum loses what falls below its last bit at every product added
                 constexpr int SMALL = (P::LO ? 1 : 0) + (P::QN ? 1 : 0);
+#pragma unroll 1
+                for (int x = 0; x <= SMALL; x++) {
+                    const uint64_t aq = P::LO && x == 0 ? ql : qh, bk = P::QN && x == (P::LO ? 1 : 0) ? kl : kh;
+#pragma unroll 1
+                    for (int y = 0; y < D / 64; y++)
 #pragma unroll
-                for (int x = 0; x <= SMALL; x++)
-#pragma unroll
-                    for (int k = 0; k < D / 16; k++) {
-                        const uint64_t o = ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16;
-                        const bool lq = P::LO && x == 0, lk = P::QN && x == (P::LO ? 1 : 0);
-                        mma_f16(tmem + (n & 1) * KC_KEYS, (lq ? ql : qh) + o, (lk ? kl : kh) + o, idS, x + k > 0 ? 1u : 0u);
-                    }
+                        for (int k = 0; k < 4; k++) {
+                            const uint64_t o = (uint64_t)(y * (128 * 128 / 16) + k * 2);
+                            mma_f16(tmem + (n & 1) * KC_KEYS, aq + o, bk + o, idS, x + y + k > 0 ? 1u : 0u);
+                        }
+                }
                 mma_commit(&sh.sfull[n & 1]);
                 mma_commit(&sh.kempty[st]);
                 any_mma = true;
@@ -535,7 +544,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             auto pv = [&](int n, bool fresh) -> bool {
                 const int st = n % NS;
                 if (!kc_wait(&sh.vfull[n & 1], (n >> 1) & 1, abort_flag, err)) return false;
-#pragma unroll
+#pragma unroll 1
                 for (int w = 0; w < 2; w++) {
                     if (!kc_wait(&sh.pfull[w][n & 1], (n >> 1) & 1, abort_flag, err)) return false;
                     tc_fence_after();
@@ -559,11 +568,12 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             for (int seg = begin; seg < end && go;) {
                 cc.at(seg, sh.prefix, entries, c.n_kv);
                 const int seg_end = min(end, cc.first + cc.tiles), N = seg_end - seg;
-                go = qk(n, true);
-                for (int i = 0; i < N && go; i++, n++) {
-                    if (i + 1 < N) go = qk(n + 1, false);
-                    go = go && pv(n, P::LO ? i % P::FLUSH == 0 : i == 0);
+#pragma unroll 1
+                for (int i = -1; i < N && go; i++) {
+                    if (i + 1 < N) go = qk(n + i + 1, i < 0);
+                    if (i >= 0) go = go && pv(n + i, P::LO ? i % P::FLUSH == 0 : i == 0);
                 }
+                n += N;
                 seg = seg_end;
             }
             if (any_mma) {  // every product complete before the TMEM is given back
