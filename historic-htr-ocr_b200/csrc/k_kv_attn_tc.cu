@@ -3,9 +3,10 @@
 //
 // A CTA takes 128 (row, query head) pairs of a kv head (the pairs of a row side by side, so K and V are read once for
 // the whole group) against the keys that any of them sees, in tiles of 128 keys. Floor: the tensor cores. What bounds it now
-// is the chain S → P → O of one triple (one fits an SM) with the softmax's instructions in it: tensor pipe 16 to 20 % busy,
-// issue 32 to 43 %. Measured: 512 f16 rows by 16896 f16 keys, 16 heads of 64, four slots: 278 us, 379 TFLOP/s; 2214 f32 rows
-// in a window of 512, q8_0, 16 heads of 128: 64 us; 8 trees of 61 drafts in windows of 8192, q4_0, f16 rows, 32 heads: 217 us.
+// is the chain S → P → O of one triple (one fits an SM) with the softmax's instructions and the issuing thread's waits in it:
+// before the products were issued by an elected thread (307, 72 and 234 us below) the tensor pipe was 16 to 20 % busy, issue
+// 32 to 42 %. Measured: 512 f16 rows by 16896 f16 keys, 16 heads of 64, four slots: 273 us, 386 TFLOP/s; 2214 f32 rows
+// in a window of 512, q8_0, 16 heads of 128: 63 us; 8 trees of 61 drafts in windows of 8192, q4_0, f16 rows, 32 heads: 211 us.
 //
 // Products: S = Q K^T (M = N = 128, both operands in shared memory), O += P V (A = P in TMEM, written over S in place;
 // B = V in shared memory, MN-major), f16 operands, f32 sums in TMEM. Exactness: f32 queries and P are f16 hi + lo (22 bits);
@@ -30,7 +31,7 @@
 // The sums in TMEM lose what falls below their last bit at every product added (about 1.7 10^-8 of a sum each time, towards
 // zero). For f32 rows a group adds its O to a sum of its own in memory after KcPlan::FLUSH tiles and starts O afresh —
 // between a tile's weights and the word that they are there, when the products of the tile before are nearly done. 666 rows
-// by 2214 f16 keys twice: errors of 1.6 10^-6 of the output instead of 2.3, for 6 us of 63. For f16 rows nothing is
+// by 2214 f16 keys twice: errors of 1.6 10^-6 of the output instead of 2.3, for 6 us of 62. For f16 rows nothing is
 // moved: 40000 keys lose 4 10^-5 of a sum, a sixth of the output's rounding.
 //
 // The work: as in k_kv_attn.cu, the tiles of all (slot, row block, kv head) triples form a line cut evenly over the
@@ -78,11 +79,11 @@ struct KcPlan {
 
 // Barriers: a parity tells one completion only from the next, so a waiter must know that the one before has come and that
 // the one after has not. Per stage: kfull, kempty, vempty (their waiters meet every tile in turn). Per place of S, tile
-// n's being n % 2: sfull, pfull of each group (a group may be a tile ahead of the products, not two: it needs S, which
+// n's being n % 2: sfull, pfull (both groups' warps; a group may be a tile ahead of the products, not two: it needs S, which
 // needs both groups' P of two tiles before), odone, vfull.
 template <int NB>
 struct KcShared {
-    uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2][2], odone[2],
+    uint64_t kfull[2], kempty[2], vfull[2], vempty[2], sfull[2], pfull[2], odone[2],
         xfull[KC_RING], qfull, mdone;
     uint32_t tmem;
     int abort_flag, last, longest;
@@ -284,8 +285,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             mbar_init(&sh.vfull[i], KC_LOADERS);
             mbar_init(&sh.vempty[i], 1);
             mbar_init(&sh.sfull[i], 1);
-            mbar_init(&sh.pfull[i][0], 4);
-            mbar_init(&sh.pfull[i][1], 4);
+            mbar_init(&sh.pfull[i], 8);
             mbar_init(&sh.odone[i], 1);
         }
         for (int i = 0; i < KC_RING; i++) {
@@ -515,12 +515,13 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             constexpr uint64_t T16 = P::T_BYTES / 16;
             auto qk = [&](int n, bool first) -> bool {
                 const int st = n % NS;
+                // (K first: this wait's own time then passes while the products before are still running)
+                if (!kc_wait(&sh.kfull[st], (n / NS) & 1, abort_flag, err)) return false;
                 // (a triple's first: its Q is there, and every product of the one before is done)
                 if (first ? !kc_wait(&sh.qfull, qn++ & 1, abort_flag, err)
                           // P of tile n - 2 lies over this S: its products are done
                           : n >= 2 && !kc_wait(&sh.odone[n & 1], ((n >> 1) - 1) & 1, abort_flag, err))
                     return false;
-                if (!kc_wait(&sh.kfull[st], (n / NS) & 1, abort_flag, err)) return false;
                 tc_fence_after();
                 const uint64_t kh = kd + st * P::PARTS * T16, kl = kh + T16;
                 // the small products first: a sum loses what falls below its last bit at every product added
@@ -544,10 +545,10 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             auto pv = [&](int n, bool fresh) -> bool {
                 const int st = n % NS;
                 if (!kc_wait(&sh.vfull[n & 1], (n >> 1) & 1, abort_flag, err)) return false;
-#pragma unroll 1
+                if (!kc_wait(&sh.pfull[n & 1], (n >> 1) & 1, abort_flag, err)) return false;
+                tc_fence_after();
+#pragma unroll
                 for (int w = 0; w < 2; w++) {
-                    if (!kc_wait(&sh.pfull[w][n & 1], (n >> 1) & 1, abort_flag, err)) return false;
-                    tc_fence_after();
                     const uint64_t vh = vd + st * P::PARTS * T16 + w * HALF * 128 / 16, vl = vh + T16;
                     const uint32_t tP = tmem + (n & 1) * KC_KEYS + w * HALF, tD = tmem + 256 + w * 128;
 #pragma unroll
@@ -773,7 +774,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 ok = ok && tile(i);
                 tc_fence_before();
                 __syncwarp();
-                if (ok && lane == 0) mbar_arrive(&sh.pfull[wg][n & 1]);
+                if (ok && lane == 0) mbar_arrive(&sh.pfull[n & 1]);
             }
             // both groups' products are done
             const int last = n0 + N - 1;
