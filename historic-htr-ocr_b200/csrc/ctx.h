@@ -27,9 +27,8 @@ struct ocr_ctx {
     void* op_scratch = nullptr;
     size_t op_scratch_bytes = 0;
     // partial results and tickets of the attentions over a caller's KV cache: the tickets are zero between calls, so
-    // no other op writes here (grown on demand, freed with the context)
+    // no other op writes here (made by the first of them, freed with the context: captured steps hold its address)
     void* kv_work = nullptr;
-    size_t kv_work_bytes = 0;
     // pinned staging for uploads
     void* h_stage = nullptr;
     void* d_stage = nullptr;

@@ -633,7 +633,8 @@ static cudaError_t launch_type(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
     return a.half ? launch_rows<TYPE, 64, __half>(st, a, pdl) : launch_rows<TYPE, 64, float>(st, a, pdl);
 }
 
-static size_t few_work(const KvAttnArgs& a) { return KV_TICKETS + (size_t)a.num_sms * 2 * 4 * (a.c.d * 8 + 16) * 4; }
+// tickets, two parts for each CTA (of heads of 128, four warps to a team)
+size_t kv_attention_few_work(int num_sms) { return KV_TICKETS + (size_t)num_sms * 2 * 4 * (128 * 8 + 16) * 4; }
 static cudaError_t launch_few(cudaStream_t st, const KvAttnArgs& all, bool pdl) {
     for (int b = 0; b < all.c.n_slot; b += KA_LINE) {
         const KvAttnArgs a = kv_slots(all, b, min(KA_LINE, all.c.n_slot - b));
@@ -651,6 +652,6 @@ static bool is_few(const KvAttnArgs& a) { return (long)a.r.T * (a.n_head / a.c.n
 cudaError_t launch_kv_attention(cudaStream_t st, const KvAttnArgs& a, bool pdl) {
     return is_few(a) ? launch_few(st, a, pdl) : launch_kv_attention_many(st, a, pdl);
 }
-size_t kv_attention_work_bytes(const KvAttnArgs& a) { return is_few(a) ? few_work(a) : kv_attention_many_work(a); }
+size_t kv_attention_work_bytes(int num_sms) { return max(kv_attention_few_work(num_sms), kv_attention_many_work(num_sms)); }
 
 }  // namespace ocr

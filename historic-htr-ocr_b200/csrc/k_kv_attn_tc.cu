@@ -921,10 +921,8 @@ static cudaError_t launch_type(cudaStream_t st, const KvAttnArgs& a, int blocks,
         return a.half ? launch_tc<TYPE, 128, __half>(st, a, blocks, pdl) : launch_tc<TYPE, 128, float>(st, a, blocks, pdl);
     return a.half ? launch_tc<TYPE, 64, __half>(st, a, blocks, pdl) : launch_tc<TYPE, 64, float>(st, a, blocks, pdl);
 }
-// tickets, two parts for each CTA, the groups' sums
-size_t kv_attention_many_work(const KvAttnArgs& a) {
-    return KV_TICKETS + (size_t)a.num_sms * 2 * ((a.c.d + 2) + a.c.d) * KC_M * 4;
-}
+// tickets, two parts for each CTA, the groups' sums (of heads of 128)
+size_t kv_attention_many_work(int num_sms) { return KV_TICKETS + (size_t)num_sms * 2 * ((128 + 2) + 128) * KC_M * 4; }
 // (row, query head) pairs of a kv head in one slot that one call takes
 long kv_attention_many_rows() { return (long)KV_LINE * KC_M; }
 cudaError_t launch_kv_attention_many(cudaStream_t st, const KvAttnArgs& all, bool pdl) {

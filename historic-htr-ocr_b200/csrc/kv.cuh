@@ -116,9 +116,11 @@ cudaError_t launch_kv_attention(cudaStream_t st, const KvAttnArgs& a, bool pdl);
 constexpr int KV_ONE_ROWS = 2;
 cudaError_t launch_kv_attention_one(cudaStream_t st, const KvAttnArgs& a, bool pdl);
 cudaError_t launch_kv_attention_many(cudaStream_t st, const KvAttnArgs& a, bool pdl);
-size_t kv_attention_many_work(const KvAttnArgs& a);
+// the bytes of the workspace that any call needs
+size_t kv_attention_few_work(int num_sms);
+size_t kv_attention_many_work(int num_sms);
+size_t kv_attention_work_bytes(int num_sms);
 long kv_attention_many_rows();
-size_t kv_attention_work_bytes(const KvAttnArgs& a);
 
 // a launch that may start while its predecessor on the stream still runs: the kernel calls pdl_wait() before it
 // touches memory

@@ -72,17 +72,23 @@ ocr_status move(ocr_ctx* ctx, const ocr_kv_cache* c, const ocr_rows* k, const oc
                     write ? "ocr_op_kv_write" : "ocr_op_kv_read");
 }
 
-// the attentions' workspace, zero when it is made (the tickets count from zero, and each last arriver leaves zero)
-ocr_status ensure_kv_work(ocr_ctx* ctx, size_t n) {
-    if (ctx->kv_work_bytes >= n) return OCR_OK;
-    if (ctx->kv_work) {
-        OCR_CUDA(cudaStreamSynchronize(ctx->stream));
-        dfree(ctx->kv_work, ctx->kv_work_bytes, &ctx->mem_work);
-        ctx->kv_work = nullptr;
-        ctx->kv_work_bytes = 0;
+// The attentions' workspace: made by a context's first such call, large enough for any, and kept as long as the context,
+// since a captured step holds its address. Zero when it is made (the tickets count from zero, and each last arriver
+// leaves zero).
+ocr_status ensure_kv_work(ocr_ctx* ctx) {
+    if (ctx->kv_work) return OCR_OK;
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    OCR_CUDA(cudaStreamIsCapturing(ctx->stream, &capture));
+    if (capture != cudaStreamCaptureStatusNone)
+        return fail(OCR_ERR_STATE, "a context's first attention over a KV cache makes its workspace: call one before capturing");
+    const size_t n = kv_attention_work_bytes(ctx->num_sms);
+    void* p = nullptr;
+    const cudaError_t e = dalloc(&p, n, &ctx->mem_work);
+    if (e != cudaSuccess) {
+        if (p) dfree(p, n, &ctx->mem_work);
+        return cuda_fail(e, "the KV attentions' workspace");
     }
-    OCR_CUDA(dalloc(&ctx->kv_work, n, &ctx->mem_work));
-    ctx->kv_work_bytes = n;
+    ctx->kv_work = p;
     return OCR_OK;
 }
 
@@ -103,7 +109,7 @@ ocr_status attend(ocr_ctx* ctx, const ocr_kv_cache* c, const ocr_rows* q, int n_
                  q->half ? 1 : 0, n_head,            q->slot_stride,   q->row_stride,   q->head_stride,
                  out->slot_stride, out->row_stride,  out->head_stride, scale,           nullptr,
                  ctx->num_sms,     ctx->d_err};
-    OCR_TRY(ensure_kv_work(ctx, kv_attention_work_bytes(a)));
+    OCR_TRY(ensure_kv_work(ctx));
     a.work = ctx->kv_work;
     return launched(launch_kv_attention(ctx->stream, a, ctx->pdl), what);
 }

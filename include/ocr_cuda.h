@@ -301,7 +301,8 @@ ocr_status ocr_op_attention_decode(ocr_ctx* ctx, float* d_qkv, const float* d_q_
 /* Operators over ONE layer's KV cache in the caller's device memory (the reference keeps an f16 cache per layer,
  * Session, app/crates/ocr-wgpu/src/text.rs:242-328, and has no counterpart of the rest). All run on the context's
  * stream and return when queued; memory that another stream wrote needs an order against ocr_ctx_stream's stream. The
- * rows' positions and counts are device memory, so a captured step can be replayed as the sequences grow; what is
+ * rows' positions and counts are device memory, so a captured step can be replayed as the sequences grow (a context's
+ * first attention call makes its workspace, 39 MB kept as long as the context: inside a capture it is refused); what is
  * wrong with them shows as OCR_ERR_DEVICE at the next ocr_ctx_sync, and the slot concerned is left alone. */
 enum { OCR_KV_F16 = 1, OCR_KV_Q4_0 = 2, OCR_KV_Q8_0 = 8 }; /* ggml's type numbers */
 /* k and v: quants [n_slot][n_kv][n_rows][row bytes], 16-byte aligned; k_scale and v_scale: f16 [n_slot][n_kv][n_rows]

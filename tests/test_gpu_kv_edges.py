@@ -1,0 +1,87 @@
+"""The KV cache operators where they can go wrong apart from their formulas' ordinary cases: captured steps beside other
+calls, the context's state after an error, the last rows of a cache, numbers far apart, arguments that are no device
+memory. Tolerances are those of test_gpu_kv.py unless a test derives its own."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_kv import i32, make_cache
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- the workspace ----
+def attend(ocr, ctx, T, n_slot=1, keys=2000, d=128, kind="q8_0", seed=0):
+    """a window attention's call over a cache of some contents → (call, out, the tensors it works on)"""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    cache = make_cache(ocr, kind, n_slot, 2, keys + T, d)
+    k, v = (torch.randn(n_slot, keys + T, 2, d, device="cuda", generator=g) for _ in "kv")
+    q = torch.randn(n_slot, T, 4, d, device="cuda", generator=g)
+    out, zero, ps = torch.zeros_like(q), i32([0] * n_slot), i32([keys] * n_slot)
+    torch.cuda.synchronize()
+    ocr.op_kv_write(ctx, cache, k, v, zero)
+    ctx.sync()
+    return lambda: ocr.op_attention_window(ctx, cache, q, out, ps, 0.09), out, (cache, q, ps)
+
+
+def test_the_workspace_does_not_depend_on_the_call(ocr):
+    ctx = ocr.Context(0)
+    held = set()
+    for T, d in ((1, 64), (16, 128), (130, 64), (300, 128)):
+        call, _, keep = attend(ocr, ctx, T, d=d)
+        call()
+        ctx.sync()
+        held.add(ctx.memory()["work"])
+    assert len(held) == 1 and held.pop() > 0
+    ctx.close()
+
+
+def test_a_captured_step_replays_after_larger_calls(ocr):
+    """a decode step and a tree-sized one captured, then prompts on the same context (pairs cut over many CTAs, so that
+    both use the tickets and the partial results), then the replays: the same bits as before"""
+    ctx = ocr.Context(0)
+    stream = torch.cuda.ExternalStream(ctx.stream())
+    steps = [attend(ocr, ctx, T, keys=6000, d=64) for T in (1, 8)]
+    larger = [attend(ocr, ctx, T, n_slot=2, keys=1000 + T, d=128) for T in (100, 700)]
+    want, graphs = [], []
+    for call, out, _ in steps:
+        call()
+        ctx.sync()
+        want.append(out.clone())
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=stream):
+            call()
+        graphs.append(g)
+    for call, out, _ in larger:
+        call()
+    ctx.sync()
+    filler = [torch.full((8 << 20,), 3.0, device="cuda") for _ in range(4)]  # (what was given back would be taken again)
+    for _ in range(2):
+        for g, (_, out, _), w in zip(graphs, steps, want):
+            out.zero_()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                g.replay()
+            ctx.sync()
+            assert torch.equal(out, w)
+    assert all(bool((f == 3).all()) for f in filler)
+    del graphs
+    ctx.close()
+
+
+def test_a_first_call_inside_a_capture_is_refused(ocr):
+    maker, ctx = ocr.Context(0), ocr.Context(0)
+    _, out, (cache, q, ps) = attend(ocr, maker, 3)
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=torch.cuda.ExternalStream(ctx.stream())):
+        with pytest.raises(ocr.OcrError, match="before capturing"):
+            ocr.op_attention_window(ctx, cache, q, out, ps, 0.09)
+    ocr.op_attention_window(ctx, cache, q, out, ps, 0.09)
+    ctx.sync()
+    assert out.any()
+    del g
+    ctx.close()
+    maker.close()
