@@ -496,7 +496,7 @@ class Session:
         """a layer's KV rows, live, as an f16 cache for the op_kv_* and op_attention_* calls"""
         c = KvCacheC()
         _check(lib().ocr_session_kv_cache(self.h, layer, C.byref(c)))
-        return KvCache._of(c, (self,))
+        return KvCache._of(c, (self,), self.model.ctx.device)
 
     def prefill(self, slot: int = 0, ids: Optional[Sequence[int]] = None, embd: Optional[np.ndarray] = None,
                 logits: bool = True) -> Optional[np.ndarray]:
@@ -794,6 +794,16 @@ KV_TYPES = {"f16": 1, "q4_0": 2, "q8_0": 8}
 _KV_ITEM = {1: 2.0, 2: 0.5, 8: 1.0}
 
 
+def _device_of(t, device: Optional[int] = None) -> int:
+    """the GPU that a tensor is on (device: the one it has to be on); the kernels take its address as device memory"""
+    if not getattr(t, "is_cuda", False):
+        raise OcrError(1, f"the KV operators take device tensors, not {type(t).__name__} in host memory")
+    at = t.get_device()
+    if device is not None and at != device:
+        raise OcrError(1, f"a tensor on GPU {at}, its KV cache on GPU {device}")
+    return at
+
+
 class KvCache:
     """A view of one layer's cache (ocr_kv_cache): k, v [n_slot][n_kv][n_rows][row bytes] and, for q8_0 and q4_0, the
     f16 scales [n_slot][n_kv][n_rows][d_head / 32], contiguous device tensors that this view keeps alive. window 0: every
@@ -804,6 +814,7 @@ class KvCache:
         if type not in KV_TYPES:
             raise OcrError(1, f"KV cache type {type!r}: one of {', '.join(KV_TYPES)}")
         t = KV_TYPES[type]
+        self.device = _device_of(k)
         lead = tuple(k.shape[:3])
         for x, width in ((k, int(d_head * _KV_ITEM[t])), (v, int(d_head * _KV_ITEM[t])), (k_scale, d_head // 16),
                          (v_scale, d_head // 16)):
@@ -812,15 +823,22 @@ class KvCache:
             if x is None or tuple(x.shape[:3]) != lead or x.dim() != 4 or not x.is_contiguous() or \
                     x.shape[3] * x.element_size() != width:
                 raise OcrError(1, "KV cache tensors must be contiguous [n_slot][n_kv][n_rows][row], rows of d_head")
+            _device_of(x, self.device)
         self.c = KvCacheC(t, *lead[:2], d_head, lead[2], window, sinks, int(ring), _ptr(k), _ptr(v),
                           None if t == 1 else _ptr(k_scale), None if t == 1 else _ptr(v_scale))
         self._keep = (k, v, k_scale, v_scale)
 
     @classmethod
-    def _of(cls, c: KvCacheC, keep: tuple) -> "KvCache":
+    def _of(cls, c: KvCacheC, keep: tuple, device: int) -> "KvCache":
         v = cls.__new__(cls)
-        v.c, v._keep = c, keep
+        v.c, v._keep, v.device = c, keep, device
         return v
+
+    def _on(self, ctx: Context) -> KvCacheC:
+        """the view for a call on ctx"""
+        if self.device != ctx.device:
+            raise OcrError(1, f"the KV cache is on GPU {self.device}, the context on GPU {ctx.device}")
+        return self.c
 
     def nbytes(self) -> tuple[int, int]:
         """the bytes of k (or v) and of k_scale (or v_scale)"""
@@ -835,6 +853,7 @@ def kv_cache_bytes(c: KvCacheC) -> tuple[int, int]:
 
 def rows_of(t, cache: KvCache, heads: Optional[int] = None) -> Rows:
     """a device tensor [n_slot][rows][heads][d_head], f32 or f16, of any strides but the last → ocr_rows"""
+    _device_of(t, cache.device)
     shape, stride, item, c = t.shape, t.stride(), t.element_size(), cache.c
     if len(shape) != 4 or shape[0] != c.n_slot or shape[3] != c.d_head or stride[3] != 1 or \
             (heads is not None and shape[2] != heads) or str(t.dtype) not in ("torch.float32", "torch.float16"):
@@ -844,9 +863,10 @@ def rows_of(t, cache: KvCache, heads: Optional[int] = None) -> Rows:
                 stride[2] if shape[2] > 1 else 0)
 
 
-def _ints(t, *shape) -> Optional[int]:
+def _ints(t, cache: KvCache, *shape) -> Optional[int]:
     if t is None:
         return None
+    _device_of(t, cache.device)
     if t.shape != shape or str(t.dtype) != "torch.int32" or not t.is_contiguous():
         raise OcrError(1, f"positions, counts, parents and paths are contiguous int32 device tensors, here {list(shape)}")
     return t.data_ptr()
@@ -855,52 +875,53 @@ def _ints(t, *shape) -> Optional[int]:
 def op_kv_write(ctx: Context, cache: KvCache, k, v, pos, n=None) -> None:
     """rows of keys and values [n_slot][rows][n_kv][d_head] → the cache, from position pos[slot] on (below 0: idle),
     n[slot] of them in use"""
-    c = cache.c
+    c = cache._on(ctx)
     if k.shape != v.shape:
         raise OcrError(1, "k and v must be of one shape")
     _check(lib().ocr_op_kv_write(ctx.h, c, rows_of(k, cache, c.n_kv),
-                                 rows_of(v, cache, c.n_kv), k.shape[1], _ints(pos, c.n_slot),
-                                 _ints(n, c.n_slot)))
+                                 rows_of(v, cache, c.n_kv), k.shape[1], _ints(pos, cache, c.n_slot),
+                                 _ints(n, cache, c.n_slot)))
 
 
 def op_kv_read(ctx: Context, cache: KvCache, k, v, pos, n=None) -> None:
     """the cache's rows → values in k and v; rows that are not in use are zeros"""
-    c = cache.c
+    c = cache._on(ctx)
     if k.shape != v.shape:
         raise OcrError(1, "k and v must be of one shape")
     _check(lib().ocr_op_kv_read(ctx.h, c, rows_of(k, cache, c.n_kv),
-                                rows_of(v, cache, c.n_kv), k.shape[1], _ints(pos, c.n_slot),
-                                _ints(n, c.n_slot)))
+                                rows_of(v, cache, c.n_kv), k.shape[1], _ints(pos, cache, c.n_slot),
+                                _ints(n, cache, c.n_slot)))
 
 
 def op_attention_window(ctx: Context, cache: KvCache, q, out, pos, scale: float, n=None) -> None:
     """rows q [n_slot][rows][n_head][d_head], which the cache already holds from pos[slot] on, attend it: causal, within
     the cache's window and sinks"""
-    c = cache.c
+    c = cache._on(ctx)
     if q.shape != out.shape:
         raise OcrError(1, "q and out must be of one shape")
     _check(lib().ocr_op_attention_window(ctx.h, c, rows_of(q, cache), q.shape[2], q.shape[1],
-                                         _ints(pos, c.n_slot), _ints(n, c.n_slot), scale, rows_of(out, cache)))
+                                         _ints(pos, cache, c.n_slot), _ints(n, cache, c.n_slot), scale, rows_of(out, cache)))
 
 
 def op_attention_tree(ctx: Context, cache: KvCache, q, out, pos, parent, scale: float, n=None) -> None:
     """the same for a tree of drafts: parent [n_slot][rows], parent[i] < i, -1 for a child of the last committed
     position"""
-    c = cache.c
+    c = cache._on(ctx)
     if q.shape != out.shape:
         raise OcrError(1, "q and out must be of one shape")
     _check(lib().ocr_op_attention_tree(ctx.h, c, rows_of(q, cache), q.shape[2], q.shape[1],
-                                       _ints(pos, c.n_slot), _ints(n, c.n_slot), _ints(parent, c.n_slot, q.shape[1]),
+                                       _ints(pos, cache, c.n_slot), _ints(n, cache, c.n_slot), _ints(parent, cache, c.n_slot, q.shape[1]),
                                        scale, rows_of(out, cache)))
 
 
 def op_kv_keep(ctx: Context, caches: Sequence[KvCache], pos, path, n) -> None:
     """the accepted drafts' rows move together in every layer's cache: position pos + path[i] → pos + i, i < n[slot]"""
-    c = caches[0].c
+    cache = caches[0]
+    c = cache.c
     rows = path.shape[1]
-    arr = (KvCacheC * len(caches))(*[x.c for x in caches])
-    _check(lib().ocr_op_kv_keep(ctx.h, arr, len(caches), rows, _ints(pos, c.n_slot), _ints(path, c.n_slot, rows),
-                                _ints(n, c.n_slot)))
+    arr = (KvCacheC * len(caches))(*[x._on(ctx) for x in caches])
+    _check(lib().ocr_op_kv_keep(ctx.h, arr, len(caches), rows, _ints(pos, cache, c.n_slot), _ints(path, cache, c.n_slot, rows),
+                                _ints(n, cache, c.n_slot)))
 
 
 def op_wait_probe(ctx: Context, tries: int) -> bool:
