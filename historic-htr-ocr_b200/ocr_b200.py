@@ -496,7 +496,7 @@ class Session:
         """a layer's KV rows, live, as an f16 cache for the op_kv_* and op_attention_* calls"""
         c = KvCacheC()
         _check(lib().ocr_session_kv_cache(self.h, layer, C.byref(c)))
-        return KvCache._of(c, (self,), self.model.ctx.device)
+        return KvCache._of(c, self)
 
     def prefill(self, slot: int = 0, ids: Optional[Sequence[int]] = None, embd: Optional[np.ndarray] = None,
                 logits: bool = True) -> Optional[np.ndarray]:
@@ -826,16 +826,18 @@ class KvCache:
             _device_of(x, self.device)
         self.c = KvCacheC(t, *lead[:2], d_head, lead[2], window, sinks, int(ring), _ptr(k), _ptr(v),
                           None if t == 1 else _ptr(k_scale), None if t == 1 else _ptr(v_scale))
-        self._keep = (k, v, k_scale, v_scale)
+        self._keep, self._session = (k, v, k_scale, v_scale), None
 
     @classmethod
-    def _of(cls, c: KvCacheC, keep: tuple, device: int) -> "KvCache":
+    def _of(cls, c: KvCacheC, session: "Session") -> "KvCache":
         v = cls.__new__(cls)
-        v.c, v._keep, v.device = c, keep, device
+        v.c, v._keep, v._session, v.device = c, (session,), session, session.model.ctx.device
         return v
 
     def _on(self, ctx: Context) -> KvCacheC:
         """the view for a call on ctx"""
+        if self._session is not None and not self._session.h:
+            raise OcrError(1, "the session whose rows this KV cache is has been closed")
         if self.device != ctx.device:
             raise OcrError(1, f"the KV cache is on GPU {self.device}, the context on GPU {ctx.device}")
         return self.c

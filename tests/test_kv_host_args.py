@@ -2,6 +2,8 @@
 address would go to the kernels. Needs no GPU: tensors that claim to be on one stand in for those that are right."""
 from __future__ import annotations
 
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -80,3 +82,17 @@ def test_a_cache_on_another_gpu_than_the_context_is_refused(ocr, op):
     call, args = calls(ocr, Ctx(), cache)[op]
     with pytest.raises(ocr.OcrError, match="the context on GPU 0"):
         call(**{k: Claims(v, 1) for k, v in args.items()})
+
+
+@pytest.mark.parametrize("op", range(5))
+def test_the_cache_of_a_closed_session_is_refused(ocr, op):
+    """its rows' memory went with the session"""
+    session = SimpleNamespace(h=1, model=SimpleNamespace(ctx=Ctx()))
+    cache = ocr.KvCache._of(ocr.KvCache("q8_0", *(Claims(x) for x in tensors())).c, session)
+    call, args = calls(ocr, Ctx(), cache)[op]
+    args = {k: Claims(v) for k, v in args.items()}
+    with pytest.raises(ocr.OcrError, match="null argument"):
+        call(**args)
+    session.h = None
+    with pytest.raises(ocr.OcrError, match="closed"):
+        call(**args)
