@@ -12,6 +12,7 @@ namespace ocr {
 
 constexpr int KV_F16 = 1, KV_Q4_0 = 2, KV_Q8_0 = 8;  // ocr_kv_cache.type (ggml's numbers)
 constexpr int KV_BLOCK = 32;                         // values that share a scale
+constexpr int KV_TICKETS = 4096;                     // bytes of the workspace before the partial results: a ticket per CTA
 constexpr int KV_TREE_MAX = 64;                      // drafts of one tree: an ancestor set is one 64-bit word
 
 __host__ __device__ constexpr int kv_row_bytes(int type, int d) {

@@ -9,7 +9,6 @@ namespace ocr {
 
 constexpr int KV_LINE = 4096;     // (slot, row block) pairs whose prefix sums a CTA holds (k_kv_attn_tc.cu)
 constexpr int KA_LINE = 256;      // slots of a launch of the attentions of few rows
-constexpr int KV_TICKETS = 4096;  // bytes of the workspace before the partial results: a ticket per CTA
 constexpr float LOG2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {

@@ -19,6 +19,7 @@
 #include "ctx.h"
 #include "gguf.h"
 #include "kernels.cuh"
+#include "kv.cuh"
 
 namespace ocr {
 
@@ -76,8 +77,9 @@ ocr_status check_device_error(ocr_ctx* ctx) {
     OCR_CUDA(cudaMemcpy(&err, ctx->d_err, sizeof(int), cudaMemcpyDeviceToHost));
     if (err != DEV_OK) {
         OCR_CUDA(cudaMemsetAsync(ctx->d_err, 0, sizeof(int), ctx->stream));  // (ordered before later kernels)
-        // a kernel that gave up may have left the KV attentions' tickets short
-        if (err == DEV_TIMEOUT && ctx->kv_work) OCR_CUDA(cudaMemsetAsync(ctx->kv_work, 0, 4096, ctx->stream));
+        // A kernel that gave up may have left the KV attentions' tickets short. (Whatever the code is: the flag keeps the
+        // first error, which may hide a wait that ran out later.)
+        if (ctx->kv_work) OCR_CUDA(cudaMemsetAsync(ctx->kv_work, 0, KV_TICKETS, ctx->stream));
         return fail(OCR_ERR_DEVICE, err == DEV_BAD_POS     ? "a kernel saw a position outside the KV cache"
                                     : err == DEV_TIMEOUT ? "a kernel's bounded wait ran out (its work was skipped)"
                                                          : "a kernel saw an index outside its buffer");

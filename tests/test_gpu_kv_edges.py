@@ -3,6 +3,8 @@ calls, the context's state after an error, the last rows of a cache, numbers far
 memory. Tolerances are those of test_gpu_kv.py unless a test derives its own."""
 from __future__ import annotations
 
+import ctypes as C
+
 import pytest
 import torch
 
@@ -85,3 +87,46 @@ def test_a_first_call_inside_a_capture_is_refused(ocr):
     del g
     ctx.close()
     maker.close()
+
+
+# ---- after an error ----
+class CtxHead(C.Structure):
+    """the first fields of the context (csrc/ctx.h)"""
+    _fields_ = [("refs", C.c_int), ("device", C.c_int), ("stream", C.c_void_p), ("num_sms", C.c_int), ("pdl", C.c_bool),
+                ("d_err", C.c_void_p), ("mem", C.c_uint64 * 3), ("op_scratch", C.c_void_p),
+                ("op_scratch_bytes", C.c_size_t), ("kv_work", C.c_void_p)]
+
+
+class Ints:
+    """device memory as torch.as_tensor takes it"""
+
+    def __init__(self, address, n):
+        self.__cuda_array_interface__ = dict(shape=(n,), typestr="<i4", data=(address, False), version=3)
+
+
+@pytest.mark.parametrize("T", [1, 8, 100])
+def test_tickets_are_set_back_after_any_error(ocr, T):
+    """A wait that runs out leaves tickets counted; the error flag keeps the first code, here a position's, so the code
+    alone does not tell. (The tickets are set by the test in the place of the wait.)"""
+    ctx = ocr.Context(0)
+    call, out, (cache, q, ps) = attend(ocr, ctx, T, keys=6000)  # (two pairs over many CTAs)
+    call()
+    ctx.sync()
+    want = out.clone()
+    head = C.cast(ctx.h, C.POINTER(CtxHead)).contents
+    assert head.device == 0 and head.stream == ctx.stream() and head.kv_work
+    tickets = torch.as_tensor(Ints(head.kv_work, 1024), device="cuda")
+    assert not tickets.any()
+    tickets.fill_(1)
+    torch.cuda.synchronize()
+    ocr.op_attention_window(ctx, cache, q, torch.zeros_like(q), i32([6001]), 0.09)
+    with pytest.raises(ocr.OcrError, match="position outside"):
+        ctx.sync()
+    ctx.sync()
+    assert not tickets.any()
+    out.zero_()
+    torch.cuda.synchronize()
+    call()
+    ctx.sync()
+    assert torch.equal(out, want)
+    ctx.close()
