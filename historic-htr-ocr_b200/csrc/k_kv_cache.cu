@@ -193,20 +193,25 @@ __global__ void __launch_bounds__(128) k_kv_keep(const __grid_constant__ KvKeepA
     const auto& L = a.layer[blockIdx.z];
     const int pos = a.pos[b], n = a.n[b];
     if (pos < 0 || n <= 0) return;
-    bool ok = n <= a.T && (c.ring ? (long)pos + a.T <= 0x7fffffffL : (long)pos + a.T <= (long)c.n_rows);
-    if (!ok) {
+    if (n > a.T) {
         if (tid == 0) dev_error(a.err, DEV_BAD_POS);
         return;
     }
-    bool bad = false;
+    // (of the step's rows only those that the path names have to lie in the cache: a slot may have used fewer than T)
+    bool bad = false, outside = false;
     if (tid < n) {
         const int p = a.path[(size_t)b * a.T + tid];
         bad = p < tid || p >= a.T || (tid > 0 && a.path[(size_t)b * a.T + tid - 1] >= p);
-        src[tid] = kv_row(c, pos + (bad ? tid : p));
-        dst[tid] = kv_row(c, pos + tid);
+        outside = !bad && (long)pos + p >= (c.ring ? 0x7fffffffL : (long)c.n_rows);
+        if (!bad && !outside) {
+            src[tid] = kv_row(c, pos + p);
+            dst[tid] = kv_row(c, pos + tid);
+        }
     }
-    if (__syncthreads_or(bad)) {
-        if (tid == 0) dev_error(a.err, DEV_BAD_INDEX);
+    bad = __syncthreads_or(bad);
+    outside = __syncthreads_or(outside);
+    if (bad || outside) {
+        if (tid == 0) dev_error(a.err, bad ? DEV_BAD_INDEX : DEV_BAD_POS);
         return;
     }
     const int rb = kv_row_bytes(c.type, c.d), pieces = rb / 16;

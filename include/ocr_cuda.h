@@ -359,7 +359,8 @@ ocr_status ocr_op_attention_tree(ocr_ctx* ctx, const ocr_kv_cache* c, const ocr_
                                  const ocr_rows* out);
 /* After the drafts are judged: the accepted path's rows move together. In each of n_layer caches of one shape (at most
  * 64), the row of position d_pos + d_path[i] becomes that of d_pos + i for i < d_n[slot]; d_path (device int32
- * [n_slot][rows]) rises strictly. The committed length is then d_pos + d_n. */
+ * [n_slot][rows]) rises strictly, and its rows lie in the cache (other rows of the step need not: a slot may have used
+ * fewer than `rows`). The committed length is then d_pos + d_n. */
 ocr_status ocr_op_kv_keep(ocr_ctx* ctx, const ocr_kv_cache* caches, int n_layer, int rows, const int32_t* d_pos,
                           const int32_t* d_path, const int32_t* d_n);
 

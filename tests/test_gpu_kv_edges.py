@@ -5,10 +5,12 @@ from __future__ import annotations
 
 import ctypes as C
 
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_kv import i32, make_cache
+import kv_plain as P
+from test_gpu_kv import TOL, TYPES, i32, make_cache, put, sequences, tree
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +132,69 @@ def test_tickets_are_set_back_after_any_error(ocr, T):
     ctx.sync()
     assert torch.equal(out, want)
     ctx.close()
+
+
+# ---- the last rows of a cache ----
+@pytest.mark.parametrize("T", [8, 40])
+@pytest.mark.parametrize("kind", TYPES)
+def test_a_ragged_step_at_the_end_of_the_cache(ocr, ctx, kind, T):
+    """trees of fewer drafts than the call's rows, the longest slot's last draft in the cache's last row: written,
+    attended, and the accepted rows moved"""
+    n_kv, d, n_rows = 2, 128, 100
+    pos, n = [n_rows - 5, 11, n_rows - T], [5, T, T]
+    paths = [[0, 2, 4], list(range(0, T, 2)), [1, T - 1]]
+    cache = make_cache(ocr, kind, 3, n_kv, n_rows, d)
+    k, v = sequences(31, 3, n_rows + T, n_kv, d)
+    put(ocr, ctx, cache, k[:, :n_rows], v[:, :n_rows], [0] * 3, n=pos)
+    parents = [tree(7 + b, T) for b in range(3)]
+    kd, vd = (torch.from_numpy(np.stack([x[b, pos[b]:pos[b] + T] for b in range(3)])).cuda() for x in (k, v))
+    q = torch.from_numpy(np.random.default_rng(5).standard_normal((3, T, 4, d), dtype=np.float32)).cuda()
+    out, ps, ns, par = torch.zeros_like(q), i32(pos), i32(n), i32(parents)
+    torch.cuda.synchronize()
+    ocr.op_kv_write(ctx, cache, kd, vd, ps, ns)
+    ocr.op_attention_tree(ctx, cache, q, out, ps, par, 0.09, ns)
+    ctx.sync()
+    for b in range(3):
+        m = n[b]
+        kb, vb = (torch.from_numpy(P.held(x[b, :pos[b] + m], kind)).double().transpose(0, 1) for x in (k, v))
+        want = P.attend(q[b, :m].double().cpu(), kb, vb, pos[b], 0.09, parent=parents[b][:m])
+        assert float((out[b, :m].double().cpu() - want).abs().max() / vb.abs().max()) <= TOL["f32"]
+    was = [t.clone() for t in cache._keep if t is not None]
+    path, kept = i32([p + [0] * (T - len(p)) for p in paths]), i32([len(p) for p in paths])
+    torch.cuda.synchronize()
+    ocr.op_kv_keep(ctx, [cache], ps, path, kept)
+    ctx.sync()
+    for now, old in zip([t for t in cache._keep if t is not None], was):
+        want = old.clone()
+        for b in range(3):
+            for i, j in enumerate(paths[b]):
+                want[b, :, pos[b] + i] = old[b, :, pos[b] + j]
+        assert torch.equal(now, want)
+
+
+@pytest.mark.parametrize("ring", [False, True])
+def test_a_path_past_the_end_is_flagged(ocr, ctx, ring):
+    """the slot concerned is left alone, the other served"""
+    end = 0x7fffffff if ring else 50
+    cache = make_cache(ocr, "q8_0", 2, 1, 50, 64, **(dict(window=20, sinks=2, ring=True) if ring else {}))
+    for t in cache._keep:
+        t.copy_(torch.arange(t.numel(), device="cuda").view(t.shape) % 100)
+    was = [t.clone() for t in cache._keep]
+    path, kept, ps = i32([[0, 3, 6, 0, 0, 0, 0, 0], [1, 2, 0, 0, 0, 0, 0, 0]]), i32([3, 2]), i32([end - 6, 5])
+    torch.cuda.synchronize()
+    ocr.op_kv_keep(ctx, [cache], ps, path, kept)
+    with pytest.raises(ocr.OcrError, match="position outside"):
+        ctx.sync()
+    ps2 = i32([end - 7, -1])
+    torch.cuda.synchronize()
+    for t, old in zip(cache._keep, was):
+        assert torch.equal(t[0], old[0]) and torch.equal(t[1, :, 5:7], old[1, :, 6:8])
+    ocr.op_kv_keep(ctx, [cache], ps2, path, kept)  # (a position less: its last row is the cache's last)
+    ctx.sync()
+
+    def row(p):
+        return P.row_of(p, 50, 2, ring)
+
+    for t, old in zip(cache._keep, was):
+        for i, j in enumerate((0, 3, 6)):
+            assert torch.equal(t[0, :, row(end - 7 + i)], old[0, :, row(end - 7 + j)])
