@@ -40,10 +40,11 @@ ocr_status check_rows(const ocr_rows* r, const char* name) {
     return OCR_OK;
 }
 
-ocr_status check_call(const ocr_kv_cache* c, int rows, const int32_t* d_pos) {
+// (read: rows that the cache holds, which overwrites none)
+ocr_status check_call(const ocr_kv_cache* c, int rows, const int32_t* d_pos, bool read = false) {
     if (!d_pos) return fail(OCR_ERR_ARG, "null argument");
     if (rows < 1) return fail(OCR_ERR_ARG, "rows must be at least 1");
-    if (c->ring ? rows > c->n_rows - c->sinks - c->window + 1 : rows > c->n_rows)
+    if (c->ring && !read ? rows > c->n_rows - c->sinks - c->window + 1 : rows > c->n_rows)
         return fail(OCR_ERR_ARG, "rows: more than the cache takes in one call");
     return OCR_OK;
 }
@@ -62,7 +63,7 @@ ocr_status move(ocr_ctx* ctx, const ocr_kv_cache* c, const ocr_rows* k, const oc
     OCR_TRY(check_rows(k, "k"));
     OCR_TRY(check_rows(v, "v"));
     if (!k->half != !v->half) return fail(OCR_ERR_ARG, "k and v must be of one type");
-    OCR_TRY(check_call(c, rows, d_pos));
+    OCR_TRY(check_call(c, rows, d_pos, !write));
     if ((double)rows * c->n_kv * (c->d_head / KV_BLOCK) * 8 > 4294967295.0)  // (the kernel counts a slot's threads in 32 bits)
         return fail(OCR_ERR_ARG, "rows: more than one launch takes");
     OCR_CUDA(cudaSetDevice(ctx->device));

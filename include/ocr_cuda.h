@@ -334,14 +334,16 @@ ocr_status ocr_session_kv_cache(const ocr_session* s, int layer, ocr_kv_cache* o
 /* Every call below takes `rows` rows of each slot, from position d_pos[slot] on (device int32 [n_slot]; below 0: the
  * slot is idle), d_n[slot] of them in use (device int32 [n_slot]; null: all). Rows that are not in use are not written
  * to the cache, and are zeros in an output. A slot whose rows do not fit the cache is flagged and treated as idle. In
- * a ring cache rows is at most n_rows - sinks - window + 1: more would overwrite what the first of them sees. */
+ * a ring cache rows is at most n_rows - sinks - window + 1: more would overwrite what the first of them sees (a read
+ * takes up to n_rows). */
 /* rows of keys and values → the cache, quantised per block of 32 as ggml's reference quantisers do: q8_0 with
  * scale = f16(max|x| / 127) and q = x / scale before its rounding to f16, to the nearest, halves away from zero; q4_0
  * with scale = f16(m / -8), m the first value of the largest magnitude. A block with an infinity or a NaN, or whose
  * scale passes f16's range, reads back as NaN. */
 ocr_status ocr_op_kv_write(ocr_ctx* ctx, const ocr_kv_cache* c, const ocr_rows* k, const ocr_rows* v, int rows,
                            const int32_t* d_pos, const int32_t* d_n);
-/* the cache's rows → values */
+/* the cache's rows → values. Of a ring cache the rows as they are now: those of a position that has left it hold a later
+ * one, which the cache does not know */
 ocr_status ocr_op_kv_read(ocr_ctx* ctx, const ocr_kv_cache* c, const ocr_rows* k, const ocr_rows* v, int rows,
                           const int32_t* d_pos, const int32_t* d_n);
 /* softmax(q k^T * scale) v of the rows, which the cache already holds, over the positions each sees: up to its own,

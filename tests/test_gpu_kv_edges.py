@@ -198,3 +198,25 @@ def test_a_path_past_the_end_is_flagged(ocr, ctx, ring):
     for t, old in zip(cache._keep, was):
         for i, j in enumerate((0, 3, 6)):
             assert torch.equal(t[0, :, row(end - 7 + i)], old[0, :, row(end - 7 + j)])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_a_tight_ring_is_read_at_once(ocr, ctx, kind):
+    """n_rows = sinks + window takes one row a call; a read overwrites nothing and takes all that it holds"""
+    n_kv, d, window, sinks, total = 2, 64, 24, 3, 70
+    cache = make_cache(ocr, kind, 1, n_kv, window + sinks, d, window=window, sinks=sinks, ring=True)
+    k, v = sequences(12, 1, total, n_kv, d)
+    put(ocr, ctx, cache, k, v, [0], chunk=1)
+    for first, m in ((total - window, window), (0, sinks)):
+        back = [torch.zeros(1, m, n_kv, d, device="cuda") for _ in "kv"]
+        ps = i32([first])
+        torch.cuda.synchronize()
+        ocr.op_kv_read(ctx, cache, *back, ps)
+        ctx.sync()
+        for x, got in zip((k, v), back):
+            np.testing.assert_array_equal(got.cpu().numpy(), P.held(x[:, first:first + m], kind))
+    many = torch.zeros(1, window + sinks + 1, n_kv, d, device="cuda")
+    with pytest.raises(ocr.OcrError, match="more than the cache"):
+        ocr.op_kv_read(ctx, cache, many, many, ps)
+    with pytest.raises(ocr.OcrError, match="more than the cache"):
+        ocr.op_kv_write(ctx, cache, back[0][:, :2], back[1][:, :2], ps)
