@@ -925,8 +925,18 @@ static cudaError_t launch_type(cudaStream_t st, const KvAttnArgs& a, int blocks,
 size_t kv_attention_many_work(int num_sms) { return KV_TICKETS + (size_t)num_sms * 2 * ((128 + 2) + 128) * KC_M * 4; }
 // (row, query head) pairs of a kv head in one slot that one call takes
 long kv_attention_many_rows() { return (long)KV_LINE * KC_M; }
+static int blocks_of(const KvAttnArgs& a) { return (int)(((long)a.r.T * (a.n_head / a.c.n_kv) + KC_M - 1) / KC_M); }
+// slots of one launch: their (slot, row block) pairs have places in the line, and its tiles are counted in 32 bits (0: not
+// even one slot's)
+int kv_attention_many_slots(const KvAttnArgs& a) {
+    const KvView& c = a.c;
+    const long keys = c.window ? min((long)c.n_rows, (long)c.window + c.sinks + a.r.T) : c.n_rows;
+    const int blocks = blocks_of(a);
+    const long tiles = (keys + KC_KEYS - 1) / KC_KEYS * c.n_kv * blocks;
+    return (int)min((long)(KV_LINE / blocks), 0x7fffffffL / tiles);
+}
 cudaError_t launch_kv_attention_many(cudaStream_t st, const KvAttnArgs& all, bool pdl) {
-    const int blocks = (int)(((long)all.r.T * (all.n_head / all.c.n_kv) + KC_M - 1) / KC_M), slots = KV_LINE / blocks;
+    const int blocks = blocks_of(all), slots = kv_attention_many_slots(all);
     for (int b = 0; b < all.c.n_slot; b += slots) {
         const KvAttnArgs a = kv_slots(all, b, min(slots, all.c.n_slot - b));
         const cudaError_t e = a.c.type == KV_F16    ? launch_type<KV_F16>(st, a, blocks, pdl)

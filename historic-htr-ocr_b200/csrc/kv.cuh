@@ -122,6 +122,7 @@ size_t kv_attention_few_work(int num_sms);
 size_t kv_attention_many_work(int num_sms);
 size_t kv_attention_work_bytes(int num_sms);
 long kv_attention_many_rows();
+int kv_attention_many_slots(const KvAttnArgs& a);
 
 // a launch that may start while its predecessor on the stream still runs: the kernel calls pdl_wait() before it
 // touches memory

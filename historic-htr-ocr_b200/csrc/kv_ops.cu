@@ -105,11 +105,12 @@ ocr_status attend(ocr_ctx* ctx, const ocr_kv_cache* c, const ocr_rows* q, int n_
     if (!(scale > 0.0f && scale <= 3.4e38f)) return fail(OCR_ERR_ARG, "scale must be positive and finite");
     if ((double)c->n_slot * rows * n_head > 1e9 || (double)rows * (n_head / c->n_kv) > (double)kv_attention_many_rows())
         return fail(OCR_ERR_ARG, "rows: more than one launch takes");
-    OCR_CUDA(cudaSetDevice(ctx->device));
     KvAttnArgs a{view(c),        {d_pos, d_n, rows}, d_parent,         q->data,         out->data,
                  q->half ? 1 : 0, n_head,            q->slot_stride,   q->row_stride,   q->head_stride,
                  out->slot_stride, out->row_stride,  out->head_stride, scale,           nullptr,
                  ctx->num_sms,     ctx->d_err};
+    if (kv_attention_many_slots(a) < 1) return fail(OCR_ERR_ARG, "rows: more than one launch takes");
+    OCR_CUDA(cudaSetDevice(ctx->device));
     OCR_TRY(ensure_kv_work(ctx));
     a.work = ctx->kv_work;
     return launched(launch_kv_attention(ctx->stream, a, ctx->pdl), what);

@@ -220,3 +220,16 @@ def test_a_tight_ring_is_read_at_once(ocr, ctx, kind):
         ocr.op_kv_read(ctx, cache, many, many, ps)
     with pytest.raises(ocr.OcrError, match="more than the cache"):
         ocr.op_kv_write(ctx, cache, back[0][:, :2], back[1][:, :2], ps)
+
+
+def test_more_tiles_than_32_bits_count_are_refused(ocr, ctx):
+    """4096 row blocks x 1000 kv heads x 525 key blocks of one slot are more than 2^31. The rows are one vector, seen
+    from everywhere."""
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("not enough memory")
+    x = torch.zeros(1, 1, 1, 64, dtype=torch.float16, device="cuda")
+    q, ps = x.expand(1, 65536, 8000, 64), i32([0])
+    cache = make_cache(ocr, "q4_0", 1, 1000, 67200, 64)
+    with pytest.raises(ocr.OcrError, match="more than one launch"):
+        ocr.op_attention_window(ctx, cache, q, q, ps, 0.1)
+    ctx.sync()
