@@ -6,15 +6,17 @@
 // is the chain S → P → O of one triple (one fits an SM) with the softmax's instructions and the issuing thread's waits in it:
 // before the products were issued by an elected thread (307, 72 and 234 us below) the tensor pipe was 16 to 20 % busy, issue
 // 32 to 42 %. Measured: 512 f16 rows by 16896 f16 keys, 16 heads of 64, four slots: 273 us, 386 TFLOP/s; 2214 f32 rows
-// in a window of 512, q8_0, 16 heads of 128: 63 us; 8 trees of 61 drafts in windows of 8192, q4_0, f16 rows, 32 heads: 211 us.
+// in a window of 512, q8_0, 16 heads of 128: 66 us; 8 trees of 61 drafts in windows of 8192, q4_0, f16 rows, 32 heads: 218 us.
 //
 // Products: S = Q K^T (M = N = 128, both operands in shared memory), O += P V (A = P in TMEM, written over S in place;
 // B = V in shared memory, MN-major), f16 operands, f32 sums in TMEM. Exactness: f32 queries and P are f16 hi + lo (22 bits);
 // f16 queries are exact, and P is rounded to f16 as the output is. f16 keys and values are exact; a quantised value
-// q d (at most 19 bits) splits exactly into f16 hi + lo, so S = Q_hi K_hi + Q_lo K_hi + Q_hi K_lo, and P V alike, carry
-// the f32 product to 2^-22. A row's query is scaled by a power of two (its lo part stays in f16's range), a tile's
-// scales by a power of two 2^-e, e from the tile's largest: S takes 2^e back with the row's factor; for V the score
-// itself takes e as an addend, so that P carries 2^e and the row's reference bounds both.
+// q d (at most 19 bits) splits into f16 hi + lo, so S = Q_hi K_hi + Q_lo K_hi + Q_hi K_lo, and P V alike, carry the f32
+// product to 2^-22. A row's query is scaled by a power of two (its lo part stays in f16's range); so are the scales d, as
+// far up as the products q d fit f16: the split is exact for scales down to 2^-21 (q8_0) or 2^-25 (q4_0) of the largest that
+// shares their exponent, and what is smaller is off by 2^-32 of the largest value. K has one exponent, which S takes back
+// with the row's factor; V has one for each block of 32 dims and O stands in their units, so an output's accuracy is that
+// of its own block (with one exponent for a tile, blocks 2^20 below another had errors of percents).
 //
 // Softmax: online. Two warpgroups take 64 keys of every tile each, with sums, reference and O of their own (joined at the
 // end). S has two places: the next tile's Q K^T runs while the groups turn this tile's S into P, so a group goes from
@@ -48,6 +50,7 @@ constexpr int KC_RING = 4;  // tiles whose exponents and scales are kept
 constexpr int KC_MARKS = 8;  // tiles whose marks are kept: looked at two tiles later
 constexpr int KC_PIECE = 10;
 constexpr float KC_LAG = 6.0f, KC_BIAS = 8.0f;
+constexpr int KC_EXP = 15;  // what an exponent has added to it in a byte (f16's own bias; its subnormals count as 2^-15)
 
 template <int BYTES>
 struct KcWord;
@@ -71,6 +74,8 @@ struct KcPlan {
     static constexpr int PARTS = QN ? 2 : 1;                                      // hi (and lo) of K and V
     static constexpr int NS = QN && D == 128 ? 1 : 2;                             // stages
     static constexpr uint32_t SMEM = (LO ? 2 : 1) * Q_BYTES + 2 * NS * PARTS * T_BYTES + 1024;
+    // a block's quants times its scale d (below 2^(e + 1)) times 2^(HEAD - e) just fit f16
+    static constexpr int HEAD = TYPE == KV_Q8_0 ? 8 : 12;
     // f32 rows: tiles between two moves of O, at most 64 products added to each of its sums in between
     static constexpr int FLUSH = QN ? 5 : 8;
     // the joined parts: [D][128] sums, [128] references, [128] weights' sums
@@ -90,9 +95,10 @@ struct KcShared {
     int prefix[KV_LINE + 1], wsum[KC_THREADS / 32];
     float fac[KC_M];             // the rows' factors on S
     float ml[2][3][KC_M];        // the groups' references, sums, and factors on their sums in memory
-    int ex[KC_RING][2];          // the tiles' exponents of K and V
+    float exk[KC_RING];          // the tiles' factors on S: 2^(e - HEAD) of K's scales
+    uint32_t exv[KC_RING];       // the exponents of V's blocks as of these tiles, a byte each
     uint32_t bad[KC_MARKS][4];   // keys of an edge tile whose values are not all finite
-    __align__(8) uint32_t top[KC_RING][2];  // the largest scales of a tile's K and V (f16 bits)
+    uint32_t top[2][NB + 1];     // the largest exponents of a tile's scales, V's blocks' and K's: two in turn
     __align__(8) __half scale[KC_RING][2][KC_KEYS][NB];
     int parent[KV_TREE_MAX], depth[KV_TREE_MAX];
 };
@@ -132,14 +138,27 @@ __device__ __forceinline__ uint32_t h2rest(uint32_t a, uint32_t b, uint32_t c) {
                               *reinterpret_cast<const __half2*>(&n));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t h2max(uint32_t a, uint32_t b) {
-    const __half2 r = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
 __device__ __forceinline__ bool h2_not_finite(uint32_t w) {
     return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
 }
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+// the exponent fields of a pair of f16 (bits 0 … 4 and 16 … 20), 0 for what is not finite
+__device__ __forceinline__ uint32_t h2exps(uint32_t w) {
+    w &= 0x7fff7fffu;
+    return (w & __vcmpltu2(w, 0x7c007c00u)) >> 10 & 0x001f001fu;
+}
+// four exponents in a word, block b's in the byte where h2exps leaves it: 0, 2, 1, 3
+__device__ __forceinline__ constexpr int exp_shift(int b) { return 8 * ((b >> 1) | (b & 1) << 1); }
+__device__ __forceinline__ int exp_of(uint32_t bytes, int b) { return (int)((bytes >> exp_shift(b)) & 255u) - KC_EXP; }
+// whether any of the `threads` threads at barrier `id` says so
+__device__ __forceinline__ bool bar_any(int id, int threads, bool mine) {
+    uint32_t any;
+    asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbar.red.or.pred q, %2, %3, p;\nselp.u32 %0, 1, 0, q;\n}"
+                 : "=r"(any)
+                 : "r"((uint32_t)mine), "r"(id), "r"(threads)
+                 : "memory");
+    return any != 0;
+}
 
 // ---- the staging of a tile, by 256 threads: raw rows to registers, later to operands ------------------------------------
 // K and V alike: rows of 64 dims (128 bytes, swizzled) in D / 64 halves of 128 keys — K is read along the dims (K-major),
@@ -206,12 +225,13 @@ struct KcRaw {
             }
         }
     }
-    // The operands, values times 2^-e. `bad` (an edge tile's V): what is not finite becomes zero and its key is marked.
-    __device__ static __forceinline__ void store(const uint4* x, uint8_t* hi, uint8_t* lo, const __half* scale, int e,
+    // The operands, the values of block b times 2^(HEAD - e), e byte b of `exps`. `bad` (an edge tile's V): what is not
+    // finite becomes zero and its key is marked.
+    __device__ static __forceinline__ void store(const uint4* x, uint8_t* hi, uint8_t* lo, const __half* scale, uint32_t exps,
                                                  uint32_t* bad, int lw, int lane) {
-        const float down = exp2i(-e);
         int key0, u;
         place(lw, lane, key0, u);
+        [[maybe_unused]] const float down = exp2i((TYPE == KV_Q8_0 ? 8 : 12) - exp_of(exps, TYPE == KV_Q8_0 ? u >> 1 : u));
 #pragma unroll
         for (int i = 0; i < KU; i++) {
             const int key = key0 + i * STEP;
@@ -288,10 +308,8 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
             mbar_init(&sh.pfull[i], 8);
             mbar_init(&sh.odone[i], 1);
         }
-        for (int i = 0; i < KC_RING; i++) {
-            mbar_init(&sh.xfull[i], 1);
-            sh.top[i][0] = sh.top[i][1] = 0u;
-        }
+        for (int i = 0; i < KC_RING; i++) mbar_init(&sh.xfull[i], 1);
+        for (int j = 0; j <= (P::QN ? P::NB : 1); j++) sh.top[0][j] = sh.top[1][j] = 0u;
         mbar_init(&sh.mdone, 1);
         mbar_init(&sh.qfull, 8);
         sh.abort_flag = 0;
@@ -410,6 +428,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
         }
         typename Raw::Tile tv;             // of the V tile to load next: K's of the tile before
         bool next_edge = false, edge = false;
+        uint32_t vexp = 0u, kexp = 0u, tops = 0u;  // the exponents in the triple so far: V's blocks', K's; times they moved
         int plain = 0;                     // tiles that follow at 128 rows' distance, whole and seen by every row
         auto load_k = [&](int n) {         // tile n's K and scales; its place is V's next
             if (plain > 0) {
@@ -443,50 +462,71 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 raw.load(raw.v, c.v, c, x.sp, x.base, t, lw, lane);
             }
         };
-        auto put_k = [&](int n) {  // → the exponent of V's tile
+        // The exponents that the operands are scaled by: one for K (S takes it back with the row's factor), one for each
+        // block of 32 dims of V (O is in their units). They stay from tile to tile until a scale passes one, or a triple
+        // begins; they are then a power of two above the largest, so that they seldom move.
+        auto put_k = [&](int n) {  // → the exponents of V's tile
             const int st = n % NS, x = n % KC_RING;
-            int eK = 0, eV = 0;
             if (lt < 4) sh.bad[n % KC_MARKS][lt] = 0u;
+            uint32_t kf = 0u, vf = 0u;  // a key's largest exponent of K, those of V's blocks
             if (P::QN && lt < KC_KEYS) {
 #pragma unroll
-                for (int y = 0; y < 2; y++) {
-                    uint32_t big = 0u;
-#pragma unroll
-                    for (int j = 0; j < P::NB / 2; j++) {
-                        big = h2max(big, raw.ex[y][j] & 0x7fff7fffu);
-                        reinterpret_cast<uint32_t*>(sh.scale[x][y][lt])[j] = raw.ex[y][j];
-                    }
-                    big = __reduce_max_sync(FULL, max(big & 0xffffu, big >> 16));
-                    if (lane == 0) atomicMax(&sh.top[x][y], big);
+                for (int j = 0; j < P::NB / 2; j++) {
+                    reinterpret_cast<uint32_t*>(sh.scale[x][0][lt])[j] = raw.ex[0][j];
+                    reinterpret_cast<uint32_t*>(sh.scale[x][1][lt])[j] = raw.ex[1][j];
+                    kf = __vmaxu2(kf, h2exps(raw.ex[0][j]));
+                    vf |= h2exps(raw.ex[1][j]) << (8 * j);
                 }
-                if (lt < 2) sh.top[(x + 2) % KC_RING][lt] = 0u;  // (tile n - 2's, read by all before the last barrier)
+                kf = max(kf & 0xffffu, kf >> 16);
             }
-            bar_sync(2, KC_LOADERS * 32);
             if constexpr (P::QN) {
-                auto exponent = [&](uint32_t bits) {
-                    const float f = __half2float(__ushort_as_half((unsigned short)bits));
-                    return f > 0.0f ? min(16, (int)(__float_as_uint(f) >> 23) - 127) : 0;
-                };
-                const uint2 top = *reinterpret_cast<const uint2*>(sh.top[x]);
-                eK = exponent(top.x), eV = exponent(top.y);
+                const bool first = n == 0 || begin + n == kc.first;
+                // (bytes below 128: a byte of the difference keeps its top bit unless the exponent is passed)
+                const bool pass = first || kf > kexp || (((vexp | 0x80808080u) - vf) & 0x80808080u) != 0x80808080u;
+                if (bar_any(2, KC_LOADERS * 32, pass)) {
+                    uint32_t* top = sh.top[tops & 1];
+                    if (lt < KC_KEYS) {
+                        const uint32_t k = __reduce_max_sync(FULL, kf);
+                        if (lane == 0) atomicMax(&top[P::NB], k);
+#pragma unroll
+                        for (int j = 0; j < P::NB; j++) {
+                            const uint32_t v = __reduce_max_sync(FULL, vf >> exp_shift(j) & 255u);
+                            if (lane == 0) atomicMax(&top[j], v);
+                        }
+                    }
+                    if (lt <= P::NB) sh.top[~tops & 1][lt] = 0u;  // (read before this tile's barrier)
+                    bar_sync(2, KC_LOADERS * 32);
+                    if (first || top[P::NB] > kexp) kexp = top[P::NB] + 1;
+                    uint32_t now = 0u;
+#pragma unroll
+                    for (int j = 0; j < P::NB; j++) {
+                        const uint32_t was = vexp >> exp_shift(j) & 255u;
+                        now |= (first || top[j] > was ? top[j] + 1 : was) << exp_shift(j);
+                    }
+                    vexp = now;
+                    tops++;
+                }
                 if (lt == 0) {
-                    sh.ex[x][0] = eK, sh.ex[x][1] = eV;
+                    sh.exk[x] = exp2i((int)kexp - KC_EXP - P::HEAD), sh.exv[x] = vexp;
                     mbar_arrive(&sh.xfull[x]);
                 }
+            } else {
+                bar_sync(2, KC_LOADERS * 32);
             }
             ok = ok && (n < NS || kc_wait(&sh.kempty[st], (n / NS - 1) & 1, abort_flag, err));
             uint8_t* kh = Kr + st * P::PARTS * P::T_BYTES;
-            if (ok) Raw::store(raw.k, kh, kh + P::T_BYTES, sh.scale[x][0][0], eK, nullptr, lw, lane);
+            if (ok) Raw::store(raw.k, kh, kh + P::T_BYTES, sh.scale[x][0][0], kexp * 0x01010101u, nullptr, lw, lane);
             fence_proxy_async();
             __syncwarp();
             if (ok && lane == 0) mbar_arrive(&sh.kfull[st]);
-            return eV;
+            return vexp;
         };
-        int eV = 0;
+        uint32_t eV = 0u;
         // (from -2: one copy of each step's code — the instruction cache is short of room)
 #pragma unroll 1
         for (int n = -2; n < tiles; n++) {
-            const int st = n % NS, x = n % KC_RING, e = eV;
+            const int st = n % NS, x = n % KC_RING;
+            const uint32_t e = eV;
             const typename Raw::Tile t1 = tv;  // of tile n + 1
             const bool e1 = next_edge;
             const bool next = n + 1 >= 0 && n + 1 < tiles;
@@ -660,6 +700,9 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 sight.rows(c, sp, sp.pos + row, sp.pos + row);
             const float fac0 = sh.fac[r];
             float m = -INFINITY, l = 0.0f;
+            uint32_t vexp = 0u;  // the exponents of the blocks of O
+            // block b's factor from O's unit
+            auto unit = [&](int b) { return P::QN ? exp2i(exp_of(vexp, b) - P::HEAD) : 1.0f; };
             // the group's sums in memory, [D][128]: their reference
             float m_kept = -INFINITY;
             float* kept = reinterpret_cast<float*>(static_cast<uint8_t*>(a.work) + KV_TICKETS) +
@@ -680,11 +723,12 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 const int n = n0 + i, x = n % KC_RING, v0 = (seg - cc.first + i) * KC_KEYS;
                 const uint32_t tS = tmem + lanes + (n & 1) * KC_KEYS + wg * HALF;
                 const bool edge = plain.edge(v0);
-                float fac = fac0, ev = 0.0f;
+                float fac = fac0;
+                uint32_t ve = 0u;
                 if constexpr (P::QN) {
                     if (!kc_wait_warp(&sh.xfull[x], (n / KC_RING) & 1, abort_flag, err)) return false;
-                    fac *= exp2i(sh.ex[x][0]);
-                    ev = (float)sh.ex[x][1];
+                    fac *= sh.exk[x];
+                    ve = sh.exv[x];
                 }
                 if (!kc_wait_warp(&sh.sfull[n & 1], (n >> 1) & 1, abort_flag, err)) return false;
                 tc_fence_after();
@@ -705,7 +749,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int j = 0; j < HALF; j++) mq[j & 3] = fmaxf(mq[j & 3], __uint_as_float(s[j]));
-                const float mt = fmaf(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])), fac, ev);
+                const float mt = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) * fac;
                 const bool flush = P::LO && i > 0 && i % P::FLUSH == 0;
                 const float m_was = m;
                 if (i == 0) {
@@ -713,8 +757,9 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 } else if (flush) {  // (O starts afresh)
                     m = fmaxf(m, mt);
                     if (m_was != -INFINITY) l *= ex2(m_was - m);
-                } else if (__any_sync(FULL, mt > m + KC_LAG)) {
-                    // (warp-uniform: TMEM loads and stores are the whole warp's; a row that stays scales by 1)
+                } else if (__any_sync(FULL, mt > m + KC_LAG || (P::QN && ve != vexp))) {
+                    // (the reference moves, or a block's exponent did. Warp-uniform: TMEM loads and stores are the whole
+                    // warp's; a row that stays scales by 1)
                     if (!kc_wait_warp(&sh.odone[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, err)) return false;
                     tc_fence_after();
                     const bool up = mt > m + KC_LAG;
@@ -722,16 +767,17 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
 #pragma unroll 1
                     for (int d = 0; d < D; d += 16) {
                         uint32_t o[16];
+                        const float g = P::QN ? f * exp2i(exp_of(vexp, d >> 5) - exp_of(ve, d >> 5)) : f;
                         tmem_ld16(tO + d, o);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                        for (int j = 0; j < 16; j++) o[j] = __float_as_uint(__uint_as_float(o[j]) * g);
                         tmem_st16(tO + d, o);
                     }
                     l *= f;
                     if (up) m = mt;
                 }
-                const float ref = ev + KC_BIAS - (m == -INFINITY ? 0.0f : m);
+                const float ref = KC_BIAS - (m == -INFINITY ? 0.0f : m);
                 float sum[2] = {0.0f, 0.0f};
 #pragma unroll
                 for (int ch = 0; ch < 2; ch++) {
@@ -747,7 +793,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                     tmem_st16(tS + 32 * ch, h);
                     if constexpr (P::LO) tmem_st16(tS + 32 * ch + 16, lo);
                 }
-                l = fmaf(sum[0] + sum[1], exp2i(P::QN ? -(int)ev : 0), l);
+                l += sum[0] + sum[1];
                 tmem_wait_st();
                 if (flush) {
                     if (!kc_wait_warp(&sh.odone[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag, err)) return false;
@@ -758,15 +804,17 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                     for (int d = 0; d < D; d += 32) {
                         uint32_t o[32];
                         float k[32];
+                        const float g = unit(d >> 5);
                         tmem_ld32(tO + d, o);
 #pragma unroll
                         for (int j = 0; j < 32; j++) k[j] = more ? __ldcg(&kept[(d + j) * KC_M]) : 0.0f;
                         tmem_wait_ld();
 #pragma unroll
-                        for (int j = 0; j < 32; j++) __stcg(&kept[(d + j) * KC_M], fmaf(k[j], f, __uint_as_float(o[j])));
+                        for (int j = 0; j < 32; j++) __stcg(&kept[(d + j) * KC_M], fmaf(k[j], f, __uint_as_float(o[j]) * g));
                     }
                     m_kept = m_was;
                 }
+                vexp = ve;
                 return true;
             };
             for (int i = 0; i < N; i++) {
@@ -817,6 +865,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
 #pragma unroll 1
                 for (int d = wg * (D / 2); d < (wg + 1) * (D / 2); d += 16) {
                     uint32_t o[16], o2[16];
+                    const float oa = fa * unit(d >> 5), ob = fb * unit(d >> 5);
                     tmem_ld16(tmem + lanes + 256 + d, o);
                     tmem_ld16(tmem + lanes + 384 + d, o2);
                     float y[16] = {};
@@ -828,7 +877,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                     }
                     tmem_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 16; j++) y[j] = fmaf(__uint_as_float(o2[j]), fb, fmaf(__uint_as_float(o[j]), fa, y[j]));
+                    for (int j = 0; j < 16; j++) y[j] = fmaf(__uint_as_float(o2[j]), ob, fmaf(__uint_as_float(o[j]), oa, y[j]));
                     if (whole) {
 #pragma unroll
                         for (int j = 0; j < 16; j++) y[j] = lt == 0.0f ? 0.0f : y[j] * inv;

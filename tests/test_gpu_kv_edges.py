@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import kv_plain as P
-from test_gpu_kv import TOL, TYPES, i32, make_cache, put, sequences, tree
+from test_gpu_kv import TOL, TYPES, case, i32, make_cache, put, sequences, tree
 
 pytestmark = pytest.mark.gpu
 
@@ -233,3 +233,50 @@ def test_more_tiles_than_32_bits_count_are_refused(ocr, ctx):
     with pytest.raises(ocr.OcrError, match="more than one launch"):
         ocr.op_attention_window(ctx, cache, q, q, ps, 0.1)
     ctx.sync()
+
+
+# ---- numbers far apart ----
+def by_block(got, want, v, kind):
+    """the largest error in each block of 32 dims, in units of the block's largest |value|"""
+    top = np.abs(P.held(v, kind)).reshape(-1, v.shape[-1] // 32, 32).max((0, 2))
+    err = (got - want).abs().reshape(-1, v.shape[-1] // 32, 32).amax((0, 2)).numpy()
+    return err / top
+
+
+@pytest.mark.parametrize("T", [1, 8, 130, 700])  # whole numbers, warp-level products, tcgen05 in parts and whole
+@pytest.mark.parametrize("item", ["f32", "f16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kind", TYPES)
+def test_values_whose_blocks_differ_along_d(ocr, ctx, kind, d, item, T):
+    """blocks of 32 dims 2^20 apart in size: an output's error is bounded by its own block's values (the weights' errors
+    are the same for every dim), not by the largest block's"""
+    held = {}
+
+    def change(k, v):
+        v *= np.exp2(np.repeat(np.linspace(-9, 11, d // 32), 32)).astype(np.float32)
+        if item == "f16":
+            v[:] = v.astype(np.float16)
+        held["v"] = v
+
+    call, want, _ = case(ocr, ctx, kind, item, (1, 2, 2, d, T, [900], 0, 0, False, False), change=change)
+    err = by_block(call(), want, held["v"], kind)
+    assert err.max() <= TOL[item], err
+
+
+@pytest.mark.parametrize("T", [1, 8, 130, 700])
+@pytest.mark.parametrize("window", [0, 300])
+@pytest.mark.parametrize("kind", ["q8_0", "q4_0"])
+def test_single_values_far_above_the_others(ocr, ctx, kind, window, T):
+    """a few positions whose first block is 2^20 (q8_0) times the others', at the start, inside and at the end: the other
+    blocks keep their own accuracy, whatever tile the large one lies in"""
+    d, held = 128, {}
+
+    def change(k, v):
+        v *= np.float32(2.0 ** -4)
+        for j in (3, 290, 700, 890):
+            v[:, j, :, :32] *= np.float32(2.0 ** (20 if kind == "q8_0" else 16))
+        held["v"] = v
+
+    call, want, _ = case(ocr, ctx, kind, "f32", (1, 2, 2, d, T, [900], window, 4 if window else 0, False, False), change=change)
+    err = by_block(call(), want, held["v"], kind)
+    assert err.max() <= TOL["f32"], err
