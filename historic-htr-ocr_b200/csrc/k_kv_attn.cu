@@ -20,8 +20,8 @@
 // for the 128-row tcgen05 shapes, and the operands here come out of registers, where the quants become f16 — no pass
 // through shared memory. Exactness: q8_0 and q4_0 quants are integers and exact in f16; a key's block scale multiplies
 // the block's f32 partial score, a value's block scale goes into P (one P per block of 32 dims). f32 queries, and P,
-// are split into f16 hi + lo (22 bits); f16 queries are exact, and P is rounded to f16 like the output. A row's query
-// is scaled by a power of two so that its lo part does not fall below f16's range, P likewise by the tile's largest
+// are split into f16 hi + lo (22 bits); f16 queries are exact, and P (times the scale) is rounded to f16 once, like the
+// output. A row's query is scaled by a power of two so that its lo part does not fall below f16's range, P likewise by the tile's largest
 // scale.
 #include "kv_tile.cuh"
 
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     const uint32_t h = pack2(p[i][2 * j], p[i][2 * j + 1]);
-                    if constexpr (sizeof(T) == 4) {
+                    if constexpr (sizeof(T) == 4 || TYPE != KV_F16) {  // (over quants the product with the scale is rounded)
                         const uint32_t r = rest2(p[i][2 * j], p[i][2 * j + 1], h);
                         if (PACK && TYPE == KV_F16) {
                             ph[i][j] = transpose8(t < 2 ? h : r);
@@ -358,11 +358,8 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
 #pragma unroll
                     for (int u = 0; u < 2; u++) {
                         const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&ph[i][u]));
-                        w[i][2 * u] = h.x, w[i][2 * u + 1] = h.y;
-                        if constexpr (sizeof(T) == 4) {
-                            const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&pl[i][u]));
-                            w[i][2 * u] += r.x, w[i][2 * u + 1] += r.y;
-                        }
+                        const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&pl[i][u]));
+                        w[i][2 * u] = h.x + r.x, w[i][2 * u + 1] = h.y + r.y;
                     }
 #pragma unroll
                     for (int u = 0; u < 4; u++) {

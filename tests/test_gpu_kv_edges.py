@@ -280,3 +280,31 @@ def test_single_values_far_above_the_others(ocr, ctx, kind, window, T):
     call, want, _ = case(ocr, ctx, kind, "f32", (1, 2, 2, d, T, [900], window, 4 if window else 0, False, False), change=change)
     err = by_block(call(), want, held["v"], kind)
     assert err.max() <= TOL["f32"], err
+
+
+@pytest.mark.parametrize("G", [2, 8, 64])  # whole numbers, warp-level products, tcgen05
+@pytest.mark.parametrize("kind", TYPES)
+def test_weights_of_f16_rows_are_rounded_once(ocr, ctx, kind, G):
+    """One position far above the others with values of zero, the others all alike: their weights' rounding errors are the
+    same and do not average out. One rounding to f16 is 2^-11 of the output, the output's own half a unit in its last
+    place; scores and sums in f32 add less than 10^-5."""
+    n_slot, n_kv, d, n = 12, 8, 128, 33
+    g = np.random.default_rng(17)
+    k, v = np.zeros((n_slot, n, n_kv, d), np.float32), np.zeros((n_slot, n, n_kv, d), np.float32)
+    k[:, 0, :, 0] = 4.0
+    v[:, 1:] = np.repeat(g.uniform(0.3, 3, (n_slot, 1, n_kv, d // 32)), 32, -1)
+    q = np.zeros((n_slot, 1, n_kv * G, d), np.float16)
+    q[..., 0] = g.uniform(0.2, 4, q.shape[:3])
+    cache = make_cache(ocr, kind, n_slot, n_kv, n, d)
+    put(ocr, ctx, cache, k, v, [0] * n_slot)
+    qd = torch.from_numpy(q).cuda()
+    out, ps = torch.zeros_like(qd), i32([n - 1] * n_slot)
+    torch.cuda.synchronize()
+    ocr.op_attention_window(ctx, cache, qd, out, ps, 0.5)
+    ctx.sync()
+    got = out.double().cpu().numpy()
+    for b in range(n_slot):
+        kb, vb = (torch.from_numpy(P.held(x[b], kind)).double().transpose(0, 1) for x in (k, v))
+        want = P.attend(torch.from_numpy(q[b]).double(), kb, vb, n - 1, 0.5).numpy()
+        half_ulp = np.spacing(np.abs(want).astype(np.float16)).astype(np.float64) / 2
+        assert (np.abs(got[b] - want) <= (2.0 ** -11 + 1e-5) * np.abs(want) + half_ulp).all()
