@@ -162,7 +162,8 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
             for (int s = 0; s < KSTEPS; s++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    qh[s][i] = pack2(x[4 * s + 2 * i], x[4 * s + 2 * i + 1]);
+                    qh[s][i] = sizeof(T) == 4 && TYPE == KV_F16 ? pack2_below(x[4 * s + 2 * i], x[4 * s + 2 * i + 1])
+                                                                : pack2(x[4 * s + 2 * i], x[4 * s + 2 * i + 1]);
                     if constexpr (PACK) {
                         const uint32_t lo = rest2(x[4 * s + 2 * i], x[4 * s + 2 * i + 1], qh[s][i]);
                         if (g >= 4) qh[s][i] = lo;

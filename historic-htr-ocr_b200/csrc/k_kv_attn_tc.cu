@@ -672,7 +672,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                 const uint32_t at = (byte >> 7) * (KC_M * 128) + kc_sw(r, (byte >> 4) & 7) + (byte & 15);
 #pragma unroll
                 for (int j = 0; j < V / 2; j++) {
-                    const uint32_t h = pack2(x[2 * j], x[2 * j + 1]);
+                    const uint32_t h = P::LO && !P::QN ? pack2_below(x[2 * j], x[2 * j + 1]) : pack2(x[2 * j], x[2 * j + 1]);
                     *reinterpret_cast<uint32_t*>(Qh + at + 4 * j) = h;
                     if constexpr (P::LO) *reinterpret_cast<uint32_t*>(Ql + at + 4 * j) = rest2(x[2 * j], x[2 * j + 1], h);
                 }

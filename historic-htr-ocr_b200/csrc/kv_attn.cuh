@@ -25,6 +25,14 @@ __device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t hi) {
     const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
     return pack2(a - h.x, b - h.y);
 }
+// A query's values a and b in f16 hi (→) + lo (rest2) whose products with an infinite key are infinities of one sign, as the
+// value's own: hi is rounded towards zero from a little less than the value, so lo is of its sign and not zero either
+// (values above 2^-24 of the row's largest, which is scaled to 2^10 … 2^11).
+__device__ __forceinline__ uint32_t pack2_below(float a, float b) {
+    uint32_t hi;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(__fmul_rz(b, 0.99999994f)), "f"(__fmul_rz(a, 0.99999994f)));
+    return hi;
+}
 // an unsigned byte pair placed as halves of 1024 + u, less `bias`
 __device__ __forceinline__ uint32_t bytes_h2(uint32_t w, uint32_t sel, uint32_t bias) {
     const uint32_t m = __byte_perm(w, 0x64646464u, sel);

@@ -349,9 +349,10 @@ ocr_status ocr_op_kv_read(ocr_ctx* ctx, const ocr_kv_cache* c, const ocr_rows* k
 /* softmax(q k^T * scale) v of the rows, which the cache already holds, over the positions each sees: up to its own,
  * within the window, the sinks. n_head query heads, head h reading kv head h / (n_head / n_kv). A row that
  * sees nothing gives zeros; what a row does not see has no part in it, not even a NaN. A NaN that a row sees, in a key
- * or a value, or an infinite value, leaves its output without a finite value there. At most 524288 (row, query head)
- * pairs of a kv head in one slot, and 10^9 (row, query head) pairs in all; a slot's blocks of 128 pairs times its blocks
- * of 128 keys, over its kv heads, stay below 2^31. */
+ * or a value, or an infinite value, leaves its output without a finite value there; an infinite key has no weight where
+ * the score is minus infinity, and leaves no finite value where it is infinity. At most 524288 (row, query head) pairs of a
+ * kv head in one slot, and 10^9 (row, query head) pairs in all; a slot's blocks of 128 pairs times its blocks of 128 keys,
+ * over its kv heads, stay below 2^31. */
 ocr_status ocr_op_attention_window(ocr_ctx* ctx, const ocr_kv_cache* c, const ocr_rows* q, int n_head, int rows,
                                    const int32_t* d_pos, const int32_t* d_n, float scale, const ocr_rows* out);
 /* the same for a tree of at most 64 drafted tokens per slot: row i, held at position d_pos + i, stands at position

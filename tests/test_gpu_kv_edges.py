@@ -308,3 +308,23 @@ def test_weights_of_f16_rows_are_rounded_once(ocr, ctx, kind, G):
         want = P.attend(torch.from_numpy(q[b]).double(), kb, vb, n - 1, 0.5).numpy()
         half_ulp = np.spacing(np.abs(want).astype(np.float16)).astype(np.float64) / 2
         assert (np.abs(got[b] - want) <= (2.0 ** -11 + 1e-5) * np.abs(want) + half_ulp).all()
+
+
+@pytest.mark.parametrize("T,G", [(1, 2), (3, 2), (1, 12), (8, 4), (130, 2), (700, 2)])
+@pytest.mark.parametrize("item", ["f32", "f16"])
+def test_infinite_keys(ocr, ctx, item, T, G):
+    """an infinite value in an f16 key, written as one or as a finite f32 beyond f16's range: a row whose query has the
+    other sign there gives the key no weight; one of the same sign has no finite output"""
+    def change(k, v):
+        k[0, 40, 0, 7] = np.inf
+        k[0, 41, 0, 9] = -np.inf
+        k[0, 300, 0, 7] = 1e5 if item == "f32" else np.inf
+        k[0, 401, 0, 70] = -1e30 if item == "f32" else -np.inf
+
+    with np.errstate(over="ignore"):
+        call, want, top = case(ocr, ctx, "f16", item, (1, 2, G, 128, T, [401], 0, 0, False, False), change=change)
+    got = call()
+    fine = torch.isfinite(want)
+    assert 0.05 < float(fine[..., 0].double().mean()) < 0.95
+    assert float((got - want)[fine].abs().max()) / top <= TOL[item]
+    assert not torch.isfinite(got[~fine]).any()
