@@ -30,11 +30,11 @@
 // is bounded: a role that gives up sets a flag and goes on without work, meeting every barrier, and no copy is in flight
 // (the staging is plain loads and stores).
 //
-// The sums in TMEM lose what falls below their last bit at every product added (about 1.7 10^-8 of a sum each time, towards
-// zero). For f32 rows a group adds its O to a sum of its own in memory after KcPlan::FLUSH tiles and starts O afresh —
-// between a tile's weights and the word that they are there, when the products of the tile before are nearly done. 666 rows
-// by 2214 f16 keys twice: errors of 1.6 10^-6 of the output instead of 2.3, for 6 us of 62. For f16 rows nothing is
-// moved: 40000 keys lose 4 10^-5 of a sum, a sixth of the output's rounding.
+// The sums in TMEM lose what falls below their last bit at every product added, towards zero: a million values of one size,
+// 31250 products, 2.9 10^-3 of their sum. For f32 rows a group adds its O to a sum of its own in memory after KcPlan::FLUSH
+// tiles and starts O afresh — between a tile's weights and the word that they are there, when the products of the tile
+// before are nearly done. 666 rows by 2214 f16 keys twice: errors of 1.6 10^-6 of the output instead of 2.3, for 6 us of 62.
+// For f16 rows a variant for long caches does so.
 //
 // The work: as in k_kv_attn.cu, the tiles of all (slot, row block, kv head) triples form a line cut evenly over the
 // SMs, triples in several CTAs joined by the last to arrive.
@@ -66,9 +66,10 @@ template <>
 struct KcWord<4> {
     using type = uint32_t;
 };
-template <int TYPE, int D, class T>
+template <int TYPE, int D, class T, bool LONG>
 struct KcPlan {
     static constexpr bool LO = sizeof(T) == 4, QN = TYPE != KV_F16;
+    static constexpr bool MOVES = LO || LONG;  // O is moved out of TMEM now and then
     static constexpr int NB = D / KV_BLOCK, ROW = kv_row_bytes(TYPE, D);
     static constexpr uint32_t Q_BYTES = KC_M * D * 2, T_BYTES = KC_KEYS * D * 2;  // one f16 operand of Q; of K or V
     static constexpr int PARTS = QN ? 2 : 1;                                      // hi (and lo) of K and V
@@ -76,8 +77,8 @@ struct KcPlan {
     static constexpr uint32_t SMEM = (LO ? 2 : 1) * Q_BYTES + 2 * NS * PARTS * T_BYTES + 1024;
     // a block's quants times its scale d (below 2^(e + 1)) times 2^(HEAD - e) just fit f16
     static constexpr int HEAD = TYPE == KV_Q8_0 ? 8 : 12;
-    // f32 rows: tiles between two moves of O, at most 64 products added to each of its sums in between
-    static constexpr int FLUSH = QN ? 5 : 8;
+    // tiles between two moves of O: at most 64 products are added to each of its sums in between, for f16 rows 256
+    static constexpr int FLUSH = LO ? QN ? 5 : 8 : QN ? 32 : 64;
     // the joined parts: [D][128] sums, [128] references, [128] weights' sums
     static constexpr int PART = (D + 2) * KC_M;
 };
@@ -281,9 +282,9 @@ struct KcRaw {
     }
 };
 
-template <int TYPE, int D, class T>
+template <int TYPE, int D, class T, bool LONG>
 __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_constant__ KvAttnArgs a, int blocks) {
-    using P = KcPlan<TYPE, D, T>;
+    using P = KcPlan<TYPE, D, T, LONG>;
     using Raw = KcRaw<TYPE, D>;
     constexpr int NS = P::NS;
     extern __shared__ uint8_t sm_raw[];
@@ -612,7 +613,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
 #pragma unroll 1
                 for (int i = -1; i < N && go; i++) {
                     if (i + 1 < N) go = qk(n + i + 1, i < 0);
-                    if (i >= 0) go = go && pv(n + i, P::LO ? i % P::FLUSH == 0 : i == 0);
+                    if (i >= 0) go = go && pv(n + i, P::MOVES ? i % P::FLUSH == 0 : i == 0);
                 }
                 n += N;
                 seg = seg_end;
@@ -750,7 +751,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
 #pragma unroll
                 for (int j = 0; j < HALF; j++) mq[j & 3] = fmaxf(mq[j & 3], __uint_as_float(s[j]));
                 const float mt = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) * fac;
-                const bool flush = P::LO && i > 0 && i % P::FLUSH == 0;
+                const bool flush = P::MOVES && i > 0 && i % P::FLUSH == 0;
                 const float m_was = m;
                 if (i == 0) {
                     m = mt;
@@ -869,7 +870,7 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
                     tmem_ld16(tmem + lanes + 256 + d, o);
                     tmem_ld16(tmem + lanes + 384 + d, o2);
                     float y[16] = {};
-                    if (P::LO && N > P::FLUSH) {
+                    if (P::MOVES && N > P::FLUSH) {
                         const float *k0 = kept - wg * D * KC_M, *k1 = k0 + D * KC_M;
                         const float ga = fa * sh.ml[0][2][r], gb = fb * sh.ml[1][2][r];
 #pragma unroll
@@ -957,18 +958,28 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
     }
 }
 
-template <int TYPE, int D, class T>
+template <int TYPE, int D, class T, bool LONG>
 static cudaError_t launch_tc(cudaStream_t st, const KvAttnArgs& a, int blocks, bool pdl) {
-    using P = KcPlan<TYPE, D, T>;
+    using P = KcPlan<TYPE, D, T, LONG>;
     static PerDeviceOnce once;
-    once([] { cudaFuncSetAttribute(k_kv_attn_tc<TYPE, D, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::SMEM); });
-    return kv_launch(k_kv_attn_tc<TYPE, D, T>, dim3(a.num_sms), KC_THREADS, P::SMEM, st, pdl, a, blocks);
+    once([] { cudaFuncSetAttribute(k_kv_attn_tc<TYPE, D, T, LONG>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)P::SMEM); });
+    return kv_launch(k_kv_attn_tc<TYPE, D, T, LONG>, dim3(a.num_sms), KC_THREADS, P::SMEM, st, pdl, a, blocks);
+}
+// the most keys that a row can see
+static long keys_of(const KvAttnArgs& a) {
+    return a.c.window ? min((long)a.c.n_rows, (long)a.c.window + a.c.sinks + a.r.T) : a.c.n_rows;
+}
+// f16 rows: keys from which sums are moved out of TMEM (1024 products to a sum: they may lose 10^-4 of it, two fifths of the
+// output's rounding). It takes code that all calls would pay for: 4 x 512 rows by 16.9k f16 keys 273 us, with it 301.
+static bool is_long(const KvAttnArgs& a) { return keys_of(a) > (a.c.type == KV_F16 ? 32768 : 16384); }
+template <int TYPE, int D>
+static cudaError_t launch_rows(cudaStream_t st, const KvAttnArgs& a, int blocks, bool pdl) {
+    if (!a.half) return launch_tc<TYPE, D, float, false>(st, a, blocks, pdl);
+    return is_long(a) ? launch_tc<TYPE, D, __half, true>(st, a, blocks, pdl) : launch_tc<TYPE, D, __half, false>(st, a, blocks, pdl);
 }
 template <int TYPE>
 static cudaError_t launch_type(cudaStream_t st, const KvAttnArgs& a, int blocks, bool pdl) {
-    if (a.c.d == 128)
-        return a.half ? launch_tc<TYPE, 128, __half>(st, a, blocks, pdl) : launch_tc<TYPE, 128, float>(st, a, blocks, pdl);
-    return a.half ? launch_tc<TYPE, 64, __half>(st, a, blocks, pdl) : launch_tc<TYPE, 64, float>(st, a, blocks, pdl);
+    return a.c.d == 128 ? launch_rows<TYPE, 128>(st, a, blocks, pdl) : launch_rows<TYPE, 64>(st, a, blocks, pdl);
 }
 // tickets, two parts for each CTA, the groups' sums (of heads of 128)
 size_t kv_attention_many_work(int num_sms) { return KV_TICKETS + (size_t)num_sms * 2 * ((128 + 2) + 128) * KC_M * 4; }
@@ -979,9 +990,8 @@ static int blocks_of(const KvAttnArgs& a) { return (int)(((long)a.r.T * (a.n_hea
 // even one slot's)
 int kv_attention_many_slots(const KvAttnArgs& a) {
     const KvView& c = a.c;
-    const long keys = c.window ? min((long)c.n_rows, (long)c.window + c.sinks + a.r.T) : c.n_rows;
     const int blocks = blocks_of(a);
-    const long tiles = (keys + KC_KEYS - 1) / KC_KEYS * c.n_kv * blocks;
+    const long tiles = (keys_of(a) + KC_KEYS - 1) / KC_KEYS * c.n_kv * blocks;
     return (int)min((long)(KV_LINE / blocks), 0x7fffffffL / tiles);
 }
 cudaError_t launch_kv_attention_many(cudaStream_t st, const KvAttnArgs& all, bool pdl) {

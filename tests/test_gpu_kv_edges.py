@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import kv_plain as P
-from test_gpu_kv import TOL, TYPES, case, i32, make_cache, put, sequences, tree
+from test_gpu_kv import ITEM, TOL, TYPES, case, i32, make_cache, put, sequences, tree
 
 pytestmark = pytest.mark.gpu
 
@@ -328,3 +328,29 @@ def test_infinite_keys(ocr, ctx, item, T, G):
     assert 0.05 < float(fine[..., 0].double().mean()) < 0.95
     assert float((got - want)[fine].abs().max()) / top <= TOL[item]
     assert not torch.isfinite(got[~fine]).any()
+
+
+@pytest.mark.parametrize("item", ["f32", "f16"])
+@pytest.mark.parametrize("kind", TYPES)
+def test_sums_over_a_million_keys(ocr, ctx, kind, item):
+    """Rows on the tensor cores, every triple in one CTA, values of one size: the output is the value. A sum in TMEM may lose
+    10^-7 of itself at each product; it is moved out after 64 (f32 rows) or 256 (f16 rows) of them: 6.4 10^-6, 2.6 10^-5.
+    With the sum of the weights, 10^-5 and 5 10^-5 are allowed, beside half a unit of the output in f16."""
+    n, T, G, d = 1_000_000, 148, 128, 64
+    cache = make_cache(ocr, kind, 1, 1, n + T, d)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for a in range(0, n + T, 1 << 17):
+        m = min(1 << 17, n + T - a)
+        k = torch.randn(1, m, 1, d, device="cuda", generator=g)
+        ps = i32([a])
+        torch.cuda.synchronize()
+        ocr.op_kv_write(ctx, cache, k, torch.ones_like(k), ps)
+        ctx.sync()
+    q = torch.randn(1, T, G, d, device="cuda", generator=g).to(ITEM[item])
+    out, ps = torch.zeros_like(q), i32([n])
+    torch.cuda.synchronize()
+    ocr.op_attention_window(ctx, cache, q, out, ps, 0.125)
+    ctx.sync()
+    one = float(P.held(np.ones((1, 32), np.float32), kind)[0, 0])  # (1, or a little less: half a unit is 2^-12)
+    assert one <= 1
+    assert float((out.double() - one).abs().max()) <= (2.0 ** -12 + 5e-5 if item == "f16" else 1e-5)
