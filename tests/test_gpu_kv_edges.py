@@ -10,6 +10,7 @@ import pytest
 import torch
 
 import kv_plain as P
+import test_gpu_kv as common
 from test_gpu_kv import ITEM, TOL, TYPES, case, i32, make_cache, put, sequences, tree
 
 pytestmark = pytest.mark.gpu
@@ -354,3 +355,37 @@ def test_sums_over_a_million_keys(ocr, ctx, kind, item):
     one = float(P.held(np.ones((1, 32), np.float32), kind)[0, 0])  # (1, or a little less: half a unit is 2^-12)
     assert one <= 1
     assert float((out.double() - one).abs().max()) <= (2.0 ** -12 + 5e-5 if item == "f16" else 1e-5)
+
+
+# ---- shapes between the kernels' ordinary ones ----
+BETWEEN = [  # (as test_gpu_kv.SHAPES) two rows of one head: whole numbers over quants
+    (2, 2, 1, 128, 2, [300, 5], 0, 0, False, False),
+    (2, 2, 1, 64, 2, [200, 77], 40, 3, False, False),
+    (1, 1, 1, 128, 2, [500], 33, 4, True, False),
+    (3, 2, 1, 128, 2, [260, -1, 0], 0, 0, False, True),
+    (2, 1, 1, 64, 2, [400, 90], 50, 5, False, True),
+    (1, 8, 1, 128, 2, [6000], 0, 0, False, False),
+    # five to eight pairs of several rows: one warp to a team, hi and lo in products of their own
+    (2, 2, 2, 128, 3, [310, 9], 0, 0, False, False),
+    (1, 2, 1, 64, 7, [150], 20, 2, False, False),
+    (2, 1, 4, 128, 2, [270, 31], 64, 4, True, False),
+    (2, 2, 1, 128, 6, [199, 0], 0, 0, False, True),
+    (1, 1, 1, 64, 8, [333], 30, 6, False, True),
+    (1, 8, 2, 128, 4, [5000], 0, 0, False, False),
+]
+
+
+@pytest.mark.parametrize("shape", BETWEEN, ids=lambda s: "-".join(map(str, s)).replace(" ", ""))
+@pytest.mark.parametrize("item", ["f32", "f16"])
+@pytest.mark.parametrize("kind", TYPES)
+def test_shapes_between(ocr, ctx, kind, item, shape):
+    call, want, top = case(ocr, ctx, kind, item, shape)
+    got = call()
+    assert float((got - want).abs().max()) / top <= TOL[item]
+    assert torch.equal(got, call())
+
+
+@pytest.mark.parametrize("shape", [s for s in BETWEEN if max(s[5]) < 1000], ids=lambda s: "-".join(map(str, s)).replace(" ", ""))
+@pytest.mark.parametrize("kind", TYPES)
+def test_what_rows_of_these_shapes_do_not_see(ocr, ctx, kind, shape):
+    common.test_what_a_row_does_not_see_has_no_part(ocr, ctx, kind, shape)
