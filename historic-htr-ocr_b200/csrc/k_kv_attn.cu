@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(KA_THREADS, 1) k_kv_attn(const __grid_constant
         sp.set(a, line.pos[cc.b], line.m[cc.b], 0, a.r.T);
         const int seg_end = min(end, cc.first + cc.tiles);
         const int rows = sp.m * G;
-        const bool many = a.r.T > 1;
+        const bool many = a.r.T > 1 || a.parent;  // (else every row sees the whole span)
         // ---- what each row sees ----
         if (many) {
             if (a.parent) {

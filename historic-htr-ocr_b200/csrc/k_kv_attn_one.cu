@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(KO_THREADS, 1) k_kv_attn_one(const __grid_cons
         cc.at(seg, line.prefix, c.n_slot, c.n_kv);
         sp.set(a, line.pos[cc.b], line.m[cc.b], 0, a.r.T);
         const int seg_end = min(end, cc.first + cc.tiles), rows = sp.m * G;
-        const bool many = a.r.T > 1;
+        const bool many = a.r.T > 1 || a.parent;  // (else every row sees the whole span)
         if (many) {
             if (a.parent) {
                 if (tid < sp.m) s_parent[tid] = a.parent[(size_t)cc.b * a.r.T + tid];

@@ -389,3 +389,23 @@ def test_shapes_between(ocr, ctx, kind, item, shape):
 @pytest.mark.parametrize("kind", TYPES)
 def test_what_rows_of_these_shapes_do_not_see(ocr, ctx, kind, shape):
     common.test_what_a_row_does_not_see_has_no_part(ocr, ctx, kind, shape)
+
+
+@pytest.mark.parametrize("G", [1, 4])
+@pytest.mark.parametrize("kind", TYPES)
+def test_a_tree_of_one_draft(ocr, ctx, kind, G):
+    """it sees what a row sees, and its parent is looked at as in any tree"""
+    cache = make_cache(ocr, kind, 2, 1, 300, 128, window=100, sinks=3)
+    k, v = sequences(44, 2, 300, 1, 128)
+    put(ocr, ctx, cache, k, v, [0, 0])
+    q = torch.randn(2, 1, G, 128, device="cuda")
+    out, want, ps = torch.zeros_like(q), torch.zeros_like(q), i32([299, 50])
+    good, bad = i32([[-1], [-1]]), i32([[-1], [0]])
+    torch.cuda.synchronize()
+    ocr.op_attention_window(ctx, cache, q, want, ps, 0.09)
+    ocr.op_attention_tree(ctx, cache, q, out, ps, good, 0.09)
+    ctx.sync()
+    assert float((out - want).abs().max()) <= TOL["f32"] * float(np.abs(P.held(v, kind)).max())
+    ocr.op_attention_tree(ctx, cache, q, out, ps, bad, 0.09)
+    with pytest.raises(ocr.OcrError, match="index outside"):
+        ctx.sync()
