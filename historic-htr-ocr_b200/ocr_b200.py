@@ -796,9 +796,12 @@ _KV_ITEM = {1: 2.0, 2: 0.5, 8: 1.0}
 
 def _device_of(t, device: Optional[int] = None) -> int:
     """the GPU that a tensor is on (device: the one it has to be on); the kernels take its address as device memory"""
-    if not getattr(t, "is_cuda", False):
+    try:
+        at = t.get_device()
+    except AttributeError:
+        at = -1
+    if at < 0:
         raise OcrError(1, f"the KV operators take device tensors, not {type(t).__name__} in host memory")
-    at = t.get_device()
     if device is not None and at != device:
         raise OcrError(1, f"a tensor on GPU {at}, its KV cache on GPU {device}")
     return at

@@ -12,7 +12,7 @@ class Claims:
     """a host tensor that says that it is on GPU `index`"""
 
     def __init__(self, t, index=0):
-        self.t, self.is_cuda, self.index = t, True, index
+        self.t, self.index = t, index
 
     def get_device(self):
         return self.index
