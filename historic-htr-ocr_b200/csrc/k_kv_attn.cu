@@ -27,8 +27,9 @@
 
 namespace ocr {
 
-// (row, query head) pairs of a kv head up to which this kernel runs: at 16 (32 slots, 8 drafts) 140 us against 263 in
-// k_kv_attn_tc.cu, at 32 (one slot, 16 drafts) 44 against 58; more would need more than four warps to a team
+// (row, query head) pairs of a kv head up to which this kernel runs. In this kernel and in k_kv_attn_tc.cu: 16 pairs (a step of 32
+// slots, 8 drafts, q8_0) 148 and 243 us; 32 pairs, one slot (a step of 16 drafts) 45 and 51; 32 pairs, 32 slots x 16 rows, 199 and
+// 225 over q8_0, 175 and 195 over f16. More would need more than four warps to a team.
 constexpr int KA_ROWS = 32;
 constexpr int KA_WARPS = 12;
 constexpr int KA_THREADS = KA_WARPS * 32;

@@ -4,9 +4,9 @@
 // A CTA takes 128 (row, query head) pairs of a kv head (the pairs of a row side by side, so K and V are read once for
 // the whole group) against the keys that any of them sees, in tiles of 128 keys. Floor: the tensor cores. What bounds it now
 // is the chain S → P → O of one triple (one fits an SM) with the softmax's instructions and the issuing thread's waits in it:
-// before the products were issued by an elected thread (307, 72 and 234 us below) the tensor pipe was 16 to 20 % busy, issue
-// 32 to 42 %. Measured: 512 f16 rows by 16896 f16 keys, 16 heads of 64, four slots: 273 us, 386 TFLOP/s; 2214 f32 rows
-// in a window of 512, q8_0, 16 heads of 128: 66 us; 8 trees of 61 drafts in windows of 8192, q4_0, f16 rows, 32 heads: 218 us.
+// the tensor pipe is 19 to 33 % busy, issue 36 to 49 % (the three calls below). Measured: 512 f16 rows by 16896 f16 keys, 16
+// heads of 64, four slots: 273 us, 386 TFLOP/s; 2214 f32 rows in a window of 512, q8_0, 16 heads of 128: 66 us; 8 trees of 61
+// drafts in windows of 8192, q4_0, f16 rows, 32 heads: 218 us.
 //
 // Products: S = Q K^T (M = N = 128, both operands in shared memory), O += P V (A = P in TMEM, written over S in place;
 // B = V in shared memory, MN-major), f16 operands, f32 sums in TMEM. Exactness: f32 queries and P are f16 hi + lo (22 bits);
@@ -161,7 +161,7 @@ __device__ __forceinline__ bool bar_any(int id, int threads, bool mine) {
     return any != 0;
 }
 
-// ---- the staging of a tile, by 256 threads: raw rows to registers, later to operands ------------------------------------
+// ---- the staging of a tile, by 224 threads: raw rows to registers, later to operands ------------------------------------
 // K and V alike: rows of 64 dims (128 bytes, swizzled) in D / 64 halves of 128 keys — K is read along the dims (K-major),
 // V along the keys (MN-major), from the same layout. A warp's load covers four whole 128-byte lines; the lanes stand so
 // that the eight of a store's phase (one or more keys, units side by side) meet all eight 16-byte pieces of a row.
@@ -378,9 +378,9 @@ __global__ void __launch_bounds__(KC_THREADS, 1) k_kv_attn_tc(const __grid_const
     cut.cut(total, n_cta);
     int begin, end;
     // Even parts cut most triples in two, and each piece costs the time of some KC_PIECE tiles beside its own (the
-    // queries staged, the sums joined); whole ones leave SMs idle. 2214 rows in a window of 512 (280 triples of 6
-    // tiles on 148 SMs): 72 us whole, 129 cut; 666 pairs by 2214 keys twice (96 of 18): 62 and 71; 2048 by 16896
-    // keys four times (256 of 132): 422 and 299. (Before sums of f32 rows were moved out of TMEM.)
+    // queries staged, the sums joined); whole ones leave SMs idle. 2214 rows in a window of 512 (280 triples of at most
+    // five tiles on 148 SMs): 66 us whole, 121 cut; 666 pairs by 2214 keys twice (96 triples of 8 to 18): 62 and 66; 2048 by
+    // 16896 keys four times (256 of 65 to 132): 405 and 272; 8 trees of 61 drafts (128 of 65): 213 and 218.
     kv_share(cut, cta, sh.prefix, entries, c.n_kv, total, sh.longest, (int)gridDim.x, KC_PIECE, KC_PIECE / 2, begin, end);
     KvCursor cc;
     bool any_mma = false;  // (the issuing thread)

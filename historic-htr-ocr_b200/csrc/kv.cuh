@@ -1,5 +1,6 @@
 // kv.cuh — one layer's KV cache in f16, q8_0 or q4_0, as the kernels see it (ocr_kv_cache, include/ocr_cuda.h), and the
-// launchers of the operators over it: rows written and read back (k_kv_cache.cu), the attentions (k_kv_attn.cu).
+// launchers of the operators over it: rows written, read back and moved (k_kv_cache.cu), the attentions (k_kv_attn.cu,
+// k_kv_attn_one.cu, k_kv_attn_tc.cu).
 //
 // Layout, per tensor (K and V alike): quants [n_slot][n_kv][n_rows][row bytes], scales [n_slot][n_kv][n_rows][d / 32]
 // f16. Offsets are 64-bit: a long cache passes 2^31 bytes. A position p of a slot lives in row p; in a ring cache the
@@ -112,7 +113,7 @@ inline KvAttnArgs kv_slots(const KvAttnArgs& all, int b, int n) {
 }
 cudaError_t launch_kv_attention(cudaStream_t st, const KvAttnArgs& a, bool pdl);
 // (row, query head) pairs of a kv head up to which k_kv_attn_one.cu serves a quantised cache: with 2, 32 slots of some 3100
-// keys in q8_0 take 55 us there and 73 in k_kv_attn.cu, in a q4_0 ring of 1028 keys 32 and 41 (cut evenly). Its digits take
+// keys in q8_0 take 55 us there and 73 in k_kv_attn.cu, in a q4_0 ring of 1028 keys 25 and 34. Its digits take
 // four columns of eight a pair, so two pairs are what one product holds.
 constexpr int KV_ONE_ROWS = 2;
 cudaError_t launch_kv_attention_one(cudaStream_t st, const KvAttnArgs& a, bool pdl);

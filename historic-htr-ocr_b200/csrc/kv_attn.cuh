@@ -1,6 +1,6 @@
-// kv_attn.cuh — what the two attentions over a KV cache share (k_kv_attn.cu: a few rows per kv head; k_kv_attn_tc.cu:
-// many): the line of key tiles that is cut evenly over the CTAs, the positions that a range of rows sees, the quants'
-// way to f16.
+// kv_attn.cuh — what the three attentions over a KV cache share (k_kv_attn_one.cu, k_kv_attn.cu: a few rows per kv head;
+// k_kv_attn_tc.cu: many): the line of key tiles that is cut evenly over the CTAs, the positions that a range of rows sees,
+// the quants' way to f16.
 #pragma once
 
 #include "kv.cuh"

@@ -1,5 +1,5 @@
 // kv_ops.cu — the C ABI of the operators over a caller's KV cache (include/ocr_cuda.h): argument checks, workspaces and
-// launches. The kernels are in k_kv_cache.cu and k_kv_attn.cu.
+// launches. The kernels are in k_kv_cache.cu, k_kv_attn.cu, k_kv_attn_one.cu and k_kv_attn_tc.cu.
 #include "ctx.h"
 #include "kv.cuh"
 

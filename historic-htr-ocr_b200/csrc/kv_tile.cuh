@@ -53,7 +53,7 @@ __device__ __forceinline__ void cp_wait() {
 }
 // Short pairs are taken whole: a pair costs the time of some KA_PIECE tiles beside its own (queries, the teams joined), as
 // much again where it is cut (parts written, counted, joined). 32 slots, 8 kv heads, a window of 1024 in q4_0 (256 pairs
-// of 33 tiles): 25 us whole, 33 cut.
+// of 33 tiles): 25 us whole, 32 cut.
 constexpr int KA_PIECE = 14;
 struct KaLine {
     int prefix[KA_LINE + 1], pos[KA_LINE], m[KA_LINE];  // of the slots: tiles before, position, rows in use

@@ -338,8 +338,8 @@ ocr_status ocr_session_kv_cache(const ocr_session* s, int layer, ocr_kv_cache* o
  * takes up to n_rows). */
 /* rows of keys and values → the cache, quantised per block of 32 as ggml's reference quantisers do: q8_0 with
  * scale = f16(max|x| / 127) and q = x / scale before its rounding to f16, to the nearest, halves away from zero; q4_0
- * with scale = f16(m / -8), m the first value of the largest magnitude. A block with an infinity or a NaN, or whose
- * scale passes f16's range, reads back as NaN. */
+ * with scale = f16(m / -8), m the first value of the largest magnitude. A block whose scale rounds to zero is stored as
+ * zeros; a block with an infinity or a NaN, or whose scale passes f16's range, reads back as NaN. */
 ocr_status ocr_op_kv_write(ocr_ctx* ctx, const ocr_kv_cache* c, const ocr_rows* k, const ocr_rows* v, int rows,
                            const int32_t* d_pos, const int32_t* d_n);
 /* the cache's rows → values. Of a ring cache the rows as they are now: those of a position that has left it hold a later
